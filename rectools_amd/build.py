@@ -16,7 +16,8 @@ CSRC = os.path.join(PKG_DIR, "csrc")
 LIB_PATH = os.path.join(PKG_DIR, "librectools_hip.so")
 OBJ_DIR = os.path.join(CSRC, "_obj")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wno-unused-result"]
+# (no packed fp32 instructions: some of their forms have given wrong results on this hardware; the host pass warns that it does not know the feature)
+FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wno-unused-result", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 FLAGS += os.environ.get("RT_EXTRA_HIPCC_FLAGS", "").split()   # diagnostic builds (e.g. -DRT_ATTN_TRACE); part of the digests
 
 

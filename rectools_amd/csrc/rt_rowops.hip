@@ -263,6 +263,17 @@ __device__ __forceinline__ f32x4 ln_keep_cols(f32x4 v, int c, int grp, int grp_r
   v[2] = r + 2 < grp_real ? v[2] : 0.f;  v[3] = r + 3 < grp_real ? v[3] : 0.f;
   return v;
 }
+// a . b of four columns, the products rounded before they are added: what the row statistics have always been (a contraction to fused
+// multiply-adds is the compiler's choice and moves last bits; here it has none)
+__device__ __forceinline__ f32x4 mul4_rounded(const f32x4& a, const f32x4& b) {
+#pragma clang fp contract(off)
+  return a * b;
+}
+__device__ __forceinline__ float dot4_rounded(const f32x4& a, const f32x4& b) {
+#pragma clang fp contract(off)
+  const f32x4 p = a * b;
+  return p[0] + p[1] + p[2] + p[3];
+}
 template <bool COLS = false>
 __global__ __launch_bounds__(256) void layernorm_fwd_kernel(const float* __restrict__ x, const float* __restrict__ w,
                                                             const float* __restrict__ b, float eps, int M, int d,
@@ -291,7 +302,7 @@ __global__ __launch_bounds__(256) void layernorm_fwd_kernel(const float* __restr
     f32x4 v = pad ? zero4 : *reinterpret_cast<const f32x4*>(xr + c);
     v -= mu;
     if (COLS) v = ln_keep_cols(v, c, grp, grp_real);
-    q += v[0] * v[0] + v[1] * v[1] + v[2] * v[2] + v[3] * v[3];
+    q += dot4_rounded(v, v);
   }
   const float rs = 1.0f / sqrtf(wave_sum(q) / n_cols + eps);
   for (int c = lane * 4; c < d; c += 256) {
@@ -366,9 +377,12 @@ __global__ __launch_bounds__(256) void layernorm_bwd_kernel(const float* __restr
         f32x4 z = {0.f, 0.f, 0.f, 0.f};
         xh[u][i] = (c < d) ? (xh[u][i] - mu[u]) * rs[u] : z;
         if (COLS && c < d) xh[u][i] = ln_keep_cols(xh[u][i], c, grp, grp_real);
-        f32x4 gw = g[u][i] * wv[i];
+        const f32x4 gw = (NDV == 1 && !COLS) ? mul4_rounded(g[u][i], wv[i]) : g[u][i] * wv[i];
         s1[u] += gw[0] + gw[1] + gw[2] + gw[3];
-        s2[u] += gw[0] * xh[u][i][0] + gw[1] * xh[u][i][1] + gw[2] * xh[u][i][2] + gw[3] * xh[u][i][3];
+        // (up to 256 columns the second row's products are fused: the bits of this pass are kept as they have been)
+        s2[u] += (NDV == 1 && !COLS && u == 1)
+                     ? fmaf(gw[3], xh[u][i][3], fmaf(gw[2], xh[u][i][2], fmaf(gw[0], xh[u][i][0], gw[1] * xh[u][i][1])))
+                     : dot4_rounded(gw, xh[u][i]);
       }
 #pragma unroll
     for (int u = 0; u < 2; ++u) { s1[u] = wave_sum(s1[u]) / n_cols; s2[u] = wave_sum(s2[u]) / n_cols; }
@@ -725,7 +739,7 @@ __global__ __launch_bounds__(256) void embed_block1_kernel(EmbedBlock1Args a) {
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int c = lane * 4 + 256 * i;
-    if (c < d) { const f32x4 v = x[i] - mu; q2 += v[0] * v[0] + v[1] * v[1] + v[2] * v[2] + v[3] * v[3]; }
+    if (c < d) { const f32x4 v = x[i] - mu; q2 += NV > 1 ? dot4_rounded(v, v) : v[0] * v[0] + v[1] * v[1] + v[2] * v[2] + v[3] * v[3]; }
   }
   const float rs = 1.0f / sqrtf(wave_sum(q2) / d + a.eps);      // (layernorm_fwd_kernel's own two passes)
   if (PLN > 0) {
