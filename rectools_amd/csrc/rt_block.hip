@@ -138,14 +138,10 @@ Side* side_of_current_device() {
   if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 16) return nullptr;
   Side& s = g_side[dev];
   if (s.stream == nullptr) {
-    // LOW priority: what runs here is needed by the optimiser only.  At equal priority the dispatcher keeps refilling the CUs' wave slots
-    // with the side stream's small-footprint workgroups (the loss's row reductions: 8 waves per SIMD) and a main-stream kernel that needs
-    // a whole CU's LDS waits for a slot: v2_bwd_dq 227 us instead of 67 beside sampled_bwd_rows (profiles/r4_timeline_train.txt).
-    // RT_SIDE_PRIORITY=normal keeps the default priority.
-    const char* e = getenv("RT_SIDE_PRIORITY");
-    int least = 0, greatest = 0;
-    const bool low = (e == nullptr || e[0] != 'n') && hipDeviceGetStreamPriorityRange(&least, &greatest) == hipSuccess && least != greatest;
-    const hipError_t rc = low ? hipStreamCreateWithPriority(&s.stream, hipStreamNonBlocking, least) : hipStreamCreateWithFlags(&s.stream, hipStreamNonBlocking);
+    // Default priority, as every stream here: work on streams of different priorities has hung on this hardware.  (At equal priority the
+    // dispatcher keeps refilling the CUs' wave slots with this stream's small-footprint workgroups, and a main-stream kernel that needs a
+    // whole CU's LDS can wait for a slot.)
+    const hipError_t rc = hipStreamCreateWithFlags(&s.stream, hipStreamNonBlocking);
     if (rc != hipSuccess) return nullptr;
     (void)hipEventCreateWithFlags(&s.fork, hipEventDisableTiming);
     (void)hipEventCreateWithFlags(&s.join, hipEventDisableTiming);
