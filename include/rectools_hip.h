@@ -740,6 +740,57 @@ int rt_dp_allgather(void* comm, const float* send, float* recv, int64_t n, rt_st
 int rt_dp_finalize(void* comm);
 const char* rt_dp_last_error(void);
 
+/* ------------------------------------------------------------------------------------------------
+ * Operators of a differential-attention layer stack (`nn.DifferentialTransformerLayers`; the reference has no counterpart)
+ * ------------------------------------------------------------------------------------------------ */
+/* Rotary positions of n_heads q heads and n_kv_heads k heads (either may be 0) of hd columns in one launch: the pairs of a head's first
+ * `rot` (even) columns turn by pos[row] * freq[j] radians and are scaled by `gain`, the columns behind are copied.  interleaved: pair j =
+ * columns (2 j, 2 j + 1), else (j, j + rot / 2).  freq: rot / 2 doubles; angles are formed and reduced in 64 bits.  backward = 1: the
+ * transposed map (gradients in, gradients out).  In and out rows may be strided (ld >= heads * hd); out may be the input. */
+int rt_rotary(const float* q, int64_t ldq, float* q_out, int64_t ldq_out, int32_t n_heads, const float* k, int64_t ldk, float* k_out,
+              int64_t ldk_out, int32_t n_kv_heads, const int64_t* pos, const double* freq, int64_t M, int32_t hd, int32_t rot,
+              int32_t interleaved, float gain, int32_t backward, rt_stream_t stream);
+
+/* lam[h] = exp(q1[h] . k1[h]) - exp(q2[h] . k2[h]) + init over [H, hd] vectors, and its backward */
+int rt_diff_lambda_fwd(const float* q1, const float* k1, const float* q2, const float* k2, float init, int32_t H, int32_t hd, float* lam,
+                       rt_stream_t stream);
+int rt_diff_lambda_bwd(const float* dlam, const float* q1, const float* k1, const float* q2, const float* k2, int32_t H, int32_t hd, float* dq1,
+                       float* dk1, float* dq2, float* dk2, rt_stream_t stream);
+
+/* Differential attention: o = (softmax(scale q1 k1^T) - lam_h softmax(scale q2 k2^T)) v, y = out_scale * norm_w * o / sqrt(mean(o^2) + eps)
+ * (norm_w null: y = out_scale * o).  q [Nq, H][2][hd], k [Nk, Hkv][2][hd], v [Nk, Hkv][2 hd], y [Nq, H][2 hd] (row strides ld*); query head h
+ * reads key head h / (H / Hkv); hd <= 64.  cu_q / cu_k [B+1] (first 0, ascending): first row of every session, or null: B sessions of Lq / Lk
+ * rows (then Nq == B * Lq, Nk == B * Lk).  With cu, Lq / Lk are the expected longest sessions (longer ones are served all the same).  The last
+ * query of a session is aligned with its last key: causal = key j is seen by query i iff j <= i + nk - nq.  key_ids (null or [Nk]): keys with id 0
+ * are masked.  A query that sees no key gives 0.  scale <= 0: 1 / sqrt(hd).  Rows behind the last session of cu_q are written as zeros.
+ * o12 [Nq, H, 2, 2 hd] and lse [Nq, H, 2]: both or neither; what the backward pass reads.  ws: rt_diffattn_fwd_workspace_bytes(train = o12 given). */
+size_t rt_diffattn_fwd_workspace_bytes(int32_t B, int32_t H, int32_t Hkv, int32_t hd, int32_t Lq, int32_t Lk, int64_t Nq, int32_t train);
+int rt_diffattn_fwd(const float* q, int64_t ldq, const float* k, int64_t ldk, const float* v, int64_t ldv, const float* lam, const int64_t* cu_q,
+                    const int64_t* cu_k, const int64_t* key_ids, int32_t B, int32_t H, int32_t Hkv, int32_t hd, int32_t Lq, int32_t Lk, int64_t Nq,
+                    int64_t Nk, float scale, int32_t causal, const float* norm_w, float out_scale, float eps, float* y, int64_t ldy, float* o12,
+                    float* lse, void* ws, size_t ws_bytes, rt_stream_t stream);
+/* Gradients of q, k, v, lam and norm_w (dw null iff norm_w null) from dy; every element of dq, dk, dv, dlam, dw is written. */
+size_t rt_diffattn_bwd_workspace_bytes(int32_t H, int32_t hd, int64_t Nq);
+int rt_diffattn_bwd(const float* q, int64_t ldq, const float* k, int64_t ldk, const float* v, int64_t ldv, const float* lam, const int64_t* cu_q,
+                    const int64_t* cu_k, const int64_t* key_ids, int32_t B, int32_t H, int32_t Hkv, int32_t hd, int32_t Lq, int32_t Lk, int64_t Nq,
+                    int64_t Nk, float scale, int32_t causal, const float* norm_w, float out_scale, float eps, const float* o12, const float* lse,
+                    const float* dy, int64_t lddy, float* dq, int64_t lddq, float* dk, int64_t lddk, float* dv, int64_t lddv, float* dlam,
+                    float* dw, void* ws, size_t ws_bytes, rt_stream_t stream);
+
+/* The norm behind a block, its gate, its residual scale and the norm in front of the next block: n = N_post(f), y = alpha x + scale * sigmoid(z) *
+ * drop(n), h = N_pre(y) over contiguous [M, d] rows, d <= 8192.  layer = 1: LayerNorm, 0: root mean square.  post_w / pre_w null: that norm is left
+ * out (h null iff pre_w null); post_b, pre_b, z, scale null: left out.  p, seed, stream_id: the dropout mask of rt_act_dropout_*.  stat [M, 4]
+ * (16-byte aligned, null without a backward pass): the norms' statistics.  Backward: gy / gh may be null (no gradient); dscale .. dpre_b: the ones that
+ * are asked for. */
+int rt_norm_gate_fwd(const float* x, const float* f, const float* z, const float* scale, const float* post_w, const float* post_b, const float* pre_w,
+                     const float* pre_b, int32_t layer, float alpha, float eps, float p, uint64_t seed, uint64_t stream_id, int64_t M, int32_t d, float* y,
+                     float* h, float* stat, rt_stream_t stream);
+size_t rt_norm_gate_bwd_workspace_bytes(int64_t M, int32_t d);
+int rt_norm_gate_bwd(const float* gy, const float* gh, const float* y, const float* f, const float* z, const float* scale, const float* post_w,
+                     const float* post_b, const float* pre_w, int32_t layer, float alpha, float p, uint64_t seed, uint64_t stream_id, int64_t M, int32_t d,
+                     const float* stat, float* dx, float* df, float* dz, float* dscale, float* dpost_w, float* dpost_b, float* dpre_w, float* dpre_b,
+                     void* ws, size_t ws_bytes, rt_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

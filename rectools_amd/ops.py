@@ -2530,3 +2530,322 @@ def softmax_loss(sess: torch.Tensor, table: torch.Tensor, act_idx: torch.Tensor,
                  logits_t: float) -> torch.Tensor:
     """sess [M,d] (already L2-normalised for cosine), table [V,d]; act_idx = positions with y != 0 (int64, ascending)."""
     return _SoftmaxLoss.apply(sess, table, act_idx, y_act, w_act, logits_t, sess.shape[0])
+
+
+# --------------------------------------------------------------------------------------------------
+# a differential-attention stack's operators: rotary positions, differential attention, norms with gate and residual scale
+# --------------------------------------------------------------------------------------------------
+def _rows(t: torch.Tensor, what: str, cols: tp.Optional[int] = None) -> torch.Tensor:
+    """A float32 HIP matrix whose rows the kernels can read in place: unit column stride, rows that do not overlap; else a copy."""
+    _chk(t, what)
+    if t.dim() != 2 or (cols is not None and t.shape[1] != cols):
+        raise ValueError(f"{what}: expected [rows, {'columns' if cols is None else cols}], got {tuple(t.shape)}")
+    if t.shape[1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+        t = t.contiguous()
+    return t
+
+
+def _ld(t: torch.Tensor) -> int:
+    return int(t.stride(0)) if t.shape[0] > 1 else int(t.shape[1])
+
+
+def _same_device(what: str, first: torch.Tensor, *others: tp.Optional[torch.Tensor]) -> None:
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"{what}: tensors on {first.device} and {t.device}")
+
+
+def _ints(t: tp.Optional[torch.Tensor], what: str, n: int) -> tp.Optional[torch.Tensor]:
+    if t is None:
+        return None
+    if t.dtype != torch.int64 or not t.is_cuda or t.dim() != 1 or t.shape[0] != n:
+        raise ValueError(f"{what}: expected {n} int64 values on the HIP device, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    return t.contiguous()
+
+
+def _needs_tape(*tensors: tp.Optional[torch.Tensor]) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def rotary_frequencies(rot: int, base: float = 10_000.0, scaling: str = "none", factor: float = 1.0, trained_len: int = 4096,
+                       device: tp.Optional[tp.Any] = None) -> tp.Tuple[torch.Tensor, float]:
+    """-> (radians per position of the rot / 2 pairs, float64; gain) for `rotary` / `rotary_qk`.  f_j = base^(-2 j / rot), and for sessions
+    longer than the trained ones by `factor`: "linear" divides every frequency by it (Chen et al. 2023, position interpolation); "base"
+    raises the base so that the slowest pair is stretched by it and the fastest kept; "parts" (Peng et al. 2023) keeps pairs that turn 32
+    times and more within `trained_len`, divides pairs that turn less than once, with a linear ramp between, and gain = 0.1 ln(factor) + 1."""
+    if rot <= 0 or rot % 2 != 0:
+        raise ValueError(f"rotary_frequencies: the rotated columns come in pairs, got rot={rot}")
+    if scaling not in ("none", "linear", "base", "parts"):
+        raise ValueError(f"rotary_frequencies: scaling is 'none', 'linear', 'base' or 'parts', got {scaling!r}")
+    if not factor >= 1.0 or not base > 1.0 or trained_len <= 0:
+        raise ValueError(f"rotary_frequencies: factor >= 1, base > 1 and trained_len > 0, got {factor}, {base}, {trained_len}")
+    j = torch.arange(rot // 2, dtype=torch.float64)
+    if scaling == "base" and rot > 2:
+        base = base * factor ** (rot / (rot - 2))
+    f = base ** (-2.0 * j / rot)
+    gain = 1.0
+    if scaling == "linear":
+        f = f / factor
+    elif scaling == "parts":
+        keep = ((trained_len * f / (2.0 * math.pi) - 1.0) / 31.0).clamp(0.0, 1.0)
+        f = f * keep + f / factor * (1.0 - keep)
+        gain = 0.1 * math.log(factor) + 1.0
+    return f.to(device) if device is not None else f, gain
+
+
+def _rotary_call(tensors: tp.Sequence[tp.Tuple[tp.Optional[torch.Tensor], int]], pos, freq, hd: int, interleaved: bool, gain: float,
+                 backward: bool) -> tp.List[tp.Optional[torch.Tensor]]:
+    args: tp.List[tp.Any] = []
+    outs: tp.List[tp.Optional[torch.Tensor]] = []
+    for x, heads in tensors:
+        if x is None:
+            args += [None, 0, None, 0, 0]
+            outs.append(None)
+            continue
+        y = torch.empty(tuple(x.shape), dtype=torch.float32, device=x.device)
+        args += [x, _ld(x), y, int(y.shape[1]), heads]
+        outs.append(y)
+    with torch.cuda.device(pos.device):
+        _c("rt_rotary", *args, pos, freq, int(pos.shape[0]), hd, 2 * int(freq.shape[0]), int(interleaved), float(gain), int(backward))
+    return outs
+
+
+class _Rotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, pos, freq, n_heads, n_kv_heads, hd, interleaved, gain):
+        ctx.save_for_backward(pos, freq)
+        ctx.meta = (n_heads, n_kv_heads, hd, interleaved, gain)
+        ctx.set_materialize_grads(False)
+        q2, k2 = _rotary_call([(q, n_heads), (k, n_kv_heads)], pos, freq, hd, interleaved, gain, False)
+        return q2 if k is None else (q2, k2)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gq, gk=None):
+        pos, freq = ctx.saved_tensors
+        n_heads, n_kv_heads, hd, interleaved, gain = ctx.meta
+        if gq is None and gk is None:
+            return (None,) * 9
+        gq, gk = (None if g is None else _rows(g, "rotary gradient") for g in (gq, gk))
+        dq, dk = _rotary_call([(gq, n_heads), (gk, n_kv_heads)], pos, freq, hd, interleaved, gain, True)
+        return (dq, dk) + (None,) * 7
+
+
+def _rotary_args(q, k, pos, freq, n_heads, n_kv_heads):
+    if n_heads <= 0 or (k is not None and n_kv_heads <= 0):
+        raise ValueError(f"rotary: head counts must be positive, got {n_heads} and {n_kv_heads}")
+    q = _rows(q, "rotary")
+    M, cols = q.shape
+    if cols % n_heads != 0 or cols == 0:
+        raise ValueError(f"rotary: {cols} columns do not split into {n_heads} heads")
+    hd = cols // n_heads
+    if k is not None:
+        k = _rows(k, "rotary", n_kv_heads * hd)
+        if k.shape[0] != M:
+            raise ValueError(f"rotary: {M} query rows and {k.shape[0]} key rows")
+    pos = _ints(pos, "rotary positions", M)
+    if freq.dtype != torch.float64 or freq.dim() != 1 or not freq.is_cuda or not 0 < 2 * int(freq.shape[0]) <= hd:
+        raise ValueError(f"rotary: expected at most {hd // 2} float64 frequencies on the HIP device (rotary_frequencies), got {freq.dtype} "
+                         f"{tuple(freq.shape)} on {freq.device}")
+    _same_device("rotary", q, k, pos, freq)
+    return q, k, pos, freq.contiguous(), hd
+
+
+def rotary(x: torch.Tensor, positions: torch.Tensor, freq: torch.Tensor, n_heads: int, interleaved: bool = False, gain: float = 1.0) -> torch.Tensor:
+    """Rotary positions on x [M, n_heads * hd] (a column block of a wider matrix is read in place): the first 2 * len(freq) columns of every
+    head turn by positions[row] * freq; interleaved pairs (2 j, 2 j + 1) or halves (j, j + rot / 2).  positions [M] int64."""
+    x, _, positions, freq, hd = _rotary_args(x, None, positions, freq, n_heads, 0)
+    return _Rotary.apply(x, None, positions, freq, n_heads, 0, hd, bool(interleaved), float(gain))
+
+
+def rotary_qk(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, freq: torch.Tensor, n_heads: int, n_kv_heads: int,
+              interleaved: bool = False, gain: float = 1.0) -> tp.Tuple[torch.Tensor, torch.Tensor]:
+    """`rotary` of the queries and the keys of the same rows in one launch (their sines and cosines are shared)."""
+    q, k, positions, freq, hd = _rotary_args(q, k, positions, freq, n_heads, n_kv_heads)
+    return _Rotary.apply(q, k, positions, freq, n_heads, n_kv_heads, hd, bool(interleaved), float(gain))
+
+
+class _DiffLambda(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q1, k1, q2, k2, init):
+        H, hd = q1.shape
+        lam = torch.empty((H,), dtype=torch.float32, device=q1.device)
+        with torch.cuda.device(q1.device):
+            _c("rt_diff_lambda_fwd", q1, k1, q2, k2, float(init), H, hd, lam)
+        ctx.save_for_backward(q1, k1, q2, k2)
+        return lam
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        q1, k1, q2, k2 = ctx.saved_tensors
+        H, hd = q1.shape
+        outs = [torch.empty_like(q1) for _ in range(4)]
+        with torch.cuda.device(q1.device):
+            _c("rt_diff_lambda_bwd", g.contiguous(), q1, k1, q2, k2, H, hd, *outs)
+        return (*outs, None)
+
+
+def diff_lambda(q1: torch.Tensor, k1: torch.Tensor, q2: torch.Tensor, k2: torch.Tensor, init: float) -> torch.Tensor:
+    """The weight of the second softmax map of every head, [H] = exp(q1 . k1) - exp(q2 . k2) + init over learned [H, hd] vectors."""
+    vs = [_chk(t, "diff_lambda") for t in (q1, k1, q2, k2)]
+    if q1.dim() != 2 or any(t.shape != q1.shape for t in vs) or q1.shape[1] == 0:
+        raise ValueError(f"diff_lambda: four [heads, columns] matrices of one shape, got {[tuple(t.shape) for t in vs]}")
+    _same_device("diff_lambda", *vs)
+    return _DiffLambda.apply(*(t.contiguous() for t in vs), float(init))
+
+
+def _diff_attention_fwd(q, k, v, lam, cu_q, cu_k, key_ids, norm_w, meta, train):
+    B, H, Hkv, hd, Lq, Lk, causal, scale, out_scale, eps = meta
+    Nq, Nk = int(q.shape[0]), int(k.shape[0])
+    y = torch.empty((Nq, 2 * H * hd), dtype=torch.float32, device=q.device)
+    o12 = torch.empty((Nq, H, 2, 2 * hd), dtype=torch.float32, device=q.device) if train else None
+    lse = torch.empty((Nq, H, 2), dtype=torch.float32, device=q.device) if train else None
+    with torch.cuda.device(q.device):
+        n = _lib.load().rt_diffattn_fwd_workspace_bytes(B, H, Hkv, hd, Lq, Lk, Nq, int(train))
+        ws = torch.empty((n,), dtype=torch.uint8, device=q.device) if n > 0 else None
+        _c("rt_diffattn_fwd", q, _ld(q), k, _ld(k), v, _ld(v), lam, cu_q, cu_k, key_ids, B, H, Hkv, hd, Lq, Lk, Nq, Nk, scale, causal, norm_w,
+           out_scale, eps, y, int(y.shape[1]), o12, lse, ws, n)
+    return y, o12, lse
+
+
+class _DiffAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, lam, cu_q, cu_k, key_ids, norm_w, meta):
+        y, o12, lse = _diff_attention_fwd(q, k, v, lam, cu_q, cu_k, key_ids, norm_w, meta, True)
+        ctx.save_for_backward(q, k, v, lam, cu_q, cu_k, key_ids, norm_w, o12, lse)
+        ctx.meta = meta
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        q, k, v, lam, cu_q, cu_k, key_ids, norm_w, o12, lse = ctx.saved_tensors
+        B, H, Hkv, hd, Lq, Lk, causal, scale, out_scale, eps = ctx.meta
+        Nq, Nk = int(q.shape[0]), int(k.shape[0])
+        dy = _rows(dy, "diff_attention gradient")
+        dq, dk, dv = (torch.empty(tuple(t.shape), dtype=torch.float32, device=q.device) for t in (q, k, v))
+        dlam = torch.empty((H,), dtype=torch.float32, device=q.device)
+        dw = None if norm_w is None else torch.empty((2 * hd,), dtype=torch.float32, device=q.device)
+        with torch.cuda.device(q.device):
+            n = _lib.load().rt_diffattn_bwd_workspace_bytes(H, hd, max(Nq, 1))
+            ws = torch.empty((n,), dtype=torch.uint8, device=q.device)
+            _c("rt_diffattn_bwd", q, _ld(q), k, _ld(k), v, _ld(v), lam, cu_q, cu_k, key_ids, B, H, Hkv, hd, Lq, Lk, Nq, Nk, scale, causal,
+               norm_w, out_scale, eps, o12, lse, dy, _ld(dy), dq, 2 * H * hd, dk, 2 * Hkv * hd, dv, 2 * Hkv * hd, dlam, dw, ws, n)
+        return dq, dk, dv, dlam, None, None, None, dw, None
+
+
+def diff_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam: torch.Tensor, cu_q: tp.Optional[torch.Tensor],
+                   cu_k: tp.Optional[torch.Tensor], B: int, H: int, H_kv: int, Lq: int, Lk: int, causal: bool,
+                   key_ids: tp.Optional[torch.Tensor] = None, norm_w: tp.Optional[torch.Tensor] = None, out_scale: float = 1.0,
+                   eps: float = 1e-5, scale: tp.Optional[float] = None) -> torch.Tensor:
+    """Differential attention over sessions, [Nq, H * 2 hd]: (softmax(q1 k1^T) - lam softmax(q2 k2^T)) v per head, then (norm_w given) the
+    head's root-mean-square norm, times out_scale.  q [Nq, H * 2 hd]: the two maps' queries of a head next to each other; k [Nk, H_kv * 2
+    hd] the same; v [Nk, H_kv * 2 hd]; head h reads key head h // (H // H_kv); hd <= 64.  lam [H] (`diff_lambda`).
+
+    cu_q / cu_k [B + 1] int64: first row of every session (first 0, ascending), with Lq / Lk the longest sessions expected (plans the
+    launch; longer ones are served).  None: B sessions of exactly Lq / Lk rows.  The last query of a session meets its last key: with
+    causal, key j is seen by query i iff j <= i + nk - nq — so Lq = 1 is the newest row of a stored session.  key_ids [Nk] int64: keys with
+    id 0 are masked, whatever their rows hold.  A query that sees no key gives zeros; so do rows behind the last session of cu_q."""
+    if B < 0 or H <= 0 or H_kv <= 0 or H % H_kv != 0 or Lq < 0 or Lk < 0:
+        raise ValueError(f"diff_attention: B={B}, H={H}, H_kv={H_kv}, Lq={Lq}, Lk={Lk}")
+    q = _rows(q, "diff_attention q")
+    if q.shape[1] == 0 or q.shape[1] % (2 * H) != 0:
+        raise ValueError(f"diff_attention: {q.shape[1]} query columns do not split into {H} heads of two maps")
+    hd = int(q.shape[1]) // (2 * H)
+    if hd > 64:
+        raise NotImplementedError(f"diff_attention: at most 64 columns per map (128 value columns per head), got {hd}")
+    k, v = _rows(k, "diff_attention k", 2 * H_kv * hd), _rows(v, "diff_attention v", 2 * H_kv * hd)
+    if k.shape[0] != v.shape[0]:
+        raise ValueError(f"diff_attention: {k.shape[0]} key rows and {v.shape[0]} value rows")
+    for t, cu, L, what in ((q, cu_q, Lq, "query"), (k, cu_k, Lk, "key")):
+        if cu is None and t.shape[0] != B * L:
+            raise ValueError(f"diff_attention: {t.shape[0]} {what} rows for {B} sessions of {L}")
+    cu_q, cu_k = _ints(cu_q, "diff_attention cu_q", B + 1), _ints(cu_k, "diff_attention cu_k", B + 1)
+    key_ids = _ints(key_ids, "diff_attention key_ids", int(k.shape[0]))
+    lam = _chk(lam, "diff_attention lam").contiguous()
+    if tuple(lam.shape) != (H,):
+        raise ValueError(f"diff_attention: lam has one value per head, got {tuple(lam.shape)}")
+    if norm_w is not None:
+        norm_w = _chk(norm_w, "diff_attention norm_w").contiguous()
+        if tuple(norm_w.shape) != (2 * hd,):
+            raise ValueError(f"diff_attention: norm_w has {2 * hd} values, got {tuple(norm_w.shape)}")
+    if scale is not None and not scale > 0.0:
+        raise ValueError(f"diff_attention: the logit scale is positive, got {scale}")
+    _same_device("diff_attention", q, k, v, lam, cu_q, cu_k, key_ids, norm_w)
+    meta = (int(B), int(H), int(H_kv), hd, int(Lq), int(Lk), int(bool(causal)), 0.0 if scale is None else float(scale), float(out_scale), float(eps))
+    if not _needs_tape(q, k, v, lam, norm_w):
+        return _diff_attention_fwd(q, k, v, lam, cu_q, cu_k, key_ids, norm_w, meta, False)[0]
+    return _DiffAttention.apply(q, k, v, lam, cu_q, cu_k, key_ids, norm_w, meta)
+
+
+class _NormGate(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, f, z, scale, pw, pb, nw, nb, layer, alpha, eps, p, tape):
+        M, d = x.shape
+        y = torch.empty_like(x)
+        h = torch.empty_like(x) if nw is not None else None
+        stat = torch.empty((M, 4), dtype=torch.float32, device=x.device) if tape else None
+        seed, sid = RNG.next() if p > 0 else (0, 0)
+        with torch.cuda.device(x.device):
+            _c("rt_norm_gate_fwd", x, f, z, scale, pw, pb, nw, nb, layer, alpha, eps, p, seed, sid, M, d, y, h, stat)
+        ctx.save_for_backward(y if h is not None else None, f, z, scale, pw, pb, nw, stat)
+        ctx.meta = (layer, alpha, p, seed, sid, nb is not None)
+        ctx.set_materialize_grads(False)
+        return y if h is None else (y, h)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gy, gh=None):
+        y, f, z, scale, pw, pb, nw, stat = ctx.saved_tensors
+        layer, alpha, p, seed, sid, has_nb = ctx.meta
+        if gy is None and gh is None:
+            return (None,) * 13
+        M, d = f.shape
+        gy, gh = (None if g is None else g.contiguous() for g in (gy, gh))
+        dx, df = torch.empty_like(f), torch.empty_like(f)
+        dz = None if z is None else torch.empty_like(f)
+        vec = lambda there: torch.empty((d,), dtype=torch.float32, device=f.device) if there else None   # noqa: E731
+        ds, dpw, dpb, dnw, dnb = (vec(t) for t in (scale is not None, pw is not None, pb is not None, nw is not None, has_nb))
+        with torch.cuda.device(f.device):
+            n = _lib.load().rt_norm_gate_bwd_workspace_bytes(M, d)
+            ws = torch.empty((max(n, 16),), dtype=torch.uint8, device=f.device)
+            _c("rt_norm_gate_bwd", gy, gh, y if gh is not None else None, f, z, scale, pw, pb, nw, layer, alpha, p, seed, sid, M, d, stat, dx, df, dz,
+               ds, dpw, dpb, dnw, dnb, ws, n)
+        return (dx, df, dz, ds, dpw, dpb, dnw, dnb) + (None,) * 5
+
+
+NormParams = tp.Tuple[torch.Tensor, tp.Optional[torch.Tensor]]
+
+
+def norm_gate_residual(x: torch.Tensor, f: torch.Tensor, gate: tp.Optional[torch.Tensor] = None, post: tp.Optional[NormParams] = None,
+                       scale: tp.Optional[torch.Tensor] = None, pre: tp.Optional[NormParams] = None, kind: str = "rms", alpha: float = 1.0,
+                       eps: float = 1e-5, p: float = 0.0) -> tp.Tuple[torch.Tensor, tp.Optional[torch.Tensor]]:
+    """One pass over the rows between two blocks: y = alpha x + scale * sigmoid(gate) * dropout(N_post(f)), h = N_pre(y) -> (y, h).
+    x (residual stream), f (the block's output), gate (logits) [M, d]; scale [d] (a learned residual scale); post / pre = (weight [d], bias
+    [d] or None) of the norm behind this block and the one in front of the next; kind "rms" (root mean square) or "layer" (LayerNorm).  Any of
+    gate, post, scale, pre may be None (h is None without pre).  d <= 8192."""
+    if kind not in ("rms", "layer"):
+        raise ValueError(f"norm_gate_residual: kind is 'rms' or 'layer', got {kind!r}")
+    if not 0.0 <= p < 1.0:
+        raise ValueError(f"norm_gate_residual: dropout rate in [0, 1), got {p}")
+    _chk(x, "norm_gate_residual x")
+    if x.dim() != 2 or x.shape[1] == 0:
+        raise ValueError(f"norm_gate_residual: expected [rows, columns], got {tuple(x.shape)}")
+    d = int(x.shape[1])
+    if d > 8192:
+        raise NotImplementedError(f"norm_gate_residual: rows of at most 8,192 columns, got {d}")
+    if kind == "rms" and any(n is not None and n[1] is not None for n in (post, pre)):
+        raise ValueError("norm_gate_residual: the root-mean-square norm has no bias")
+    pw, pb = post if post is not None else (None, None)
+    nw, nb = pre if pre is not None else (None, None)
+    if (post is not None and pw is None) or (pre is not None and nw is None):
+        raise ValueError("norm_gate_residual: a norm needs its weight")
+    rows, cols = [x, f, gate], [scale, pw, pb, nw, nb]
+    for t, shape in [(t, tuple(x.shape)) for t in rows] + [(t, (d,)) for t in cols]:
+        if t is not None and tuple(_chk(t, "norm_gate_residual").shape) != shape:
+            raise ValueError(f"norm_gate_residual: expected {shape}, got {tuple(t.shape)}")
+    _same_device("norm_gate_residual", x, *rows[1:], *cols)
+    rows, cols = ([None if t is None else t.contiguous() for t in ts] for ts in (rows, cols))
+    out = _NormGate.apply(*rows, *cols, int(kind == "layer"), float(alpha), float(eps), float(p), _needs_tape(*rows, *cols))
+    return out if pre is not None else (out, None)
