@@ -375,102 +375,127 @@ __global__ __launch_bounds__(NT, 2) void diff_fwd_kernel(Args a) {
   }
 }
 
-// join of the key splits: one wave per (row, head)
+// join of the key splits: one workgroup per (row, head); a lane holds the statistics of a split (n_split <= 64), then a thread sums one value
+// column over its share of the splits
 __global__ __launch_bounds__(NT) void diff_combine_kernel(Args a) {
-  const int lane = threadIdx.x & 63, dv = 2 * a.hd;
-  const long long at = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (at >= a.Nq * a.H) return;
-  const long long row = at / a.H;
+  __shared__ float wgt[2][64], sums[NT], res[2][128], ssq[2];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, dv = 2 * a.hd;
+  const long long at = blockIdx.x, row = at / a.H, plane = a.Nq * a.H;
   const int h = (int)(at % a.H);
   if (row >= rows_used(a.cu_q, a.B, a.Nq)) return;      // (zeros already)
-  float o[2][2] = {{0.f, 0.f}, {0.f, 0.f}};      // [map][column lane, lane + 64]
+  if (wave < 2) {
+    const bool on = lane < a.n_split;
+    const long long p = ((long long)lane * plane + at) * 2 + wave;
+    const float m = on ? a.ml[2 * p] : -INFINITY, l = on ? a.ml[2 * p + 1] : 0.f, mx = wave_max(m), base = mx == -INFINITY ? 0.f : mx;
+    const float e = on ? __builtin_amdgcn_exp2f(m - base) : 0.f, total = wave_sum(l * e);
+    wgt[wave][lane] = e * (total > 0.f ? 1.f / total : (total == 0.f ? 0.f : total));
+    if (a.lse != nullptr && lane == 0) a.lse[at * 2 + wave] = total > 0.f ? mx + __builtin_amdgcn_logf(total) : 0.f;
+  }
+  const int slots = NT / dv, c = tid % dv, sub = tid / dv;
   for (int mp = 0; mp < 2; ++mp) {
-    float m = -INFINITY, l = 0.f;
-    for (int s = 0; s < a.n_split; ++s) m = fmaxf(m, a.ml[2 * (((long long)s * a.Nq * a.H + at) * 2 + mp)]);
-    const float base = m == -INFINITY ? 0.f : m;
-    for (int s = 0; s < a.n_split; ++s) {
-      const long long p = ((long long)s * a.Nq * a.H + at) * 2 + mp;
-      const float w = __builtin_amdgcn_exp2f(a.ml[2 * p] - base);
-      l += a.ml[2 * p + 1] * w;
-      if (w != 0.f) {      // (an empty split holds zeros)
-        if (lane < dv) o[mp][0] += a.part[p * dv + lane] * w;
-        if (lane + 64 < dv) o[mp][1] += a.part[p * dv + lane + 64] * w;
-      }
-    }
-    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-    o[mp][0] *= inv;
-    o[mp][1] *= inv;
-    if (a.lse != nullptr && lane == 0) a.lse[at * 2 + mp] = l > 0.f ? m + __builtin_amdgcn_logf(l) : 0.f;
-    if (a.o12 != nullptr) {
-      if (lane < dv) a.o12[(at * 2 + mp) * dv + lane] = o[mp][0];
-      if (lane + 64 < dv) a.o12[(at * 2 + mp) * dv + lane + 64] = o[mp][1];
+    __syncthreads();
+    float x = 0.f;
+    if (sub < slots)
+      for (int s = sub; s < a.n_split; s += slots) x = fmaf(a.part[(((long long)s * plane + at) * 2 + mp) * dv + c], wgt[mp][s], x);
+    sums[tid] = x;
+    __syncthreads();
+    if (tid < dv) {
+      for (int k = 1; k < slots; ++k) x += sums[k * dv + tid];
+      res[mp][tid] = x;
+      if (a.o12 != nullptr) a.o12[(at * 2 + mp) * dv + tid] = x;
     }
   }
-  const float lam = a.lam[h];
-  const float x0 = o[0][0] - lam * o[1][0], x1 = o[0][1] - lam * o[1][1];
-  const float ss = wave_sum(x0 * x0 + x1 * x1);
-  const float f = a.norm_w != nullptr ? a.out_scale / sqrtf(ss / (float)dv + a.eps) : a.out_scale;
-  float* y = a.y + row * a.ldy + (long long)h * dv;
-  if (lane < dv) y[lane] = x0 * f * (a.norm_w != nullptr ? a.norm_w[lane] : 1.f);
-  if (lane + 64 < dv) y[lane + 64] = x1 * f * (a.norm_w != nullptr ? a.norm_w[lane + 64] : 1.f);
+  const float o = tid < dv ? res[0][tid] - a.lam[h] * res[1][tid] : 0.f;      // (its own columns: no barrier)
+  if (tid < 128) {
+    const float q = wave_sum(o * o);
+    if (lane == 0) ssq[wave] = q;
+  }
+  __syncthreads();
+  const float f = a.norm_w != nullptr ? a.out_scale / sqrtf((ssq[0] + ssq[1]) / (float)dv + a.eps) : a.out_scale;
+  if (tid < dv) a.y[row * a.ldy + (long long)h * dv + tid] = o * f * (a.norm_w != nullptr ? a.norm_w[tid] : 1.f);
 }
 
 // ---- backward, in front: gradient of o, delta_m = do . o_m, and the sums behind dlam and dw -----------------------------------------------
-// one wave per (row, head), PRE_ROWS rows per workgroup; partial sums per workgroup in a fixed order
-constexpr int PRE_WG = 512;      // workgroups at most: the partials are [PRE_WG][H + 2 hd] doubles
+// HD / 2 lanes per (row, head), four columns each; a lane group keeps its head, so dlam and dw stay in registers over all of its rows.  They
+// are summed in 64 bits, per workgroup, in a fixed order.
+constexpr int PRE_WG = 1024;      // workgroups at most: the partials are [PRE_WG][H + 2 hd] doubles
 
+template <int LANES> __device__ __forceinline__ float group_sum(float v) {      // 16 or 32 neighbouring lanes
+  v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0xB1, 0xF, 0xF, true));
+  v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x4E, 0xF, 0xF, true));
+  v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x141, 0xF, 0xF, true));
+  v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x140, 0xF, 0xF, true));
+  if (LANES == 32) v += __builtin_bit_cast(float, __builtin_amdgcn_ds_swizzle(__builtin_bit_cast(int, v), 0x401F));
+  return v;
+}
+template <bool VEC> __device__ __forceinline__ f32x4 get4(const float* p, int c, int ncol) {
+  f32x4 x{0.f, 0.f, 0.f, 0.f};
+  if (VEC) {
+    if (c < ncol) x = *reinterpret_cast<const f32x4*>(p + c);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (c + e < ncol) x[e] = p[c + e];
+  }
+  return x;
+}
+
+template <int HD, bool VEC>
 __global__ __launch_bounds__(NT) void diff_bwd_pre_kernel(Args a, const float* dy, long long lddy, float* dout, float* delta, double* part) {
-  extern __shared__ double sums[];      // [4][H + dv]
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, dv = 2 * a.hd, H = a.H, W = H + dv;
-  for (int c = threadIdx.x; c < 4 * W; c += NT) sums[c] = 0.0;
-  __syncthreads();
-  double* mine = sums + wave * W;
+  constexpr int LANES = HD / 2, GROUPS = NT / LANES;
+  __shared__ double sw[GROUPS][2 * HD], sl[GROUPS];
+  const int tid = threadIdx.x, gid = tid / LANES, c = (tid % LANES) * 4, dv = 2 * a.hd, H = a.H;
   const long long used = rows_used(a.cu_q, a.B, a.Nq);
-  double dw0 = 0.0, dw1 = 0.0;
-  const bool c0 = lane < dv, c1 = lane + 64 < dv;
-  const float w0 = a.norm_w != nullptr && c0 ? a.norm_w[lane] : 1.f, w1 = a.norm_w != nullptr && c1 ? a.norm_w[lane + 64] : 1.f;
-  for (long long row = (long long)blockIdx.x * 4 + wave; row < a.Nq; row += (long long)gridDim.x * 4) {
-    for (int h = 0; h < H; ++h) {
-      const long long at = row * H + h;
-      float* dst = dout + row * (long long)H * dv + (long long)h * dv;
-      if (row >= used) {
-        if (c0) dst[lane] = 0.f;
-        if (c1) dst[lane + 64] = 0.f;
-        if (lane < 2) delta[at * 2 + lane] = 0.f;
-        continue;
-      }
-      const float* o = a.o12 + at * 2 * dv;
-      const float* gy = dy + row * lddy + (long long)h * dv;
-      const float a0 = c0 ? o[lane] : 0.f, a1 = c1 ? o[lane + 64] : 0.f, b0 = c0 ? o[dv + lane] : 0.f, b1 = c1 ? o[dv + lane + 64] : 0.f;
-      const float g0 = c0 ? gy[lane] : 0.f, g1 = c1 ? gy[lane + 64] : 0.f, lam = a.lam[h];
-      float d0, d1;
-      if (a.norm_w != nullptr) {
-        const float x0 = a0 - lam * b0, x1 = a1 - lam * b1;
-        const float r = 1.f / sqrtf(wave_sum(x0 * x0 + x1 * x1) / (float)dv + a.eps);
-        const float u0 = x0 * r, u1 = x1 * r, e0 = g0 * w0 * a.out_scale, e1 = g1 * w1 * a.out_scale;
-        const float mean = wave_sum(e0 * u0 + e1 * u1) / (float)dv;
-        d0 = r * (e0 - u0 * mean);
-        d1 = r * (e1 - u1 * mean);
-        dw0 += (double)(a.out_scale * g0 * u0);
-        dw1 += (double)(a.out_scale * g1 * u1);
-      } else {
-        d0 = g0 * a.out_scale;
-        d1 = g1 * a.out_scale;
-      }
-      if (c0) dst[lane] = d0;
-      if (c1) dst[lane + 64] = d1;
-      const float s1 = wave_sum(d0 * a0 + d1 * a1), s2 = wave_sum(d0 * b0 + d1 * b1);
-      if (lane == 0) {
-        delta[at * 2] = s1;
-        delta[at * 2 + 1] = s2;
-        mine[h] -= (double)s2;
+  const long long gg = (long long)blockIdx.x * GROUPS + gid, n_groups = (long long)gridDim.x * GROUPS;
+  const int h = (int)(gg % H);
+  const long long step = n_groups / H;                       // rows are dealt to the step lane groups of a head; leftover groups do nothing
+  const float lam = a.lam[h], inv = 1.f / (float)dv;
+  const f32x4 w = a.norm_w != nullptr ? get4<VEC>(a.norm_w, c, dv) * a.out_scale : f32x4{a.out_scale, a.out_scale, a.out_scale, a.out_scale};
+  double dw[4] = {0.0, 0.0, 0.0, 0.0}, dl = 0.0;
+  for (long long row = gg < step * H ? gg / H : a.Nq; row < a.Nq; row += step) {
+    const long long at = row * H + h;
+    float* dst = dout + at * dv;
+    if (row >= used) {
+      put4<VEC ? 1 : 2>(dst, c, dv, f32x4{0.f, 0.f, 0.f, 0.f});
+      if (c == 0) { delta[at * 2] = 0.f; delta[at * 2 + 1] = 0.f; }
+      continue;
+    }
+    const f32x4 o1 = get4<VEC>(a.o12 + at * 2 * dv, c, dv), o2 = get4<VEC>(a.o12 + (at * 2 + 1) * dv, c, dv);
+    const f32x4 g = get4<VEC>(dy + row * lddy + (long long)h * dv, c, dv), e = g * w;
+    f32x4 d = e;
+    if (a.norm_w != nullptr) {
+      const f32x4 x = o1 - o2 * lam;
+      const float r = 1.f / sqrtf(group_sum<LANES>(x[0] * x[0] + x[1] * x[1] + x[2] * x[2] + x[3] * x[3]) * inv + a.eps);
+      const f32x4 u = x * r;
+      const float mean = group_sum<LANES>(e[0] * u[0] + e[1] * u[1] + e[2] * u[2] + e[3] * u[3]) * inv;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        d[k] = r * (e[k] - u[k] * mean);
+        dw[k] += (double)(a.out_scale * g[k] * u[k]);
       }
     }
+    put4<VEC ? 1 : 2>(dst, c, dv, d);
+    const float s1 = group_sum<LANES>(d[0] * o1[0] + d[1] * o1[1] + d[2] * o1[2] + d[3] * o1[3]);
+    const float s2 = group_sum<LANES>(d[0] * o2[0] + d[1] * o2[1] + d[2] * o2[2] + d[3] * o2[3]);
+    if (c == 0) { delta[at * 2] = s1; delta[at * 2 + 1] = s2; }
+    dl -= (double)s2;
   }
-  if (c0) mine[H + lane] = dw0;
-  if (c1) mine[H + lane + 64] = dw1;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) sw[gid][c + k] = dw[k];
+  if (c == 0) sl[gid] = dl;
   __syncthreads();
-  for (int c = threadIdx.x; c < W; c += NT) part[(long long)blockIdx.x * W + c] = ((sums[c] + sums[W + c]) + sums[2 * W + c]) + sums[3 * W + c];
+  double* out = part + (long long)blockIdx.x * (H + dv);
+  for (int x = tid; x < dv; x += NT) {
+    double s = sw[0][x];
+    for (int k = 1; k < GROUPS; ++k) s += sw[k][x];
+    out[H + x] = s;
+  }
+  for (int x = tid; x < H; x += NT) {
+    double s = 0.0;
+    for (int k = 0; k < GROUPS; ++k)
+      if ((int)(((long long)blockIdx.x * GROUPS + k) % H) == x) s += sl[k];
+    out[x] = s;
+  }
 }
 
 __global__ __launch_bounds__(64) void diff_bwd_sums_kernel(const double* part, int n, int H, int dv, float* dlam, float* dw) {
@@ -691,22 +716,42 @@ __global__ __launch_bounds__(NT, 2) void diff_bwd_dkv_kernel(Args a) {
   }
 }
 
-// ---- few query rows: the products are matrix-vector products ---------------------------------------------------------------------------------
-// A workgroup takes the R = rows * (H / Hkv) queries that share a key head through its share of the keys, KC keys at a time: raw fp32 rows in
-// LDS, one (key, query) dot product per thread, the softmax of a chunk per (query, map) in one wave, then one value column per thread.
+// ---- few query rows: the products are matrix-vector products, the keys and values are read once and the loads are the work ---------------------
+// A workgroup takes the R queries (rows x heads) that share a key head through its share of the keys.  A wave reads TK keys at a time straight
+// into registers: a key's two maps (and its value row) lie across 2 HD / 4 lanes, four columns each, so every load is whole cache lines; a
+// dot product is four multiply-adds and a sum over the lanes of its map (cross-lane adds, no LDS), the value sums stay with the lanes' columns.  Every wave
+// keeps its own running maximum and sum; no barrier in the loop, 16 loads of 16 bytes in flight per lane.
 constexpr int MAXR = 8;
 
-template <int HD, int MODE>
-__global__ __launch_bounds__(NT) void diff_decode_kernel(Args a) {
-  constexpr int DV = 2 * HD, KC = 2048 / HD, ROW = 4 * HD + 4, C4 = HD, U = KC * C4 / NT;      // 8 float4 per thread and chunk
-  constexpr int QS = HD + 4, SUB = NT / DV;
-  extern __shared__ __attribute__((aligned(16))) float sm[];
-  float* kv = sm;                                  // [KC][k1 | k2 | v | pad]
-  float* qs = kv + KC * ROW;                       // [2 R][QS]
-  float* ps = qs + 2 * MAXR * QS;                  // [KC][2 MAXR]
-  float* st = ps + KC * 2 * MAXR;                  // [2 MAXR][m, l, alpha, -]
-  float* red = kv;                                 // [SUB][2 R][DV] behind the loop
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+template <int CTRL> __device__ __forceinline__ float dpp(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, true));
+}
+template <int HD> __device__ __forceinline__ float map_sum(float v) {      // over the HD / 4 lanes of a key's map
+  v += dpp<0xB1>(v);       // lane ^ 1
+  v += dpp<0x4E>(v);       // lane ^ 2
+  v += dpp<0x141>(v);      // mirrored in 8 lanes
+  if (HD == 64) v += dpp<0x140>(v);      // mirrored in 16 lanes
+  return v;
+}
+template <int HD> __device__ __forceinline__ float other_map(float v) {
+  if (HD == 32) return dpp<0x128>(v);      // rotated by 8 in 16 lanes
+  return __builtin_bit_cast(float, __builtin_amdgcn_ds_swizzle(__builtin_bit_cast(int, v), 0x401F));      // lane ^ 16
+}
+template <int HD> __device__ __forceinline__ float keys_max(float v) {      // over the keys of one load
+  if (HD == 32) v = fmaxf(v, __shfl_xor(v, 16, 64));
+  return fmaxf(v, __shfl_xor(v, 32, 64));
+}
+template <int HD> __device__ __forceinline__ float keys_sum(float v) {
+  if (HD == 32) v += __shfl_xor(v, 16, 64);
+  return v + __shfl_xor(v, 32, 64);
+}
+constexpr int decode_keys(int HDP) { return HDP == 32 ? 32 : 16; }      // TK
+
+template <int HD, int MODE, int R>
+__global__ __launch_bounds__(NT, 2) void diff_decode_kernel(Args a) {
+  constexpr int DV = 2 * HD, LPK = HD / 2, KPL = 64 / LPK, NL = 8, TK = KPL * NL;
+  __shared__ float wstat[4][R][2][2], wacc[4][R][2][DV];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, kk = lane / LPK, c4 = lane % LPK, mp = c4 / (HD / 4), col = (c4 % (HD / 4)) * 4;
   const int b = blockIdx.x / a.Hkv, hk = blockIdx.x % a.Hkv, rep = a.H / a.Hkv, hd = a.hd, dv = 2 * hd;
   if (b == a.B) {      // rows behind the last session: zeros
     if (blockIdx.y != 0) return;
@@ -717,112 +762,122 @@ __global__ __launch_bounds__(NT) void diff_decode_kernel(Args a) {
   long long qr0, kr0; int nq, nk;
   rows_of(a.cu_q, b, a.Lq, a.Nq, qr0, nq);
   rows_of(a.cu_k, b, a.Lk, a.Nk, kr0, nk);
-  const int off = nk - nq;
+  const int off = nk - nq, per = R / rep;          // query rows of a pass: every one of them with its `rep` heads
   const float qscale = a.scale * LOG2E;
-  const int per = MAXR / rep;                      // query rows of a pass: every one of them with its `rep` heads
   for (int first = 0; first < nq; first += per) {
-    const int rows = min(per, nq - first), R = rows * rep;
-    __syncthreads();
-    for (int x = tid; x < 2 * R * HD; x += NT) {   // query (row, head, map) = row-major index x / HD
-      const int c = x % HD, w = x / HD, mp = w & 1, hh = (w >> 1) % rep, r = (w >> 1) / rep;
-      qs[w * QS + c] = c < hd ? a.q[(qr0 + first + r) * a.ldq + (long long)(2 * (hk * rep + hh) + mp) * hd + c] * qscale : 0.f;
+    const int rows = min(per, nq - first);
+    f32x4 qv[R], acc[R][2];
+    float m[R], l[R];
+#pragma unroll
+    for (int w = 0; w < R; ++w) {                  // query w = (row w / rep, head w % rep)
+      qv[w] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (w < rows * rep) {
+        const float* p = a.q + (qr0 + first + w / rep) * a.ldq + (long long)(2 * (hk * rep + w % rep) + mp) * hd + col;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (MODE == 0 || col + e < hd) qv[w][e] = p[e] * qscale;
+      }
+      acc[w][0] = acc[w][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+      m[w] = -INFINITY;
+      l[w] = 0.f;
     }
-    if (tid < 2 * MAXR) { st[tid * 4] = -INFINITY; st[tid * 4 + 1] = 0.f; st[tid * 4 + 2] = 0.f; }
-    float acc[2 * MAXR];
-#pragma unroll
-    for (int w = 0; w < 2 * MAXR; ++w) acc[w] = 0.f;
-    const int vc = tid % DV, sub = tid / DV;
     const int k_end = a.causal ? max(0, min(nk, first + rows + off)) : nk;
-    const int n_ch = (k_end + KC - 1) / KC, each = (n_ch + a.n_split - 1) / a.n_split;
-    const int c_lo = min(n_ch, (int)blockIdx.y * each), c_hi = min(n_ch, c_lo + each);
-    f32x4 nx[U];
-    auto fetch = [&](int c) {
+    const int n_t = (k_end + TK - 1) / TK, each = (n_t + a.n_split - 1) / a.n_split, t_lo = min(n_t, (int)blockIdx.y * each), t_hi = min(n_t, t_lo + each);
+    for (int t = t_lo + wave; t < t_hi; t += 4) {
+      f32x4 kf[NL], vf[NL];
+      unsigned live = 0u;
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int idx = tid + u * NT, r = idx / C4, col = (idx % C4) * 4, j = c * KC + r;      // col: k1 [0, HD) | k2 [HD, 2 HD) | v [2 HD, 4 HD)
-        nx[u] = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (j < k_end && (a.key_ids == nullptr || a.key_ids[kr0 + j] != 0)) {
-          const bool isv = col >= 2 * HD;
-          const int cc = isv ? col - 2 * HD : col % HD, nc = isv ? dv : hd;
-          const float* p = isv ? a.v + (kr0 + j) * a.ldv + (long long)hk * dv + cc : a.k + (kr0 + j) * a.ldk + (long long)(2 * hk + (col >= HD ? 1 : 0)) * hd + cc;
+      for (int u = 0; u < NL; ++u) {
+        const int key = t * TK + u * KPL + kk;
+        kf[u] = vf[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (key < k_end && (a.key_ids == nullptr || a.key_ids[kr0 + key] != 0)) {
+          live |= 1u << u;
+          const float* kp = a.k + (kr0 + key) * a.ldk + (long long)(2 * hk + mp) * hd + col;
+          const float* vp = a.v + (kr0 + key) * a.ldv + (long long)hk * dv + 4 * c4;
           if (MODE < 2) {
-            if (MODE == 0 || cc < nc) nx[u] = *reinterpret_cast<const f32x4*>(p);
+            if (MODE == 0 || col < hd) kf[u] = *reinterpret_cast<const f32x4*>(kp);
+            if (MODE == 0 || 4 * c4 < dv) vf[u] = *reinterpret_cast<const f32x4*>(vp);
           } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (cc + e < nc) nx[u][e] = p[e];
+            for (int e = 0; e < 4; ++e) {
+              if (col + e < hd) kf[u][e] = kp[e];
+              if (4 * c4 + e < dv) vf[u][e] = vp[e];
+            }
           }
         }
       }
-    };
-    if (c_lo < c_hi) fetch(c_lo);
-    for (int c = c_lo; c < c_hi; ++c) {
-      __syncthreads();
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int idx = tid + u * NT;
-        *reinterpret_cast<f32x4*>(kv + (idx / C4) * ROW + (idx % C4) * 4) = nx[u];
-      }
-      if (c + 1 < c_hi) fetch(c + 1);
-      __syncthreads();
-      for (int x = tid; x < KC * 2 * R; x += NT) {
-        const int j = x % KC, w = x / KC, mp = w & 1, r = (w >> 1) / rep;
-        const float* kp = kv + j * ROW + mp * HD;
-        const float* qp = qs + w * QS;
-        f32x4 s4{0.f, 0.f, 0.f, 0.f};
+      for (int w = 0; w < R; ++w) {
+        if (w >= rows * rep) break;
+        const int last = a.causal ? first + w / rep + off : 0x7FFFFFFF;
+        float s[NL], mx = m[w];
 #pragma unroll
-        for (int e = 0; e < HD; e += 4) {
-          const f32x4 kk = *reinterpret_cast<const f32x4*>(kp + e), qq = *reinterpret_cast<const f32x4*>(qp + e);
-#pragma unroll
-          for (int z = 0; z < 4; ++z) s4[z] = fmaf(kk[z], qq[z], s4[z]);
+        for (int u = 0; u < NL; ++u) {
+          s[u] = map_sum<HD>(fmaf(qv[w][0], kf[u][0], qv[w][1] * kf[u][1]) + fmaf(qv[w][2], kf[u][2], qv[w][3] * kf[u][3]));
+          if (((live >> u) & 1u) == 0u || t * TK + u * KPL + kk > last) s[u] = -INFINITY;
+          mx = fmaxf(mx, s[u]);
         }
-        const int key = c * KC + j;
-        const bool seen = key < nk && (!a.causal || key <= first + r + off) && (a.key_ids == nullptr || a.key_ids[kr0 + key] != 0);
-        ps[j * 2 * MAXR + w] = seen ? (s4[0] + s4[1]) + (s4[2] + s4[3]) : -INFINITY;
-      }
-      __syncthreads();
-      for (int w = wave; w < 2 * R; w += 4) {
-        const float s = lane < KC ? ps[lane * 2 * MAXR + w] : -INFINITY;
-        const float m0 = st[w * 4], mx = fmaxf(m0, wave_max(s)), base = mx == -INFINITY ? 0.f : mx;
-        const float e = lane < KC ? __builtin_amdgcn_exp2f(s - base) : 0.f, sum = wave_sum(e), alpha = __builtin_amdgcn_exp2f(m0 - base);
-        if (lane < KC) ps[lane * 2 * MAXR + w] = e;
-        if (lane == 0) { st[w * 4] = mx; st[w * 4 + 1] = st[w * 4 + 1] * alpha + sum; st[w * 4 + 2] = alpha; }
-      }
-      __syncthreads();
-      for (int w = 0; w < 2 * MAXR; ++w)
-        if (w < 2 * R) acc[w] *= st[w * 4 + 2];
-      for (int j = sub; j < KC; j += SUB) {
-        const float x = kv[j * ROW + 2 * HD + vc];
+        mx = keys_max<HD>(mx);
+        const float base = mx == -INFINITY ? 0.f : mx, alpha = __builtin_amdgcn_exp2f(m[w] - base);
+        m[w] = mx;
+        const float alpha_o = other_map<HD>(alpha);
+        acc[w][0] *= mp == 0 ? alpha : alpha_o;
+        acc[w][1] *= mp == 0 ? alpha_o : alpha;
+        float ps = 0.f;
 #pragma unroll
-        for (int w = 0; w < 2 * MAXR; ++w)
-          if (w < 2 * R) acc[w] = fmaf(ps[j * 2 * MAXR + w], x, acc[w]);
+        for (int u = 0; u < NL; ++u) {
+          const float p = __builtin_amdgcn_exp2f(s[u] - base), po = other_map<HD>(p), p0 = mp == 0 ? p : po, p1 = mp == 0 ? po : p;
+          ps += p;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            acc[w][0][e] = fmaf(p0, vf[u][e], acc[w][0][e]);
+            acc[w][1][e] = fmaf(p1, vf[u][e], acc[w][1][e]);
+          }
+        }
+        l[w] = l[w] * alpha + ps;
+      }
+    }
+    __syncthreads();      // (the previous pass's readers are done)
+#pragma unroll
+    for (int w = 0; w < R; ++w) {
+      const float lt = keys_sum<HD>(l[w]);
+#pragma unroll
+      for (int q = 0; q < 2; ++q)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[w][q][e] = keys_sum<HD>(acc[w][q][e]);
+      if (kk == 0) {
+        if (c4 % (HD / 4) == 0) { wstat[wave][w][mp][0] = m[w]; wstat[wave][w][mp][1] = lt; }
+        *reinterpret_cast<f32x4*>(&wacc[wave][w][0][4 * c4]) = acc[w][0];
+        *reinterpret_cast<f32x4*>(&wacc[wave][w][1][4 * c4]) = acc[w][1];
       }
     }
     __syncthreads();
-#pragma unroll
-    for (int w = 0; w < 2 * MAXR; ++w)
-      if (w < 2 * R) red[(sub * 2 * R + w) * DV + vc] = acc[w];
-    __syncthreads();
-    for (int u = wave; u < R; u += 4) {            // (row, head) u: this wave
-      const int r = u / rep, h = hk * rep + u % rep;
-      const long long row = qr0 + first + r;
+    for (int u = wave; u < rows * rep; u += 4) {            // query u: this wave
+      const long long row = qr0 + first + u / rep;
+      const int h = hk * rep + u % rep;
       float o[2][2];
-      for (int mp = 0; mp < 2; ++mp) {
-        const int w = 2 * u + mp;
-        float s0 = 0.f, s1 = 0.f;
-        for (int s = 0; s < SUB; ++s) {
-          s0 += red[(s * 2 * R + w) * DV + lane];      // (DV >= 64)
-          if (lane + 64 < DV) s1 += red[(s * 2 * R + w) * DV + lane + 64];
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        float mx = -INFINITY, lt = 0.f, s0 = 0.f, s1 = 0.f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) mx = fmaxf(mx, wstat[k][u][q][0]);
+        const float base = mx == -INFINITY ? 0.f : mx;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float e = __builtin_amdgcn_exp2f(wstat[k][u][q][0] - base);
+          lt = fmaf(wstat[k][u][q][1], e, lt);
+          s0 = fmaf(wacc[k][u][q][lane], e, s0);      // (DV >= 64)
+          if (DV > 64) s1 = fmaf(wacc[k][u][q][(lane + 64) % DV], e, s1);
         }
         if (a.n_split > 1) {
-          const long long at = (((long long)blockIdx.y * a.Nq + row) * a.H + h) * 2 + mp;
-          if (lane == 0) { a.ml[2 * at] = st[w * 4]; a.ml[2 * at + 1] = st[w * 4 + 1]; }
+          const long long at = (((long long)blockIdx.y * a.Nq + row) * a.H + h) * 2 + q;
+          if (lane == 0) { a.ml[2 * at] = mx; a.ml[2 * at + 1] = lt; }
           if (lane < dv) a.part[at * dv + lane] = s0;
           if (lane + 64 < dv) a.part[at * dv + lane + 64] = s1;
         }
-        const float l = st[w * 4 + 1], inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-        o[mp][0] = s0 * inv;
-        o[mp][1] = s1 * inv;
+        const float inv = lt > 0.f ? 1.f / lt : (lt == 0.f ? 0.f : lt);
+        o[q][0] = s0 * inv;
+        o[q][1] = s1 * inv;
       }
       if (a.n_split > 1) continue;
       const float lam = a.lam[h];
@@ -867,16 +922,16 @@ int pad_hd(int hd) { return hd <= 32 ? 32 : 64; }
 struct Plan { bool decode; int n_split; };
 // Training keeps the outputs of both maps and always takes the matrix kernel.  Otherwise queries that share a key head and are few
 // (<= MAXR of them per session) go through diff_decode_kernel.  Keys are split over workgroups until the launch has about 4 (decode) or 2
-// workgroups per CU, at least 4 chunks each.
+// workgroups per CU, at least 2 (decode) or 4 chunks each.
 Plan plan_of(int B, int H, int Hkv, int hd, int Lq, int Lk, bool train) {
   Plan p;
   const int rep = H / Hkv;
   p.decode = !train && (long long)rep * Lq <= MAXR;
   const long long wgs = p.decode ? (long long)B * Hkv : (long long)B * H * ((Lq + OWN - 1) / OWN);
-  const int chunk = p.decode ? 2048 / pad_hd(hd) : CH;
+  const int chunk = p.decode ? 4 * decode_keys(pad_hd(hd)) : CH;      // keys a workgroup takes at once
   const long long want = (long long)rt_num_cus() * (p.decode ? 4 : 2);
   long long s = wgs > 0 ? want / wgs : 1;
-  const long long most = Lk / (4 * chunk);
+  const long long most = Lk / (p.decode ? 2 * chunk : 4 * chunk);
   if (s > most) s = most;
   if (s > 64) s = 64;
   p.n_split = s > 1 ? (int)s : 1;
@@ -906,6 +961,15 @@ int start(K kernel, dim3 grid, size_t lds, hipStream_t stream, const Args& a) {
 #define RT_DIFF_START(KERNEL, HDP, MODE, ...)                                                                                        \
   ((HDP) == 32 ? ((MODE) == 0 ? start(KERNEL<32, 0>, __VA_ARGS__) : (MODE) == 1 ? start(KERNEL<32, 1>, __VA_ARGS__) : start(KERNEL<32, 2>, __VA_ARGS__)) \
                : ((MODE) == 0 ? start(KERNEL<64, 0>, __VA_ARGS__) : (MODE) == 1 ? start(KERNEL<64, 1>, __VA_ARGS__) : start(KERNEL<64, 2>, __VA_ARGS__)))
+
+template <int R>
+int start_decode(int HDP, int mode, dim3 grid, hipStream_t stream, const Args& a) {
+  if (HDP == 32)
+    return mode == 0 ? start(diff_decode_kernel<32, 0, R>, grid, 0, stream, a) : mode == 1 ? start(diff_decode_kernel<32, 1, R>, grid, 0, stream, a)
+                                                                                           : start(diff_decode_kernel<32, 2, R>, grid, 0, stream, a);
+  return mode == 0 ? start(diff_decode_kernel<64, 0, R>, grid, 0, stream, a) : mode == 1 ? start(diff_decode_kernel<64, 1, R>, grid, 0, stream, a)
+                                                                                         : start(diff_decode_kernel<64, 2, R>, grid, 0, stream, a);
+}
 
 size_t img_bytes(int HDP) { return HDP == 32 ? 2 * Img<32>::BYTES + Img<64>::BYTES : 2 * Img<64>::BYTES + Img<128>::BYTES; }
 
@@ -949,9 +1013,10 @@ int rt_diffattn_fwd(const float* q, int64_t ldq, const float* k, int64_t ldk, co
   const long long B1 = B + (cu_q != nullptr ? 1 : 0);
   if (p.decode) {
     if (!grid_ok(B1 * Hkv)) return RT_ERR_INVALID_ARG;
-    const int KC = 2048 / HDP;
-    const size_t lds = sizeof(float) * ((size_t)KC * (4 * HDP + 4) + 2 * MAXR * (HDP + 4) + (size_t)KC * 2 * MAXR + 2 * MAXR * 4);
-    const int rc2 = RT_DIFF_START(diff_decode_kernel, HDP, mode, dim3((unsigned)(B1 * Hkv), p.n_split), lds, stream, a);
+    const long long queries = (long long)(H / Hkv) * (Lq > 0 ? Lq : 1);
+    const dim3 grid((unsigned)(B1 * Hkv), p.n_split);
+    const int rc2 = queries <= 1 ? start_decode<1>(HDP, mode, grid, stream, a) : queries <= 2 ? start_decode<2>(HDP, mode, grid, stream, a)
+                    : queries <= 4 ? start_decode<4>(HDP, mode, grid, stream, a) : start_decode<8>(HDP, mode, grid, stream, a);
     if (rc2 != RT_OK) return rc2;
   } else {
     a.n_tiles = (Lq + OWN - 1) / OWN > 0 ? (Lq + OWN - 1) / OWN : 1;
@@ -960,8 +1025,8 @@ int rt_diffattn_fwd(const float* q, int64_t ldq, const float* k, int64_t ldk, co
     if (rc2 != RT_OK) return rc2;
   }
   if (p.n_split > 1) {
-    if (!grid_ok((Nq * H + 3) / 4)) return RT_ERR_INVALID_ARG;
-    diff_combine_kernel<<<(unsigned)((Nq * H + 3) / 4), NT, 0, stream>>>(a);
+    if (!grid_ok(Nq * H)) return RT_ERR_INVALID_ARG;
+    diff_combine_kernel<<<(unsigned)(Nq * H), NT, 0, stream>>>(a);
     RT_CHECK_LAUNCH();
   }
   return RT_OK;
@@ -998,16 +1063,23 @@ int rt_diffattn_bwd(const float* q, int64_t ldq, const float* k, int64_t ldk, co
   a.dout = dout; a.lddo = wq; a.delta = delta;
   hipStream_t s = stream;
 
-  const long long pre_rows = (Nq + 3) / 4;
-  const int n_pre = pre_rows < 1 ? 1 : (pre_rows > PRE_WG ? PRE_WG : (int)pre_rows);
-  const size_t pre_lds = sizeof(double) * 4 * (H + 2 * (size_t)hd);
-  if (pre_lds > 65536) return RT_ERR_UNSUPPORTED;
-  diff_bwd_pre_kernel<<<n_pre, NT, pre_lds, s>>>(a, dy, lddy, dout, delta, part);
+  const int HDP = pad_hd(hd), groups = NT / (HDP / 2);
+  long long n_pre = (Nq * H + groups - 1) / groups, least = (H + groups - 1) / groups;      // (one lane group per head at least)
+  n_pre = n_pre > PRE_WG ? PRE_WG : n_pre;
+  n_pre = n_pre < least ? least : n_pre;
+  if (n_pre > PRE_WG) return RT_ERR_UNSUPPORTED;
+  const bool pre_vec = hd % 2 == 0 && vec_ok(dy, lddy) && vec_ok(o12, 4) && (norm_w == nullptr || vec_ok(norm_w, 4));
+  if (HDP == 32) {
+    if (pre_vec) diff_bwd_pre_kernel<32, true><<<(unsigned)n_pre, NT, 0, s>>>(a, dy, lddy, dout, delta, part);
+    else diff_bwd_pre_kernel<32, false><<<(unsigned)n_pre, NT, 0, s>>>(a, dy, lddy, dout, delta, part);
+  } else {
+    if (pre_vec) diff_bwd_pre_kernel<64, true><<<(unsigned)n_pre, NT, 0, s>>>(a, dy, lddy, dout, delta, part);
+    else diff_bwd_pre_kernel<64, false><<<(unsigned)n_pre, NT, 0, s>>>(a, dy, lddy, dout, delta, part);
+  }
   RT_CHECK_LAUNCH();
-  diff_bwd_sums_kernel<<<H + 2 * hd, 64, 0, s>>>(part, n_pre, H, 2 * hd, dlam, dw);
+  diff_bwd_sums_kernel<<<H + 2 * hd, 64, 0, s>>>(part, (int)n_pre, H, 2 * hd, dlam, dw);
   RT_CHECK_LAUNCH();
 
-  const int HDP = pad_hd(hd);
   const bool vec = hd % 4 == 0 && vec_ok(q, ldq) && vec_ok(k, ldk) && vec_ok(v, ldv) && vec_ok(dq, lddq) && vec_ok(dk, lddk) && vec_ok(dv, lddv);
   const int mode = !vec ? 2 : (hd == HDP ? 0 : 1);
   const size_t img = img_bytes(HDP);

@@ -274,23 +274,28 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_gate_bwd_kernel(Ng
   }
 }
 
-// [n][5][d] partial sums -> the five column vectors (the ones that are asked for)
+// [n][5][d] partial sums -> the five column vectors (the ones that are asked for): 16 columns x 64 shares of the workgroups
 struct ColOut { float* o[5]; };
 __global__ __launch_bounds__(1024) void norm_gate_sums_kernel(const float* part, int n, int d, ColOut out) {
-  __shared__ float sm[16][65];
-  const int c = threadIdx.x & 63, sl = threadIdx.x >> 6;
-  const long long W = 5LL * d, at = (long long)blockIdx.x * 64 + c;
-  float s = 0.f;
+  __shared__ float sm[64][17];
+  const int c = threadIdx.x & 15, sl = threadIdx.x >> 4;
+  const long long W = 5LL * d, at = (long long)blockIdx.x * 16 + c;
+  float s[4] = {0.f, 0.f, 0.f, 0.f};
   if (at < W)
-    for (int r = sl; r < n; r += 16) s += part[r * W + at];
-  sm[sl][c] = s;
-  __syncthreads();
-  if (sl == 0 && at < W) {
-    s = sm[0][c];
+    for (int r = sl; r < n; r += 256) {
 #pragma unroll
-    for (int k = 1; k < 16; ++k) s += sm[k][c];
+      for (int k = 0; k < 4; ++k)
+        if (r + 64 * k < n) s[k] += part[(r + 64 * k) * W + at];
+    }
+  sm[sl][c] = (s[0] + s[1]) + (s[2] + s[3]);
+  __syncthreads();
+  for (int half = 32; half > 0; half >>= 1) {
+    if (sl < half) sm[sl][c] += sm[sl + half][c];
+    __syncthreads();
+  }
+  if (sl == 0 && at < W) {
     float* o = out.o[at / d];
-    if (o != nullptr) o[at % d] = s;
+    if (o != nullptr) o[at % d] = sm[0][c];
   }
 }
 
@@ -408,7 +413,7 @@ int rt_norm_gate_bwd(const float* gy, const float* gh, const float* y, const flo
   }
   if (sums) {
     const ColOut out{{dscale, dpost_w, dpost_b, dpre_w, dpre_b}};
-    norm_gate_sums_kernel<<<(5 * d + 63) / 64, 1024, 0, stream>>>((const float*)ws, (int)n, d, out);
+    norm_gate_sums_kernel<<<(5 * d + 15) / 16, 1024, 0, stream>>>((const float*)ws, (int)n, d, out);
     RT_CHECK_LAUNCH();
   }
   return RT_OK;

@@ -2563,6 +2563,30 @@ def _ints(t: tp.Optional[torch.Tensor], what: str, n: int) -> tp.Optional[torch.
     return t.contiguous()
 
 
+def _once(what: str) -> None:
+    """First line of a backward: grad mode is on there only under create_graph (`once_differentiable` costs a launch's host time)."""
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"{what} has no second derivative (create_graph=True)")
+
+
+class _DeviceOf:
+    """`with _DeviceOf(t):` — launches and the current stream are those of t's device; free when it is the current one."""
+
+    __slots__ = ("index", "prev")
+
+    def __init__(self, t: torch.Tensor) -> None:
+        self.index = t.get_device()
+
+    def __enter__(self) -> None:
+        self.prev = torch.cuda.current_device()
+        if self.prev != self.index:
+            torch.cuda.set_device(self.index)
+
+    def __exit__(self, *exc: tp.Any) -> None:
+        if self.prev != self.index:
+            torch.cuda.set_device(self.prev)
+
+
 def _needs_tape(*tensors: tp.Optional[torch.Tensor]) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
@@ -2602,10 +2626,10 @@ def _rotary_call(tensors: tp.Sequence[tp.Tuple[tp.Optional[torch.Tensor], int]],
             args += [None, 0, None, 0, 0]
             outs.append(None)
             continue
-        y = torch.empty(tuple(x.shape), dtype=torch.float32, device=x.device)
+        y = x.new_empty(x.shape)
         args += [x, _ld(x), y, int(y.shape[1]), heads]
         outs.append(y)
-    with torch.cuda.device(pos.device):
+    with _DeviceOf(pos):
         _c("rt_rotary", *args, pos, freq, int(pos.shape[0]), hd, 2 * int(freq.shape[0]), int(interleaved), float(gain), int(backward))
     return outs
 
@@ -2620,8 +2644,8 @@ class _Rotary(torch.autograd.Function):
         return q2 if k is None else (q2, k2)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, gq, gk=None):
+        _once("rotary")
         pos, freq = ctx.saved_tensors
         n_heads, n_kv_heads, hd, interleaved, gain = ctx.meta
         if gq is None and gk is None:
@@ -2670,18 +2694,18 @@ class _DiffLambda(torch.autograd.Function):
     def forward(ctx, q1, k1, q2, k2, init):
         H, hd = q1.shape
         lam = torch.empty((H,), dtype=torch.float32, device=q1.device)
-        with torch.cuda.device(q1.device):
+        with _DeviceOf(q1):
             _c("rt_diff_lambda_fwd", q1, k1, q2, k2, float(init), H, hd, lam)
         ctx.save_for_backward(q1, k1, q2, k2)
         return lam
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, g):
+        _once("diff_lambda")
         q1, k1, q2, k2 = ctx.saved_tensors
         H, hd = q1.shape
-        outs = [torch.empty_like(q1) for _ in range(4)]
-        with torch.cuda.device(q1.device):
+        outs = q1.new_empty((4, H, hd)).unbind(0)
+        with _DeviceOf(q1):
             _c("rt_diff_lambda_bwd", g.contiguous(), q1, k1, q2, k2, H, hd, *outs)
         return (*outs, None)
 
@@ -2701,7 +2725,7 @@ def _diff_attention_fwd(q, k, v, lam, cu_q, cu_k, key_ids, norm_w, meta, train):
     y = torch.empty((Nq, 2 * H * hd), dtype=torch.float32, device=q.device)
     o12 = torch.empty((Nq, H, 2, 2 * hd), dtype=torch.float32, device=q.device) if train else None
     lse = torch.empty((Nq, H, 2), dtype=torch.float32, device=q.device) if train else None
-    with torch.cuda.device(q.device):
+    with _DeviceOf(q):
         n = _lib.load().rt_diffattn_fwd_workspace_bytes(B, H, Hkv, hd, Lq, Lk, Nq, int(train))
         ws = torch.empty((n,), dtype=torch.uint8, device=q.device) if n > 0 else None
         _c("rt_diffattn_fwd", q, _ld(q), k, _ld(k), v, _ld(v), lam, cu_q, cu_k, key_ids, B, H, Hkv, hd, Lq, Lk, Nq, Nk, scale, causal, norm_w,
@@ -2718,16 +2742,16 @@ class _DiffAttention(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
+        _once("diff_attention")
         q, k, v, lam, cu_q, cu_k, key_ids, norm_w, o12, lse = ctx.saved_tensors
         B, H, Hkv, hd, Lq, Lk, causal, scale, out_scale, eps = ctx.meta
         Nq, Nk = int(q.shape[0]), int(k.shape[0])
         dy = _rows(dy, "diff_attention gradient")
-        dq, dk, dv = (torch.empty(tuple(t.shape), dtype=torch.float32, device=q.device) for t in (q, k, v))
-        dlam = torch.empty((H,), dtype=torch.float32, device=q.device)
-        dw = None if norm_w is None else torch.empty((2 * hd,), dtype=torch.float32, device=q.device)
-        with torch.cuda.device(q.device):
+        dq, dk, dv = (t.new_empty(t.shape) for t in (q, k, v))
+        dlam = lam.new_empty((H,))
+        dw = None if norm_w is None else lam.new_empty((2 * hd,))
+        with _DeviceOf(q):
             n = _lib.load().rt_diffattn_bwd_workspace_bytes(H, hd, max(Nq, 1))
             ws = torch.empty((n,), dtype=torch.uint8, device=q.device)
             _c("rt_diffattn_bwd", q, _ld(q), k, _ld(k), v, _ld(v), lam, cu_q, cu_k, key_ids, B, H, Hkv, hd, Lq, Lk, Nq, Nk, scale, causal,
@@ -2787,7 +2811,7 @@ class _NormGate(torch.autograd.Function):
         h = torch.empty_like(x) if nw is not None else None
         stat = torch.empty((M, 4), dtype=torch.float32, device=x.device) if tape else None
         seed, sid = RNG.next() if p > 0 else (0, 0)
-        with torch.cuda.device(x.device):
+        with _DeviceOf(x):
             _c("rt_norm_gate_fwd", x, f, z, scale, pw, pb, nw, nb, layer, alpha, eps, p, seed, sid, M, d, y, h, stat)
         ctx.save_for_backward(y if h is not None else None, f, z, scale, pw, pb, nw, stat)
         ctx.meta = (layer, alpha, p, seed, sid, nb is not None)
@@ -2795,8 +2819,8 @@ class _NormGate(torch.autograd.Function):
         return y if h is None else (y, h)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, gy, gh=None):
+        _once("norm_gate_residual")
         y, f, z, scale, pw, pb, nw, stat = ctx.saved_tensors
         layer, alpha, p, seed, sid, has_nb = ctx.meta
         if gy is None and gh is None:
@@ -2805,9 +2829,9 @@ class _NormGate(torch.autograd.Function):
         gy, gh = (None if g is None else g.contiguous() for g in (gy, gh))
         dx, df = torch.empty_like(f), torch.empty_like(f)
         dz = None if z is None else torch.empty_like(f)
-        vec = lambda there: torch.empty((d,), dtype=torch.float32, device=f.device) if there else None   # noqa: E731
-        ds, dpw, dpb, dnw, dnb = (vec(t) for t in (scale is not None, pw is not None, pb is not None, nw is not None, has_nb))
-        with torch.cuda.device(f.device):
+        there = (scale is not None, pw is not None, pb is not None, nw is not None, has_nb)
+        ds, dpw, dpb, dnw, dnb = (f.new_empty((d,)) if t else None for t in there)
+        with _DeviceOf(f):
             n = _lib.load().rt_norm_gate_bwd_workspace_bytes(M, d)
             ws = torch.empty((max(n, 16),), dtype=torch.uint8, device=f.device)
             _c("rt_norm_gate_bwd", gy, gh, y if gh is not None else None, f, z, scale, pw, pb, nw, layer, alpha, p, seed, sid, M, d, stat, dx, df, dz,
