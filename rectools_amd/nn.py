@@ -796,6 +796,153 @@ class LiGRLayers(TransformerLayersBase):
         return seqs.index_select(0, cu[1:B + 1] - 1)
 
 
+class DifferentialTransformerLayer(nn.Module):
+    """One block of `DifferentialTransformerLayers`: differential attention over rotary positions, then a feed-forward, each between a
+    norm in front and a norm behind, the latter with a gate on the residual stream and a learned residual scale."""
+
+    def __init__(self, n_factors: int, n_heads: int, n_kv_heads: int, dropout_rate: float, ff_factors_multiplier: int, ff_activation: str,
+                 bias_in_ff: bool, lambda_init: float) -> None:
+        super().__init__()
+        hd = n_factors // (2 * n_heads)
+        self.n_heads, self.n_kv_heads, self.hd, self.p, self.lambda_init = n_heads, n_kv_heads, hd, dropout_rate, lambda_init
+        self.widths = [n_factors, 2 * n_kv_heads * hd, 2 * n_kv_heads * hd]
+        self.in_proj = LinearParams(n_factors, sum(self.widths), bias=False)
+        self.out_proj = LinearParams(n_factors, n_factors, bias=False)
+        for name in ("lambda_q1", "lambda_k1", "lambda_q2", "lambda_k2"):
+            setattr(self, name, nn.Parameter(torch.randn(n_heads, hd) * 0.1))
+        self.head_norm = nn.Parameter(torch.ones(2 * hd))
+        self.feed_forward = init_feed_forward(n_factors, ff_factors_multiplier, dropout_rate, ff_activation, bias_in_ff)
+        self.layer_norm_1, self.layer_norm_2 = LayerNormParams(n_factors), LayerNormParams(n_factors)              # in front of each half
+        self.post_norm_1, self.post_norm_2 = LayerNormParams(n_factors), LayerNormParams(n_factors)                # behind it
+        self.residual_scale_1, self.residual_scale_2 = nn.Parameter(torch.ones(n_factors)), nn.Parameter(torch.ones(n_factors))
+        self.gating_linear_1, self.gating_linear_2 = LinearParams(n_factors, n_factors), LinearParams(n_factors, n_factors)
+
+    def lam(self) -> torch.Tensor:
+        return ops.diff_lambda(self.lambda_q1, self.lambda_k1, self.lambda_q2, self.lambda_k2, self.lambda_init)
+
+    def attend(self, q, k, v, cu_q, cu_k, B, Lq, Lk, causal, key_ids):
+        return ops.diff_attention(q, k, v, self.lam(), cu_q, cu_k, B, self.n_heads, self.n_kv_heads, Lq, Lk, causal, key_ids=key_ids,
+                                  norm_w=self.head_norm, out_scale=1.0 - self.lambda_init)
+
+    def _join(self, x, f, gating, post, scale, pre):
+        """x + scale * sigmoid(gating(x)) * dropout(post(f)) and its norm in front of the next half: one pass over the rows."""
+        return ops.norm_gate_residual(x, f, gate=gating(x), post=(post.weight, post.bias), scale=scale, pre=(pre.weight, pre.bias),
+                                      kind="layer", eps=pre.eps, p=self.p if self.training else 0.0)
+
+    def close(self, x, a, next_norm):
+        """Everything behind the attention: x (residual stream), a (attention output) -> (x, next_norm(x))."""
+        x, h = self._join(x, self.out_proj(a), self.gating_linear_1, self.post_norm_1, self.residual_scale_1, self.layer_norm_2)
+        return self._join(x, self.feed_forward(h), self.gating_linear_2, self.post_norm_2, self.residual_scale_2, next_norm)
+
+    def forward(self, x, h, rotary, pos, cu, B, L, causal, key_ids, next_norm):
+        """x: the residual stream, h = layer_norm_1(x) -> the next block's (x, h)."""
+        q, k, v = ops.linear(h, self.in_proj.weight).split(self.widths, dim=1)
+        q, k = ops.rotary_qk(q, k, pos, rotary.freq, 2 * self.n_heads, 2 * self.n_kv_heads, rotary.interleaved, rotary.gain)
+        return self.close(x, self.attend(q, k, v, cu, cu, B, L, L, causal, key_ids), next_norm)
+
+    def forward_last(self, x, h, rotary, pos, cu_k, B, L, causal, key_ids, last_rows, next_norm):
+        """Inference: next_norm of the block's output at `last_rows` (one per session), [B, d]: keys and values of every row, one query per
+        session, everything behind the attention on B rows."""
+        d = self.widths[0]
+        k, v = ops.linear(h, self.in_proj.weight[d:]).split(self.widths[1:], dim=1)
+        q = ops.linear(h.index_select(0, last_rows), self.in_proj.weight[:d])
+        q = ops.rotary(q, pos.index_select(0, last_rows), rotary.freq, 2 * self.n_heads, rotary.interleaved, rotary.gain)
+        k = ops.rotary(k, pos, rotary.freq, 2 * self.n_kv_heads, rotary.interleaved, rotary.gain)
+        a = self.attend(q, k, v, None, cu_k, B, 1, L, causal, key_ids)
+        return self.close(x.index_select(0, last_rows), a, next_norm)[1]
+
+
+class RotaryPositions(nn.Module):
+    """Frequencies of `ops.rotary`: a buffer that moves with the model and is no part of its state."""
+
+    def __init__(self, rot: int, base: float = 10_000.0, interleaved: bool = False, scaling: str = "none", factor: float = 1.0,
+                 trained_len: int = 4096) -> None:
+        super().__init__()
+        freq, self.gain = ops.rotary_frequencies(rot, base, scaling, factor, trained_len)
+        self.register_buffer("freq", freq, persistent=False)
+        self.interleaved = interleaved
+
+    def _apply(self, fn: tp.Callable, recurse: bool = True) -> "RotaryPositions":
+        """Moves between devices; the frequencies stay in 64 bits whatever the module is cast to."""
+        freq = self.freq
+        super()._apply(fn, recurse)
+        self.freq = freq.to(self.freq.device)
+        return self
+
+
+class DifferentialTransformerLayers(TransformerLayersBase):
+    """A layer stack for `transformer_layers_type`: every attention map is the difference of two softmax maps with a learned weight
+    (`ops.diff_attention`), positions turn the queries and keys (`ops.rotary_qk`; set the model's `use_pos_emb=False` to use them alone), and every
+    half of a block stands between two norms with a gate and a learned residual scale (`ops.norm_gate_residual`).  n_heads heads of n_factors
+    / n_heads value columns, half as many query and key columns per map (n_factors divisible by 2 n_heads, at most 128 value columns);
+    n_kv_heads (a divisor of n_heads): heads share their keys and values.  rotary_part: the share of a map's columns that turn.  The
+    reference has no counterpart."""
+
+    def __init__(self, n_blocks: int, n_factors: int, n_heads: int, dropout_rate: float, n_kv_heads: tp.Optional[int] = None,
+                 ff_factors_multiplier: int = 4, ff_activation: str = "swiglu", bias_in_ff: bool = False, rotary_part: float = 1.0,
+                 rotary_base: float = 10_000.0, rotary_interleaved: bool = False, rotary_scaling: str = "none", rotary_factor: float = 1.0,
+                 rotary_trained_len: int = 4096, **kwargs: tp.Any) -> None:
+        super().__init__()
+        n_kv_heads = n_heads if n_kv_heads is None else n_kv_heads
+        if n_factors % (2 * n_heads) != 0 or n_heads % n_kv_heads != 0:
+            raise ValueError(f"DifferentialTransformerLayers: n_factors must be divisible by 2 * n_heads and n_heads by n_kv_heads, got n_factors={n_factors}, "
+                             f"n_heads={n_heads}, n_kv_heads={n_kv_heads}")
+        hd = n_factors // (2 * n_heads)
+        if hd > 64:
+            raise NotImplementedError(f"DifferentialTransformerLayers: at most 128 value columns per head, got {2 * hd}: use more heads")
+        rot = int(hd * rotary_part) // 2 * 2
+        if not 0.0 < rotary_part <= 1.0 or rot == 0:
+            raise ValueError(f"DifferentialTransformerLayers: rotary_part in (0, 1] of {hd} columns must hold a pair, got {rotary_part}")
+        self.n_blocks = n_blocks
+        self.rotary = RotaryPositions(rot, rotary_base, rotary_interleaved, rotary_scaling, rotary_factor, rotary_trained_len)
+        self.transformer_blocks = nn.ModuleList([
+            DifferentialTransformerLayer(n_factors, n_heads, n_kv_heads, dropout_rate, ff_factors_multiplier, ff_activation, bias_in_ff,
+                                         0.8 - 0.6 * math.exp(-0.3 * i)) for i in range(n_blocks)])
+        self.last_layernorm = LayerNormParams(n_factors)
+
+    def _blocks(self) -> tp.List[tp.Tuple[nn.Module, nn.Module]]:
+        """(block, the norm behind its residual stream): the next block's first norm, the stack's last one at the end."""
+        blocks = list(self.transformer_blocks)
+        return list(zip(blocks, [b.layer_norm_1 for b in blocks[1:]] + [self.last_layernorm]))
+
+    def _run(self, x, pos, cu, B, L, causal, key_ids, last_rows=None):
+        blocks = self._blocks()
+        if not blocks:
+            return self.last_layernorm(x if last_rows is None else x.index_select(0, last_rows))
+        with ops.active_planes(self._fresh_planes()):      # the Linear products read the pre-split weight planes
+            h = blocks[0][0].layer_norm_1(x)
+            for i, (blk, norm) in enumerate(blocks):
+                if last_rows is not None and i + 1 == len(blocks):
+                    return blk.forward_last(x, h, self.rotary, pos, cu, B, L, causal, key_ids, last_rows, norm)
+                x, h = blk(x, h, self.rotary, pos, cu, B, L, causal, key_ids, norm)
+        return h
+
+    def forward(self, seqs, ids, B, L, causal, keypad, batch):
+        pos = torch.arange(L, device=seqs.device).repeat(B)
+        return self._run(seqs, pos, None, B, L, causal, ids if keypad else None)
+
+    def forward_last(self, seqs, ids, B, L, causal, keypad, batch):
+        """Inference: [B, d] encodings of the last position; the final block on one query row per session."""
+        pos = torch.arange(L, device=seqs.device).repeat(B)
+        return self._run(seqs, pos, None, B, L, causal, ids if keypad else None, torch.arange(L - 1, B * L, L, device=seqs.device))
+
+    def packed_ok(self, n_factors: int, window: int, causal: bool, keypad: bool = False) -> bool:
+        """Packed rows serve this stack when the pad positions are masked as keys: nothing else couples rows, and rotary positions only see
+        differences.  Without the mask the pad rows carry state that real queries read: the padded window."""
+        return len(self.transformer_blocks) > 0 and keypad
+
+    @staticmethod
+    def _packed_positions(cu: torch.Tensor, n: int) -> torch.Tensor:
+        row = torch.arange(n, device=cu.device)
+        return row - cu[torch.searchsorted(cu, row, right=True) - 1]
+
+    def forward_packed_train(self, seqs, cu, B, window, keypad, rows_real=None, causal=True):
+        return self._run(seqs, self._packed_positions(cu, int(seqs.shape[0])), cu, B, window, causal, None)
+
+    def forward_last_packed(self, seqs, cu, B, window, keypad, rows_real=None, causal=True):
+        return self._run(seqs, self._packed_positions(cu, int(seqs.shape[0])), cu[:B + 1], B, window, causal, None, cu[1:B + 1] - 1)
+
+
 def _with_dump_row(x: torch.Tensor) -> torch.Tensor:
     """[n, d] -> [n + 1, d] with a zero row behind it: the slot the unused tail rows of a packed block gather from."""
     return torch.nn.functional.pad(x, (0, 0, 0, 1))

@@ -1,0 +1,253 @@
+"""`nn.DifferentialTransformerLayers`: rotary positions, differential attention and the fused norms / gate / residual scale together, as a layer
+stack of the models — against the same stack written out in 64 bits, packed against padded, the last rows alone, captured and replayed, through
+fit and recommend."""
+import math
+
+import numpy as np
+import pandas as pd
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+# Two blocks are eight stages in a row (in_proj, attention, out_proj, join, ff up, ff down, join, norm).  A stage is a sum over at most 256
+# products and one statistic over 64 columns: at most (256 + 64 + 80) u of its magnitude, and the norms hold the magnitudes near one.
+STACK_K = 8 * 400 * U
+
+
+def _stack(d=64, H=2, kv=1, blocks=2, p=0.0, **kw):
+    from rectools_amd import nn as hnn
+
+    torch.manual_seed(5)
+    layers = hnn.DifferentialTransformerLayers(blocks, d, H, p, n_kv_heads=kv, ff_factors_multiplier=2, **kw)
+    with torch.no_grad():
+        for n, t in layers.named_parameters():
+            if "norm" in n or "scale" in n:
+                t.add_(torch.randn(t.shape) * 0.1)
+    return layers.cuda()
+
+
+def _plain(layers, x, pos, see, B, L):
+    """The stack in 64 bits on [B, L] windows: x [B L, d] double (its device), see [B, L, L] -> [B L, d]."""
+    P = {n: t.detach().to(x.device).double().requires_grad_() for n, t in layers.named_parameters()}
+    freq, rot = layers.rotary.freq.to(x.device), 2 * layers.rotary.freq.numel()
+    phi = (pos.double()[:, None] * freq[None])[:, None]
+    ln = lambda t, n: torch.nn.functional.layer_norm(t, (t.shape[1],), P[n + ".weight"], P[n + ".bias"], 1e-5)   # noqa: E731
+
+    def turn(t, heads):
+        t = t.reshape(B * L, heads, -1)
+        r, rest = t[..., :rot], t[..., rot:]
+        a, b = (r[..., 0::2], r[..., 1::2]) if layers.rotary.interleaved else (r[..., :rot // 2], r[..., rot // 2:])
+        u, v = a * phi.cos() - b * phi.sin(), a * phi.sin() + b * phi.cos()
+        r = torch.stack((u, v), -1).flatten(-2) if layers.rotary.interleaved else torch.cat((u, v), -1)
+        return torch.cat((layers.rotary.gain * r, rest), -1)
+
+    for i, blk in enumerate(layers.transformer_blocks):
+        n = f"transformer_blocks.{i}."
+        H, Hk, hd = blk.n_heads, blk.n_kv_heads, blk.hd
+        h = ln(x, n + "layer_norm_1")
+        q, k, v = (h @ P[n + "in_proj.weight"].T).split(blk.widths, 1)
+        q = turn(q, 2 * H).view(B, L, H, 2, hd).permute(0, 2, 3, 1, 4)
+        k = turn(k, 2 * Hk).view(B, L, Hk, 2, hd).permute(0, 2, 3, 1, 4).repeat_interleave(H // Hk, 1)
+        v = v.view(B, L, Hk, 2 * hd).transpose(1, 2).repeat_interleave(H // Hk, 1)
+        s = (q @ k.transpose(-1, -2)) / math.sqrt(hd)
+        w = see[:, None, None]
+        s = s.masked_fill(~w, -1e30)
+        e = torch.exp(s - s.detach().amax(-1, keepdim=True).clamp(min=-1e20)).masked_fill(~w, 0.0)
+        t = e.sum(-1, keepdim=True)
+        A = e / torch.where(t > 0, t, 1.0)
+        lam = torch.exp((P[n + "lambda_q1"] * P[n + "lambda_k1"]).sum(1)) - torch.exp((P[n + "lambda_q2"] * P[n + "lambda_k2"]).sum(1)) + blk.lambda_init
+        o = (A[:, :, 0] - lam[:, None, None] * A[:, :, 1]) @ v
+        o = o / torch.sqrt((o * o).mean(-1, keepdim=True) + 1e-5) * P[n + "head_norm"] * (1.0 - blk.lambda_init)
+        f = o.transpose(1, 2).reshape(B * L, -1) @ P[n + "out_proj.weight"].T
+        gate = torch.sigmoid(x @ P[n + "gating_linear_1.weight"].T + P[n + "gating_linear_1.bias"])
+        x = x + P[n + "residual_scale_1"] * gate * ln(f, n + "post_norm_1")
+        h = ln(x, n + "layer_norm_2")
+        f = torch.nn.functional.silu(h @ P[n + "feed_forward.ff_linear_1.weight"].T) * (h @ P[n + "feed_forward.ff_linear_3.weight"].T)
+        f = f @ P[n + "feed_forward.ff_linear_2.weight"].T
+        gate = torch.sigmoid(x @ P[n + "gating_linear_2.weight"].T + P[n + "gating_linear_2.bias"])
+        x = x + P[n + "residual_scale_2"] * gate * ln(f, n + "post_norm_2")
+    return ln(x, "last_layernorm"), P
+
+
+def _near(got, want, k, what):
+    got, want = got.detach().cpu().double(), want.detach().cpu().double()
+    off, size = float((got - want).norm()), float(want.norm())
+    assert off <= k * size + 1e-30, f"{what}: off by {off / max(size, 1e-300):.2e}, allowed {k:.2e}"
+
+
+def _batch(B, L, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    ids = torch.randint(1, 50, (B, L), generator=g)
+    for b, n in enumerate([L, 1, L // 2, 3][:B]):
+        ids[b, :L - n] = 0
+    return ids, torch.randn(B * L, 64, generator=g), torch.randn(B * L, 64, generator=g)
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(kv=2, rotary_part=0.5, rotary_interleaved=True), dict(rotary_scaling="parts", rotary_factor=4.0, rotary_trained_len=16),
+                                dict(H=4, kv=1)])
+@pytest.mark.parametrize("causal,keypad", [(True, True), (True, False), (False, True)])
+def test_stack_against_64_bits(kw, causal, keypad):
+    B, L = 4, 70
+    layers = _stack(**kw)
+    ids, x, up = _batch(B, L)
+    see = torch.ones(L, L, dtype=torch.bool).tril() if causal else torch.ones(L, L, dtype=torch.bool)
+    see = see[None].expand(B, L, L)
+    if keypad:
+        see = see & (ids != 0)[:, None, :]
+    xr = x.double().requires_grad_()
+    want, P = _plain(layers, xr, torch.arange(L).repeat(B), see, B, L)
+    live = (ids.reshape(-1) != 0).double()[:, None] if keypad else torch.ones(B * L, 1).double()
+    wg = dict(zip(["x"] + list(P), torch.autograd.grad(want, [xr] + list(P.values()), up.double() * live)))
+    xd = x.cuda().requires_grad_()
+    y = layers(xd, ids.cuda().reshape(-1), B, L, causal, keypad, {})
+    _near(y, want, STACK_K, "output")
+    params = dict(layers.named_parameters())
+    got = torch.autograd.grad(y, [xd] + list(params.values()), (up.double() * live).float().cuda())
+    for n, t in zip(["x"] + list(params), got):
+        _near(t, wg[n], 4 * STACK_K, n)      # (a gradient passes the forward's stages and its own; sums over 280 rows)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+def test_packed_rows_and_last_rows(causal):
+    """Packed rows give what the padded window gives at its real rows; the last rows alone what the whole stack gives there."""
+    B, L = 4, 70
+    layers = _stack(kv=1).eval()
+    ids, x, up = _batch(B, L, 1)
+    keep = (ids != 0).reshape(-1)
+    cu = torch.cat([torch.zeros(1, dtype=torch.int64), (ids != 0).sum(1).cumsum(0)]).cuda()
+    n = int(cu[-1])
+    rows = (n + 127) // 128 * 128
+    xp = torch.zeros(rows, 64)
+    xp[:n] = x[keep]
+    idd = ids.cuda().reshape(-1)
+    with torch.no_grad():
+        full = layers(x.cuda(), idd, B, L, causal, True, {})
+        pack = layers.forward_packed_train(xp.cuda(), cu, B, L, True, rows_real=n, causal=causal)
+        last = layers.forward_last(x.cuda(), idd, B, L, causal, True, {})
+        plast = layers.forward_last_packed(xp.cuda(), cu, B, L, True, rows_real=n, causal=causal)
+    assert torch.isfinite(pack).all()
+    _near(pack[:n], full[keep.cuda()], STACK_K, "packed")
+    want = full.view(B, L, -1)[:, -1]
+    _near(last, want, STACK_K, "last rows")
+    _near(plast, want, STACK_K, "last packed rows")
+    # training on packed rows: the gradients of the padded window
+    layers.train()
+    xa, xb = x.cuda().requires_grad_(), xp.cuda().requires_grad_()
+    uk = (up * keep[:, None]).cuda()
+    ups = torch.zeros(rows, 64)
+    ups[:n] = up[keep]
+    params = list(layers.parameters())
+    ga = torch.autograd.grad(layers(xa, idd, B, L, causal, True, {}), [xa] + params, uk)
+    cu_tail = torch.cat([cu, torch.tensor([rows], device="cuda")])      # (the unused tail as one more session, as the models' loop hands it over)
+    gb = torch.autograd.grad(layers.forward_packed_train(xb, cu_tail, B + 1, L, True, rows_real=rows, causal=causal), [xb] + params, ups.cuda())
+    _near(gb[0][:n], ga[0][keep.cuda()], 4 * STACK_K, "packed x gradient")
+    for (name, _), a, b in zip(layers.named_parameters(), ga[1:], gb[1:]):
+        _near(b, a, 4 * STACK_K, "packed " + name)
+
+
+def test_operators_captured_and_replayed_beside_eager_work():
+    """Forward and backward of all three in one graph, replayed on new inputs with eager calls between; two graphs do not share scratch."""
+    from rectools_amd import ops
+
+    dev, H, hd, L, d = "cuda", 2, 32, 90, 128
+    freq, _ = ops.rotary_frequencies(16, device=dev)
+    pos = torch.arange(L, device=dev)
+    lam, w = torch.full((H,), 0.4, device=dev), torch.ones(2 * hd, device=dev)
+
+    def step(q, k, v, f, up):
+        a, b = ops.rotary_qk(q, k, pos, freq, 2 * H, 2 * H)
+        o = ops.diff_attention(a, b, v, lam, None, None, 1, H, H, L, L, True, norm_w=w)
+        y, h = ops.norm_gate_residual(o, f, gate=q, post=(scale, None), scale=scale, pre=(scale, None))
+        return (y, h) + torch.autograd.grad((y, h), (q, k, v, f, scale), (up, up))
+
+    def newest(q, k, v):      # one query against many keys: split and joined through scratch
+        with torch.no_grad():
+            return ops.diff_attention(q, k, v, lam, None, None, 1, H, H, 1, k.shape[0], True, norm_w=w)
+
+    scale = torch.rand(d, device=dev).add_(0.5).requires_grad_()
+    g = torch.Generator(device=dev).manual_seed(1)
+    new = lambda n=L: torch.randn(n, d, generator=g, device=dev)   # noqa: E731
+    ins = [new().requires_grad_() for _ in range(4)] + [new()]
+    one = [new(1), new(7000), new(7000)]
+    other = [new(1), new(7000), new(7000)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step(*ins)
+            newest(*one)
+            newest(*other)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    g1, g2 = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g1):
+        out1, one1 = step(*ins), newest(*one)
+    with torch.cuda.graph(g2):
+        one2 = newest(*other)
+    for _ in range(4):
+        with torch.no_grad():
+            for t in ins + one + other:
+                t.copy_(torch.randn(t.shape, generator=g, device=dev))
+        g2.replay()
+        g1.replay()
+        torch.cuda.synchronize()
+        want = step(*[t.detach().clone().requires_grad_() for t in ins[:4]], ins[4])
+        for a, b in zip(out1, want):
+            assert torch.equal(a, b)
+        assert torch.equal(one1, newest(*one)) and torch.equal(one2, newest(*other))
+
+
+def test_operators_on_another_stream():
+    from rectools_amd import ops
+
+    dev, H, hd, n = "cuda", 2, 32, 3000
+    q, k, v = (torch.randn(n, H * 2 * hd, device=dev) for _ in range(3))
+    lam = torch.full((H,), 0.4, device=dev)
+    want = ops.diff_attention(q, k, v, lam, None, None, 10, H, H, 300, 300, True)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = ops.diff_attention(q, k, v, lam, None, None, 10, H, H, 300, 300, True)
+    s.synchronize()
+    assert torch.equal(got, want)
+
+
+def test_no_second_derivative():
+    from rectools_amd import ops
+
+    x = torch.randn(4, 64, device="cuda", requires_grad=True)
+    y, _ = ops.norm_gate_residual(x, x)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(y.sum(), x, create_graph=True)
+
+
+def _dataset():
+    from rectools_amd.dataset import Dataset
+
+    rng = np.random.default_rng(3)
+    n = 4000
+    df = pd.DataFrame({"user_id": rng.integers(0, 120, n), "item_id": rng.integers(0, 90, n) + 100, "weight": 1.0,
+                       "datetime": pd.to_datetime("2022-01-01") + pd.to_timedelta(rng.integers(0, 500_000, n), unit="m")})
+    return Dataset.construct(df)
+
+
+@pytest.mark.parametrize("family,kw", [("sasrec", dict(use_key_padding_mask=True)), ("sasrec", dict(use_key_padding_mask=False, use_pos_emb=False)), ("bert", {})])
+def test_fit_recommend_and_checkpoint(family, kw, tmp_path, monkeypatch):
+    from rectools_amd import models as M
+    from rectools_amd import nn as hnn
+
+    ds = _dataset()
+    cls = M.SASRecModel if family == "sasrec" else M.BERT4RecModel
+    m = cls(n_factors=64, n_blocks=2, n_heads=2, session_max_len=24, lr=0.002, batch_size=48, dropout_rate=0.1, loss="softmax", epochs=1, seed=1, deterministic=True,
+            transformer_layers_type=hnn.DifferentialTransformerLayers, transformer_layers_kwargs=dict(n_kv_heads=1, rotary_part=0.5), **kw).fit(ds)
+    users = ds.user_id_map.external_ids[:40]
+    reco = m.recommend(users=users, dataset=ds, k=5, filter_viewed=True)
+    assert len(reco) == 200 and np.isfinite(reco["score"]).all()
+    m.save_to_checkpoint(str(tmp_path / "m.ckpt"))
+    again = cls.load_from_checkpoint(str(tmp_path / "m.ckpt")).recommend(users=users, dataset=ds, k=5, filter_viewed=True)
+    pd.testing.assert_frame_equal(reco, again)
+    monkeypatch.setenv("RT_PACKED", "0")      # the padded window's last rows: the same encodings up to rounding
+    other = m.recommend(users=users, dataset=ds, k=5, filter_viewed=True)
+    np.testing.assert_allclose(other["score"], reco["score"], rtol=STACK_K, atol=STACK_K * float(reco["score"].abs().max()))
