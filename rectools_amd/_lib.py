@@ -242,6 +242,24 @@ def load() -> ctypes.CDLL:
     return lib
 
 
+_torch_ops = None
+
+
+def torch_ops():
+    """The compiled torch binding (csrc/rt_torch.cpp -> _torch_ops.so), bound to the loaded library."""
+    global _torch_ops
+    if _torch_ops is None:
+        lib = load()
+        try:
+            from . import _torch_ops as mod
+        except ImportError as e:
+            raise HipLibraryError("rectools_amd/_torch_ops.so does not load. Build it with `python -m rectools_amd.build` "
+                                  f"(or `__graft_entry__.build()`): {e}") from e
+        mod.bind(lib._handle, HipLibraryError)   # pylint: disable=protected-access
+        _torch_ops = mod
+    return _torch_ops
+
+
 def check(status: int, what: str) -> None:
     """Map C status codes to the reference's exception types (Errors)."""
     if status == RT_OK:

@@ -43,8 +43,42 @@ def _lib_digest() -> str:
     return h.hexdigest()
 
 
+TORCH_OPS_SRC = os.path.join(CSRC, "rt_torch.cpp")
+TORCH_OPS_PATH = os.path.join(PKG_DIR, "_torch_ops.so")
+HEADER = os.path.join(os.path.dirname(PKG_DIR), "include", "rectools_hip.h")
+
+
+def build_torch_ops(force: bool = False, verbose: bool = False) -> str:
+    """csrc/rt_torch.cpp -> _torch_ops.so: host code only (the torch binding of the operators whose autograd nodes are compiled)."""
+    import sysconfig
+
+    import torch
+    from torch.utils.cpp_extension import include_paths
+
+    lib_dir = os.path.join(os.path.dirname(torch.__file__), "lib")
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-DTORCH_EXTENSION_NAME=_torch_ops",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]   # pylint: disable=protected-access
+    for path in (*include_paths(), "/opt/rocm/include", sysconfig.get_paths()["include"]):
+        cmd += ["-isystem", path]
+    cmd += [TORCH_OPS_SRC, "-o", TORCH_OPS_PATH, f"-L{lib_dir}", "-lc10", "-ltorch_cpu", "-ltorch_python", "-lc10_hip"]
+    h = hashlib.sha1((" ".join(cmd) + torch.__version__).encode())
+    for path in (TORCH_OPS_SRC, HEADER):
+        with open(path, "rb") as f:
+            h.update(f.read())
+    stamp = TORCH_OPS_PATH + ".sha1"
+    if not force and os.path.exists(TORCH_OPS_PATH) and os.path.exists(stamp) and open(stamp).read() == h.hexdigest():
+        return TORCH_OPS_PATH
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    subprocess.check_call(cmd)
+    with open(stamp, "w") as f:
+        f.write(h.hexdigest())
+    return TORCH_OPS_PATH
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
-    """Compile every csrc/*.hip to an object (cached by content hash) and link the shared library."""
+    """Compile every csrc/*.hip to an object (cached by content hash) and link the shared library; compile the torch binding."""
+    build_torch_ops(force, verbose)
     lib_stamp = LIB_PATH + ".sha1"
     lib_dig = _lib_digest()
     if not force and os.path.exists(LIB_PATH) and os.path.exists(lib_stamp) and open(lib_stamp).read() == lib_dig:

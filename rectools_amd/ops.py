@@ -2535,60 +2535,19 @@ def softmax_loss(sess: torch.Tensor, table: torch.Tensor, act_idx: torch.Tensor,
 # --------------------------------------------------------------------------------------------------
 # a differential-attention stack's operators: rotary positions, differential attention, norms with gate and residual scale
 # --------------------------------------------------------------------------------------------------
-def _rows(t: torch.Tensor, what: str, cols: tp.Optional[int] = None) -> torch.Tensor:
-    """A float32 HIP matrix whose rows the kernels can read in place: unit column stride, rows that do not overlap; else a copy."""
-    _chk(t, what)
-    if t.dim() != 2 or (cols is not None and t.shape[1] != cols):
-        raise ValueError(f"{what}: expected [rows, {'columns' if cols is None else cols}], got {tuple(t.shape)}")
-    if t.shape[1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]:
-        t = t.contiguous()
-    return t
-
-
-def _ld(t: torch.Tensor) -> int:
-    return int(t.stride(0)) if t.shape[0] > 1 else int(t.shape[1])
-
-
-def _same_device(what: str, first: torch.Tensor, *others: tp.Optional[torch.Tensor]) -> None:
-    for t in others:
-        if t is not None and t.device != first.device:
-            raise ValueError(f"{what}: tensors on {first.device} and {t.device}")
-
-
-def _ints(t: tp.Optional[torch.Tensor], what: str, n: int) -> tp.Optional[torch.Tensor]:
-    if t is None:
-        return None
-    if t.dtype != torch.int64 or not t.is_cuda or t.dim() != 1 or t.shape[0] != n:
-        raise ValueError(f"{what}: expected {n} int64 values on the HIP device, got {t.dtype} {tuple(t.shape)} on {t.device}")
-    return t.contiguous()
-
-
-def _once(what: str) -> None:
-    """First line of a backward: grad mode is on there only under create_graph (`once_differentiable` costs a launch's host time)."""
-    if torch.is_grad_enabled():
-        raise RuntimeError(f"{what} has no second derivative (create_graph=True)")
-
-
-class _DeviceOf:
-    """`with _DeviceOf(t):` — launches and the current stream are those of t's device; free when it is the current one."""
-
-    __slots__ = ("index", "prev")
-
-    def __init__(self, t: torch.Tensor) -> None:
-        self.index = t.get_device()
-
-    def __enter__(self) -> None:
-        self.prev = torch.cuda.current_device()
-        if self.prev != self.index:
-            torch.cuda.set_device(self.index)
-
-    def __exit__(self, *exc: tp.Any) -> None:
-        if self.prev != self.index:
-            torch.cuda.set_device(self.prev)
-
-
-def _needs_tape(*tensors: tp.Optional[torch.Tensor]) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+# Argument checks, buffers and autograd nodes are compiled (csrc/rt_torch.cpp: the host set the pace of these small launches when they were
+# written here); the kernels are the C entries rt_rotary, rt_diff_lambda_*, rt_diffattn_*, rt_norm_gate_*.  Work is issued on the current
+# stream of the tensors' device; a backward pass of any of them has no second derivative.
+def _native_op(name: str, *args: tp.Any) -> tp.Any:
+    fn = getattr(_lib.torch_ops(), name)
+    if _TIMING is None:
+        return fn(*args)
+    e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    e0.record()
+    out = fn(*args)
+    e1.record()
+    _TIMING.setdefault(name, []).append((e0, e1, None))
+    return out
 
 
 def rotary_frequencies(rot: int, base: float = 10_000.0, scaling: str = "none", factor: float = 1.0, trained_len: int = 4096,
@@ -2617,146 +2576,22 @@ def rotary_frequencies(rot: int, base: float = 10_000.0, scaling: str = "none", 
     return f.to(device) if device is not None else f, gain
 
 
-def _rotary_call(tensors: tp.Sequence[tp.Tuple[tp.Optional[torch.Tensor], int]], pos, freq, hd: int, interleaved: bool, gain: float,
-                 backward: bool) -> tp.List[tp.Optional[torch.Tensor]]:
-    args: tp.List[tp.Any] = []
-    outs: tp.List[tp.Optional[torch.Tensor]] = []
-    for x, heads in tensors:
-        if x is None:
-            args += [None, 0, None, 0, 0]
-            outs.append(None)
-            continue
-        y = x.new_empty(x.shape)
-        args += [x, _ld(x), y, int(y.shape[1]), heads]
-        outs.append(y)
-    with _DeviceOf(pos):
-        _c("rt_rotary", *args, pos, freq, int(pos.shape[0]), hd, 2 * int(freq.shape[0]), int(interleaved), float(gain), int(backward))
-    return outs
-
-
-class _Rotary(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, pos, freq, n_heads, n_kv_heads, hd, interleaved, gain):
-        ctx.save_for_backward(pos, freq)
-        ctx.meta = (n_heads, n_kv_heads, hd, interleaved, gain)
-        ctx.set_materialize_grads(False)
-        q2, k2 = _rotary_call([(q, n_heads), (k, n_kv_heads)], pos, freq, hd, interleaved, gain, False)
-        return q2 if k is None else (q2, k2)
-
-    @staticmethod
-    def backward(ctx, gq, gk=None):
-        _once("rotary")
-        pos, freq = ctx.saved_tensors
-        n_heads, n_kv_heads, hd, interleaved, gain = ctx.meta
-        if gq is None and gk is None:
-            return (None,) * 9
-        gq, gk = (None if g is None else _rows(g, "rotary gradient") for g in (gq, gk))
-        dq, dk = _rotary_call([(gq, n_heads), (gk, n_kv_heads)], pos, freq, hd, interleaved, gain, True)
-        return (dq, dk) + (None,) * 7
-
-
-def _rotary_args(q, k, pos, freq, n_heads, n_kv_heads):
-    if n_heads <= 0 or (k is not None and n_kv_heads <= 0):
-        raise ValueError(f"rotary: head counts must be positive, got {n_heads} and {n_kv_heads}")
-    q = _rows(q, "rotary")
-    M, cols = q.shape
-    if cols % n_heads != 0 or cols == 0:
-        raise ValueError(f"rotary: {cols} columns do not split into {n_heads} heads")
-    hd = cols // n_heads
-    if k is not None:
-        k = _rows(k, "rotary", n_kv_heads * hd)
-        if k.shape[0] != M:
-            raise ValueError(f"rotary: {M} query rows and {k.shape[0]} key rows")
-    pos = _ints(pos, "rotary positions", M)
-    if freq.dtype != torch.float64 or freq.dim() != 1 or not freq.is_cuda or not 0 < 2 * int(freq.shape[0]) <= hd:
-        raise ValueError(f"rotary: expected at most {hd // 2} float64 frequencies on the HIP device (rotary_frequencies), got {freq.dtype} "
-                         f"{tuple(freq.shape)} on {freq.device}")
-    _same_device("rotary", q, k, pos, freq)
-    return q, k, pos, freq.contiguous(), hd
-
-
 def rotary(x: torch.Tensor, positions: torch.Tensor, freq: torch.Tensor, n_heads: int, interleaved: bool = False, gain: float = 1.0) -> torch.Tensor:
     """Rotary positions on x [M, n_heads * hd] (a column block of a wider matrix is read in place): the first 2 * len(freq) columns of every
     head turn by positions[row] * freq; interleaved pairs (2 j, 2 j + 1) or halves (j, j + rot / 2).  positions [M] int64."""
-    x, _, positions, freq, hd = _rotary_args(x, None, positions, freq, n_heads, 0)
-    return _Rotary.apply(x, None, positions, freq, n_heads, 0, hd, bool(interleaved), float(gain))
+    return _native_op("rotary", x, None, positions, freq, n_heads, 0, interleaved, gain)[0]
 
 
 def rotary_qk(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, freq: torch.Tensor, n_heads: int, n_kv_heads: int,
               interleaved: bool = False, gain: float = 1.0) -> tp.Tuple[torch.Tensor, torch.Tensor]:
     """`rotary` of the queries and the keys of the same rows in one launch (their sines and cosines are shared)."""
-    q, k, positions, freq, hd = _rotary_args(q, k, positions, freq, n_heads, n_kv_heads)
-    return _Rotary.apply(q, k, positions, freq, n_heads, n_kv_heads, hd, bool(interleaved), float(gain))
-
-
-class _DiffLambda(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q1, k1, q2, k2, init):
-        H, hd = q1.shape
-        lam = torch.empty((H,), dtype=torch.float32, device=q1.device)
-        with _DeviceOf(q1):
-            _c("rt_diff_lambda_fwd", q1, k1, q2, k2, float(init), H, hd, lam)
-        ctx.save_for_backward(q1, k1, q2, k2)
-        return lam
-
-    @staticmethod
-    def backward(ctx, g):
-        _once("diff_lambda")
-        q1, k1, q2, k2 = ctx.saved_tensors
-        H, hd = q1.shape
-        outs = q1.new_empty((4, H, hd)).unbind(0)
-        with _DeviceOf(q1):
-            _c("rt_diff_lambda_bwd", g.contiguous(), q1, k1, q2, k2, H, hd, *outs)
-        return (*outs, None)
+    q2, k2 = _native_op("rotary", q, k, positions, freq, n_heads, n_kv_heads, interleaved, gain)
+    return q2, k2
 
 
 def diff_lambda(q1: torch.Tensor, k1: torch.Tensor, q2: torch.Tensor, k2: torch.Tensor, init: float) -> torch.Tensor:
     """The weight of the second softmax map of every head, [H] = exp(q1 . k1) - exp(q2 . k2) + init over learned [H, hd] vectors."""
-    vs = [_chk(t, "diff_lambda") for t in (q1, k1, q2, k2)]
-    if q1.dim() != 2 or any(t.shape != q1.shape for t in vs) or q1.shape[1] == 0:
-        raise ValueError(f"diff_lambda: four [heads, columns] matrices of one shape, got {[tuple(t.shape) for t in vs]}")
-    _same_device("diff_lambda", *vs)
-    return _DiffLambda.apply(*(t.contiguous() for t in vs), float(init))
-
-
-def _diff_attention_fwd(q, k, v, lam, cu_q, cu_k, key_ids, norm_w, meta, train):
-    B, H, Hkv, hd, Lq, Lk, causal, scale, out_scale, eps = meta
-    Nq, Nk = int(q.shape[0]), int(k.shape[0])
-    y = torch.empty((Nq, 2 * H * hd), dtype=torch.float32, device=q.device)
-    o12 = torch.empty((Nq, H, 2, 2 * hd), dtype=torch.float32, device=q.device) if train else None
-    lse = torch.empty((Nq, H, 2), dtype=torch.float32, device=q.device) if train else None
-    with _DeviceOf(q):
-        n = _lib.load().rt_diffattn_fwd_workspace_bytes(B, H, Hkv, hd, Lq, Lk, Nq, int(train))
-        ws = torch.empty((n,), dtype=torch.uint8, device=q.device) if n > 0 else None
-        _c("rt_diffattn_fwd", q, _ld(q), k, _ld(k), v, _ld(v), lam, cu_q, cu_k, key_ids, B, H, Hkv, hd, Lq, Lk, Nq, Nk, scale, causal, norm_w,
-           out_scale, eps, y, int(y.shape[1]), o12, lse, ws, n)
-    return y, o12, lse
-
-
-class _DiffAttention(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, lam, cu_q, cu_k, key_ids, norm_w, meta):
-        y, o12, lse = _diff_attention_fwd(q, k, v, lam, cu_q, cu_k, key_ids, norm_w, meta, True)
-        ctx.save_for_backward(q, k, v, lam, cu_q, cu_k, key_ids, norm_w, o12, lse)
-        ctx.meta = meta
-        return y
-
-    @staticmethod
-    def backward(ctx, dy):
-        _once("diff_attention")
-        q, k, v, lam, cu_q, cu_k, key_ids, norm_w, o12, lse = ctx.saved_tensors
-        B, H, Hkv, hd, Lq, Lk, causal, scale, out_scale, eps = ctx.meta
-        Nq, Nk = int(q.shape[0]), int(k.shape[0])
-        dy = _rows(dy, "diff_attention gradient")
-        dq, dk, dv = (t.new_empty(t.shape) for t in (q, k, v))
-        dlam = lam.new_empty((H,))
-        dw = None if norm_w is None else lam.new_empty((2 * hd,))
-        with _DeviceOf(q):
-            n = _lib.load().rt_diffattn_bwd_workspace_bytes(H, hd, max(Nq, 1))
-            ws = torch.empty((n,), dtype=torch.uint8, device=q.device)
-            _c("rt_diffattn_bwd", q, _ld(q), k, _ld(k), v, _ld(v), lam, cu_q, cu_k, key_ids, B, H, Hkv, hd, Lq, Lk, Nq, Nk, scale, causal,
-               norm_w, out_scale, eps, o12, lse, dy, _ld(dy), dq, 2 * H * hd, dk, 2 * Hkv * hd, dv, 2 * Hkv * hd, dlam, dw, ws, n)
-        return dq, dk, dv, dlam, None, None, None, dw, None
+    return _native_op("diff_lambda", q1, k1, q2, k2, init)
 
 
 def diff_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam: torch.Tensor, cu_q: tp.Optional[torch.Tensor],
@@ -2771,72 +2606,7 @@ def diff_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam: torch
     launch; longer ones are served).  None: B sessions of exactly Lq / Lk rows.  The last query of a session meets its last key: with
     causal, key j is seen by query i iff j <= i + nk - nq — so Lq = 1 is the newest row of a stored session.  key_ids [Nk] int64: keys with
     id 0 are masked, whatever their rows hold.  A query that sees no key gives zeros; so do rows behind the last session of cu_q."""
-    if B < 0 or H <= 0 or H_kv <= 0 or H % H_kv != 0 or Lq < 0 or Lk < 0:
-        raise ValueError(f"diff_attention: B={B}, H={H}, H_kv={H_kv}, Lq={Lq}, Lk={Lk}")
-    q = _rows(q, "diff_attention q")
-    if q.shape[1] == 0 or q.shape[1] % (2 * H) != 0:
-        raise ValueError(f"diff_attention: {q.shape[1]} query columns do not split into {H} heads of two maps")
-    hd = int(q.shape[1]) // (2 * H)
-    if hd > 64:
-        raise NotImplementedError(f"diff_attention: at most 64 columns per map (128 value columns per head), got {hd}")
-    k, v = _rows(k, "diff_attention k", 2 * H_kv * hd), _rows(v, "diff_attention v", 2 * H_kv * hd)
-    if k.shape[0] != v.shape[0]:
-        raise ValueError(f"diff_attention: {k.shape[0]} key rows and {v.shape[0]} value rows")
-    for t, cu, L, what in ((q, cu_q, Lq, "query"), (k, cu_k, Lk, "key")):
-        if cu is None and t.shape[0] != B * L:
-            raise ValueError(f"diff_attention: {t.shape[0]} {what} rows for {B} sessions of {L}")
-    cu_q, cu_k = _ints(cu_q, "diff_attention cu_q", B + 1), _ints(cu_k, "diff_attention cu_k", B + 1)
-    key_ids = _ints(key_ids, "diff_attention key_ids", int(k.shape[0]))
-    lam = _chk(lam, "diff_attention lam").contiguous()
-    if tuple(lam.shape) != (H,):
-        raise ValueError(f"diff_attention: lam has one value per head, got {tuple(lam.shape)}")
-    if norm_w is not None:
-        norm_w = _chk(norm_w, "diff_attention norm_w").contiguous()
-        if tuple(norm_w.shape) != (2 * hd,):
-            raise ValueError(f"diff_attention: norm_w has {2 * hd} values, got {tuple(norm_w.shape)}")
-    if scale is not None and not scale > 0.0:
-        raise ValueError(f"diff_attention: the logit scale is positive, got {scale}")
-    _same_device("diff_attention", q, k, v, lam, cu_q, cu_k, key_ids, norm_w)
-    meta = (int(B), int(H), int(H_kv), hd, int(Lq), int(Lk), int(bool(causal)), 0.0 if scale is None else float(scale), float(out_scale), float(eps))
-    if not _needs_tape(q, k, v, lam, norm_w):
-        return _diff_attention_fwd(q, k, v, lam, cu_q, cu_k, key_ids, norm_w, meta, False)[0]
-    return _DiffAttention.apply(q, k, v, lam, cu_q, cu_k, key_ids, norm_w, meta)
-
-
-class _NormGate(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, f, z, scale, pw, pb, nw, nb, layer, alpha, eps, p, tape):
-        M, d = x.shape
-        y = torch.empty_like(x)
-        h = torch.empty_like(x) if nw is not None else None
-        stat = torch.empty((M, 4), dtype=torch.float32, device=x.device) if tape else None
-        seed, sid = RNG.next() if p > 0 else (0, 0)
-        with _DeviceOf(x):
-            _c("rt_norm_gate_fwd", x, f, z, scale, pw, pb, nw, nb, layer, alpha, eps, p, seed, sid, M, d, y, h, stat)
-        ctx.save_for_backward(y if h is not None else None, f, z, scale, pw, pb, nw, stat)
-        ctx.meta = (layer, alpha, p, seed, sid, nb is not None)
-        ctx.set_materialize_grads(False)
-        return y if h is None else (y, h)
-
-    @staticmethod
-    def backward(ctx, gy, gh=None):
-        _once("norm_gate_residual")
-        y, f, z, scale, pw, pb, nw, stat = ctx.saved_tensors
-        layer, alpha, p, seed, sid, has_nb = ctx.meta
-        if gy is None and gh is None:
-            return (None,) * 13
-        M, d = f.shape
-        gy, gh = (None if g is None else g.contiguous() for g in (gy, gh))
-        dx, df = torch.empty_like(f), torch.empty_like(f)
-        dz = None if z is None else torch.empty_like(f)
-        there = (scale is not None, pw is not None, pb is not None, nw is not None, has_nb)
-        ds, dpw, dpb, dnw, dnb = (f.new_empty((d,)) if t else None for t in there)
-        with _DeviceOf(f):
-            n = _lib.load().rt_norm_gate_bwd_workspace_bytes(M, d)
-            ws = torch.empty((max(n, 16),), dtype=torch.uint8, device=f.device)
-            _c("rt_norm_gate_bwd", gy, gh, y if gh is not None else None, f, z, scale, pw, pb, nw, layer, alpha, p, seed, sid, M, d, stat, dx, df, dz,
-               ds, dpw, dpb, dnw, dnb, ws, n)
-        return (dx, df, dz, ds, dpw, dpb, dnw, dnb) + (None,) * 5
+    return _native_op("diff_attention", q, k, v, lam, cu_q, cu_k, B, H, H_kv, Lq, Lk, causal, key_ids, norm_w, out_scale, eps, scale)
 
 
 NormParams = tp.Tuple[torch.Tensor, tp.Optional[torch.Tensor]]
@@ -2853,23 +2623,12 @@ def norm_gate_residual(x: torch.Tensor, f: torch.Tensor, gate: tp.Optional[torch
         raise ValueError(f"norm_gate_residual: kind is 'rms' or 'layer', got {kind!r}")
     if not 0.0 <= p < 1.0:
         raise ValueError(f"norm_gate_residual: dropout rate in [0, 1), got {p}")
-    _chk(x, "norm_gate_residual x")
-    if x.dim() != 2 or x.shape[1] == 0:
-        raise ValueError(f"norm_gate_residual: expected [rows, columns], got {tuple(x.shape)}")
-    d = int(x.shape[1])
-    if d > 8192:
-        raise NotImplementedError(f"norm_gate_residual: rows of at most 8,192 columns, got {d}")
-    if kind == "rms" and any(n is not None and n[1] is not None for n in (post, pre)):
-        raise ValueError("norm_gate_residual: the root-mean-square norm has no bias")
     pw, pb = post if post is not None else (None, None)
     nw, nb = pre if pre is not None else (None, None)
     if (post is not None and pw is None) or (pre is not None and nw is None):
         raise ValueError("norm_gate_residual: a norm needs its weight")
-    rows, cols = [x, f, gate], [scale, pw, pb, nw, nb]
-    for t, shape in [(t, tuple(x.shape)) for t in rows] + [(t, (d,)) for t in cols]:
-        if t is not None and tuple(_chk(t, "norm_gate_residual").shape) != shape:
-            raise ValueError(f"norm_gate_residual: expected {shape}, got {tuple(t.shape)}")
-    _same_device("norm_gate_residual", x, *rows[1:], *cols)
-    rows, cols = ([None if t is None else t.contiguous() for t in ts] for ts in (rows, cols))
-    out = _NormGate.apply(*rows, *cols, int(kind == "layer"), float(alpha), float(eps), float(p), _needs_tape(*rows, *cols))
-    return out if pre is not None else (out, None)
+    if kind == "rms" and (pb is not None or nb is not None):
+        raise ValueError("norm_gate_residual: the root-mean-square norm has no bias")
+    seed, sid = RNG.next() if p > 0 else (0, 0)
+    out = _native_op("norm_gate", x, f, gate, scale, pw, pb, nw, nb, kind == "layer", alpha, eps, p, seed, sid)
+    return out[0], out[1] if pre is not None else None
