@@ -763,19 +763,21 @@ int rt_diff_lambda_bwd(const float* dlam, const float* q1, const float* k1, cons
  * rows (then Nq == B * Lq, Nk == B * Lk).  With cu, Lq / Lk are the expected longest sessions (longer ones are served all the same).  The last
  * query of a session is aligned with its last key: causal = key j is seen by query i iff j <= i + nk - nq.  key_ids (null or [Nk]): keys with id 0
  * are masked.  A query that sees no key gives 0.  scale <= 0: 1 / sqrt(hd).  Rows behind the last session of cu_q are written as zeros.
- * o12 [Nq, H, 2, 2 hd] and lse [Nq, H, 2]: both or neither; what the backward pass reads.  ws: rt_diffattn_fwd_workspace_bytes(train = o12 given). */
-size_t rt_diffattn_fwd_workspace_bytes(int32_t B, int32_t H, int32_t Hkv, int32_t hd, int32_t Lq, int32_t Lk, int64_t Nq, int32_t train);
+ * saved (null without a backward pass): rt_diffattn_saved_bytes, 16-byte aligned, kept as it is for rt_diffattn_bwd.  ws:
+ * rt_diffattn_fwd_workspace_bytes (train = saved given), 16-byte aligned, free again behind the launch. */
+size_t rt_diffattn_saved_bytes(int32_t H, int32_t Hkv, int32_t hd, int64_t Nq, int64_t Nk);
+size_t rt_diffattn_fwd_workspace_bytes(int32_t B, int32_t H, int32_t Hkv, int32_t hd, int32_t Lq, int32_t Lk, int64_t Nq, int64_t Nk, int32_t train);
 int rt_diffattn_fwd(const float* q, int64_t ldq, const float* k, int64_t ldk, const float* v, int64_t ldv, const float* lam, const int64_t* cu_q,
                     const int64_t* cu_k, const int64_t* key_ids, int32_t B, int32_t H, int32_t Hkv, int32_t hd, int32_t Lq, int32_t Lk, int64_t Nq,
-                    int64_t Nk, float scale, int32_t causal, const float* norm_w, float out_scale, float eps, float* y, int64_t ldy, float* o12,
-                    float* lse, void* ws, size_t ws_bytes, rt_stream_t stream);
-/* Gradients of q, k, v, lam and norm_w (dw null iff norm_w null) from dy; every element of dq, dk, dv, dlam, dw is written. */
+                    int64_t Nk, float scale, int32_t causal, const float* norm_w, float out_scale, float eps, float* y, int64_t ldy, void* saved,
+                    size_t saved_bytes, void* ws, size_t ws_bytes, rt_stream_t stream);
+/* Gradients of q, k, v, lam and norm_w (dw null iff norm_w null) from dy and what the forward call saved; every element of dq, dk, dv, dlam, dw
+ * is written. */
 size_t rt_diffattn_bwd_workspace_bytes(int32_t H, int32_t hd, int64_t Nq);
-int rt_diffattn_bwd(const float* q, int64_t ldq, const float* k, int64_t ldk, const float* v, int64_t ldv, const float* lam, const int64_t* cu_q,
-                    const int64_t* cu_k, const int64_t* key_ids, int32_t B, int32_t H, int32_t Hkv, int32_t hd, int32_t Lq, int32_t Lk, int64_t Nq,
-                    int64_t Nk, float scale, int32_t causal, const float* norm_w, float out_scale, float eps, const float* o12, const float* lse,
-                    const float* dy, int64_t lddy, float* dq, int64_t lddq, float* dk, int64_t lddk, float* dv, int64_t lddv, float* dlam,
-                    float* dw, void* ws, size_t ws_bytes, rt_stream_t stream);
+int rt_diffattn_bwd(const void* saved, size_t saved_bytes, const float* lam, const int64_t* cu_q, const int64_t* cu_k, const int64_t* key_ids, int32_t B,
+                    int32_t H, int32_t Hkv, int32_t hd, int32_t Lq, int32_t Lk, int64_t Nq, int64_t Nk, float scale, int32_t causal, const float* norm_w,
+                    float out_scale, float eps, const float* dy, int64_t lddy, float* dq, int64_t lddq, float* dk, int64_t lddk, float* dv, int64_t lddv,
+                    float* dlam, float* dw, void* ws, size_t ws_bytes, rt_stream_t stream);
 
 /* The norm behind a block, its gate, its residual scale and the norm in front of the next block: n = N_post(f), y = alpha x + scale * sigmoid(z) *
  * drop(n), h = N_pre(y) over contiguous [M, d] rows, d <= 8192.  layer = 1: LayerNorm, 0: root mean square.  post_w / pre_w null: that norm is left

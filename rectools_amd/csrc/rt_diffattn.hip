@@ -5,26 +5,37 @@
 // q rows carry [H][2][hd] columns (the two maps' queries of a head next to each other), k rows [Hkv][2][hd], v rows [Hkv][2 hd]; query head
 // h reads key head h / (H / Hkv).  Sessions are packed rows (cu) or equal windows; inside a session the last query is aligned with the last
 // key (causal: key j is seen by query i iff j <= i + nk - nq), so one launch serves whole sessions and the newest rows of stored ones.
-// Keys whose item id is 0 are masked; their K and V rows are replaced by zeros when they are staged, whatever they hold.  A query that
-// sees no key has o = 0, y = 0 and no gradients.
+// Keys whose item id is 0 are masked, whatever their rows hold.  A query that sees no key has o = 0, y = 0 and no gradients.
 //
-// Arithmetic: fp32 in, fp32 out.  The products run on the bf16 matrix instructions, six terms of an exact three-way split per product
-// (rt_attn_planes.h: split2): h m l are the top, middle and low 8 bits of the significand, the dropped terms are below 2^-24 of the product.
-// Softmax statistics, sums and accumulators are fp32.  Scores live in the base-2 domain.
+// Arithmetic: fp32 in, fp32 out.  A product runs on the fp16 matrix instruction as three terms of a two-way split: x = 2^e (h + l), e from the
+// largest magnitude of the row, h = fp16(x 2^-e), l = fp16 of the rest; x y ~ h h' + h l' + l h'.  h and l hold 11 bits each and a sign, so x
+// is held to 2^-22 of its row's largest value and the dropped l l' is below 2^-22 of the product: rounding of the size fp32 sums of
+// this length carry themselves (measured against 64 bits: DESIGN of the tests).  Three bf16 planes, the exact split, need six terms: twice the matrix work, 1.5 x the
+// LDS traffic and the registers (the dK/dV kernel spilled 263 registers at hd 64), and were measured 1.9 - 2.6 x slower.
+// The split is made ONCE per call by diff_planes_kernel (one pass over q, k, v: memory bound), not at every staging: a 4,096-row session
+// stages each of its rows 64 times.  Softmax statistics, sums and accumulators are fp32; scores live in the base-2 domain.
 //
-// Geometry: a workgroup is 4 waves = 2 row groups of 32 owner rows x the 2 maps; v_mfma_f32_32x32x16_bf16 tiles, the OWNER row (a query;
+// Geometry: a workgroup is 4 waves = 2 row groups of 32 owner rows x the 2 maps; v_mfma_f32_32x32x16_f16 tiles, the OWNER row (a query;
 // in the dK/dV pass a key) is the lane, the partner rows are the registers, so probabilities and dS feed the next product from the
-// registers they were made in.  Partner rows stream through LDS 32 at a time as plane images, both maps' waves read the same V.
-// One wave per map rather than one wave for both: its operands and accumulators are half as many registers, which leaves two waves on a
-// SIMD (one's softmax runs under the other's products).
+// registers they were made in.  One wave per map rather than one wave for both: its operands and accumulators are half as many registers, which
+// leaves two waves on a SIMD (one's softmax runs under the other's products).  Partner rows stream through LDS 32 at a time, copied as they
+// lie by LDS DMA (global_load_lds: no registers, no address arithmetic): the planes are stored head-major with 16 bytes behind every row,
+// so rows lie an odd number of 16-byte units apart and both read patterns (32 rows of 16 bytes; 4-row transpose blocks) spread over the banks.
 #include "rt_attn_planes.h"
 
 namespace {
-using namespace rt_planes;
+using rt_planes::LOG2E;
+using rt_planes::s16x4;
+using rt_planes::tr_read;
+
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+typedef short s16x8v __attribute__((ext_vector_type(8)));
 
 constexpr int NT = 256;
 constexpr int OWN = 64;    // owner rows per workgroup
 constexpr int CH = 32;     // partner rows per staged chunk
+constexpr int PAD = 32;    // rows behind the last one that a chunk may copy (never used)
 
 struct Args {
   const float* q; const float* k; const float* v; long long ldq, ldk, ldv;
@@ -35,15 +46,20 @@ struct Args {
   float scale; int causal;
   const float* norm_w; float out_scale, eps;
   float* y; long long ldy;
+  // planes: rows of [map 1: h | l][map 2: h | l] (q, k) or [h | l] (v, dO), 8 HD bytes + 16, head-major with N + PAD rows per head; scales 2^e
+  unsigned char* qp; unsigned char* kp; unsigned char* vp; unsigned char* dp;
+  float* qs; float* ks;                  // [H][2][Nq + PAD], [Hkv][2][Nk + PAD]
+  float* vs; float* ivs; float* lvb;     // [Hkv][Nk + PAD]: 2^e, 2^-e, e (minus infinity: the key is masked)
+  float* ds;                             // [H][Nq + PAD]
   float* o12;                            // [Nq, H, 2, 2 hd] normalised outputs of the two maps (training)
-  float* lse;                            // [Nq, H, 2] log2-sum-exp2 of the two maps (training)
+  float* lse;                            // [H][2][Nq + PAD] log2-sum-exp2 of the two maps (training)
   float* part; float* ml;                // split keys: [n_split, Nq, H, 2, 2 hd] and [n_split, Nq, H, 2, 2] (maximum, sum)
   int n_split;
   int n_tiles;                           // owner tiles per session in the grid (longer sessions loop)
   // backward
-  const float* dout; long long lddo;     // gradient of o, [Nq, H * 2 hd] (the pass in front makes it)
-  const float* delta;                    // [Nq, H, 2]
-  float* dq; float* dk; float* dv; long long lddq, lddk, lddv;
+  float* delta;                          // [H][2][Nq + PAD]
+  float* dq; float* dk; float* dv; long long lddq, lddk, lddv; int vec_q, vec_kv;
+  int vec_y;
 };
 
 __device__ __forceinline__ void rows_of(const long long* cu, int b, int len, long long N, long long& row0, int& n) {
@@ -64,146 +80,218 @@ __device__ __forceinline__ long long rows_used(const long long* cu, int B, long 
   return e < 0 ? 0 : (e > N ? N : e);
 }
 
-// LDS images: row r = [h | m | l] planes of C bf16 columns + 16 bytes, so that rows lie an odd number of 16-byte units apart: the 32-row
-// b128 fragment reads and the 4-row transpose reads both spread over the banks, with constant offsets and no address arithmetic.
-template <int C> struct Img {
-  static constexpr int PLANE = C * 2, ROW = 3 * PLANE + 16, BYTES = CH * ROW;
-};
-
-// ncol columns of up to CH rows -> image; rows whose bit in `live` is 0 and columns behind ncol are zeros
-template <int C, int MODE>
-__device__ __forceinline__ void stage(const float* __restrict__ src, long long ld, int ncol, unsigned live, float scale, unsigned char* img, int tid) {
-  constexpr int C4 = C / 4, U = CH * C4 / NT;
-  f32x4 x[U];
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int idx = tid + u * NT, r = idx / C4, c = (idx % C4) * 4;
-    x[u] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if ((live >> r) & 1u) {
-      const float* p = src + (long long)r * ld + c;
-      if (MODE < 2) {
-        if (MODE == 0 || c < ncol) x[u] = *reinterpret_cast<const f32x4*>(p);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (c + j < ncol) x[u][j] = p[j];
-      }
-    }
-  }
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int idx = tid + u * NT, r = idx / C4, c = (idx % C4) * 4;
-    const f32x4 t = x[u] * scale;
-    unsigned h0, m0, l0, h1, m1, l1;
-    split2(t[0], t[1], h0, m0, l0);
-    split2(t[2], t[3], h1, m1, l1);
-    unsigned char* p = img + r * Img<C>::ROW + c * 2;
-    *reinterpret_cast<u32x2*>(p) = u32x2{h0, h1};
-    *reinterpret_cast<u32x2*>(p + Img<C>::PLANE) = u32x2{m0, m1};
-    *reinterpret_cast<u32x2*>(p + 2 * Img<C>::PLANE) = u32x2{l0, l1};
-  }
+template <int CTRL> __device__ __forceinline__ float dpp(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, true));
 }
-
-// 8 values of one global row at columns c .. c + 7 (zeros behind ncol), times scale, as planes
-template <int MODE>
-__device__ __forceinline__ P3 load_planes(const float* __restrict__ row, int c, int ncol, bool ok, float scale) {
-  float x[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) x[j] = 0.f;
-  if (ok) {
-    if (MODE < 2) {
-#pragma unroll
-      for (int j = 0; j < 8; j += 4)
-        if (MODE == 0 || c + j < ncol) {
-          const f32x4 t = *reinterpret_cast<const f32x4*>(row + c + j);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[j + e] = t[e] * scale;
-        }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (c + j < ncol) x[j] = row[c + j] * scale;
-    }
-  }
-  return split8(x);
+__device__ __forceinline__ float lane_xor16(float v) { return __builtin_bit_cast(float, __builtin_amdgcn_ds_swizzle(__builtin_bit_cast(int, v), 0x401F)); }
+template <int LANES> __device__ __forceinline__ float group_sum(float v) {      // 8, 16 or 32 neighbouring lanes
+  v += dpp<0xB1>(v);       // lane ^ 1
+  v += dpp<0x4E>(v);       // lane ^ 2
+  v += dpp<0x141>(v);      // mirrored in 8 lanes
+  if (LANES > 8) v += dpp<0x140>(v);      // mirrored in 16 lanes
+  if (LANES > 16) v += lane_xor16(v);
+  return v;
 }
-
-__device__ __forceinline__ f32x16 mfma6(const P3& A, const P3& B, f32x16 acc) {
-  acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A.l, B.h, acc, 0, 0, 0);
-  acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A.h, B.l, acc, 0, 0, 0);
-  acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A.m, B.m, acc, 0, 0, 0);
-  acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A.m, B.h, acc, 0, 0, 0);
-  acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A.h, B.m, acc, 0, 0, 0);
-  acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A.h, B.h, acc, 0, 0, 0);
-  return acc;
+template <int LANES> __device__ __forceinline__ float group_max(float v) {
+  v = fmaxf(v, dpp<0xB1>(v));
+  v = fmaxf(v, dpp<0x4E>(v));
+  v = fmaxf(v, dpp<0x141>(v));
+  if (LANES > 8) v = fmaxf(v, dpp<0x140>(v));
+  if (LANES > 16) v = fmaxf(v, lane_xor16(v));
+  return v;
 }
-
-// acc[r] += sum_c img[row(r)][c0 + c] * own[c], row(r) = 8 (r / 4) + 4 g + r % 4: the partner rows are the registers, the owner the lane
-template <int C, int NS>
-__device__ __forceinline__ void rows_dot(const unsigned char* img, int c0, const P3 (&own)[NS], int i, int g, f32x16& acc) {
-  const unsigned char* p = img + i * Img<C>::ROW + c0 * 2 + 16 * g;
-#pragma unroll
-  for (int s = 0; s < NS; ++s) {
-    P3 A;
-    A.h = *reinterpret_cast<const bf16x8*>(p + 32 * s);
-    A.m = *reinterpret_cast<const bf16x8*>(p + 32 * s + Img<C>::PLANE);
-    A.l = *reinterpret_cast<const bf16x8*>(p + 32 * s + 2 * Img<C>::PLANE);
-    acc = mfma6(A, own[s], acc);
-  }
-}
-
-// acc[cb][r] += sum over the 32 partner rows of img[row][c0 + 32 cb + col(r)] * w[row], the lane's weights in the accumulator order of rows_dot
-// (slot j of step t = register 8 t + j = row 16 t + 8 (j / 4) + 4 g + j % 4): the partner rows are the reduction index, read transposed
-template <int C, int NB>
-__device__ __forceinline__ void cols_dot(const unsigned char* img, int c0, const P3 (&w)[2], int lane, f32x16 (&acc)[NB]) {
-  const int g = lane >> 5;
-  const unsigned char* p = img + (4 * g + ((lane & 15) >> 2)) * Img<C>::ROW + (c0 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3)) * 2;
-#pragma unroll
-  for (int t = 0; t < 2; ++t)
-#pragma unroll
-    for (int cb = 0; cb < NB; ++cb) {
-      const unsigned char* a = p + 16 * t * Img<C>::ROW + 64 * cb;
-      const unsigned char* b = a + 8 * Img<C>::ROW;
-      P3 A;
-      A.h = __builtin_bit_cast(bf16x8, (s16x8)__builtin_shufflevector(tr_read(a), tr_read(b), 0, 1, 2, 3, 4, 5, 6, 7));
-      A.m = __builtin_bit_cast(bf16x8, (s16x8)__builtin_shufflevector(tr_read(a + Img<C>::PLANE), tr_read(b + Img<C>::PLANE), 0, 1, 2, 3, 4, 5, 6, 7));
-      A.l = __builtin_bit_cast(bf16x8, (s16x8)__builtin_shufflevector(tr_read(a + 2 * Img<C>::PLANE), tr_read(b + 2 * Img<C>::PLANE), 0, 1, 2, 3, 4, 5, 6, 7));
-      acc[cb] = mfma6(A, w[t], acc[cb]);
-    }
-}
-
-__device__ __forceinline__ void split16(const float (&x)[16], P3 (&out)[2]) {
-#pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    const float y[8] = {x[8 * t], x[8 * t + 1], x[8 * t + 2], x[8 * t + 3], x[8 * t + 4], x[8 * t + 5], x[8 * t + 6], x[8 * t + 7]};
-    out[t] = split8(y);
-  }
-}
-__device__ __forceinline__ int reg_row(int r, int g) { return 8 * (r >> 2) + 4 * g + (r & 3); }
-__device__ __forceinline__ f32x16 zero16() { f32x16 z; for (int r = 0; r < 16; ++r) z[r] = 0.f; return z; }
-
-// bit j: key t0 + j exists and is not masked
-__device__ __forceinline__ unsigned live_keys(const Args& a, long long row0, int t0, int n, int lane) {
-  const int left = n - t0;
-  unsigned bits = left >= 32 ? 0xFFFFFFFFu : (left <= 0 ? 0u : (1u << left) - 1u);
-  if (a.key_ids != nullptr) {
-    const int j = lane & 31;
-    const bool on = j < left && a.key_ids[row0 + t0 + j] != 0;
-    bits = (unsigned)__ballot(on);
-  }
-  return bits;
-}
-
-template <int MODE>
-__device__ __forceinline__ void put4(float* row, int c, int ncol, f32x4 x) {
+template <int MODE>      // 0 the row fills its columns, 1 aligned, 2 single columns
+__device__ __forceinline__ f32x4 get4(const float* p, int c, int ncol) {
+  f32x4 x{0.f, 0.f, 0.f, 0.f};
   if (MODE < 2) {
-    if (MODE == 0 || c < ncol) *reinterpret_cast<f32x4*>(row + c) = x;
+    if (MODE == 0 || c < ncol) x = *reinterpret_cast<const f32x4*>(p + c);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (c + e < ncol) x[e] = p[c + e];
+  }
+  return x;
+}
+__device__ __forceinline__ void put4(float* row, int c, int ncol, f32x4 x, bool vec) {
+  if (vec) {
+    if (c < ncol) *reinterpret_cast<f32x4*>(row + c) = x;
   } else {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
       if (c + j < ncol) row[c + j] = x[j];
   }
 }
+
+// ---- the planes --------------------------------------------------------------------------------------------------------------------------
+template <int HD> struct Row {
+  static constexpr int BYTES = 8 * HD + 16, CHUNK = CH * BYTES, UNITS = CHUNK / 16;      // UNITS of 16 bytes per chunk
+};
+// exponent of the row's scale: its largest magnitude comes to 2^13 .. 2^14 (2 x below the fp16 range; what is 2^-18 of it keeps all 22 bits)
+// `least`: values below 2^(least + 14) lose bits.  -126 keeps 2^e a normal number; v takes -80, so that a row sum of weights that carry 2^-e
+// stays finite over any number of keys.
+__device__ __forceinline__ int row_exp(float top, int least) {
+  if (!(top > 0.f) || top > 3.0e38f) return 0;      // a zero row; infinities and NaN stay what they are
+  const int e = __builtin_amdgcn_frexp_expf(top) - 14;
+  return e < least ? least : e;
+}
+__device__ __forceinline__ float pow2(int e) { return __builtin_amdgcn_ldexpf(1.f, e); }
+// four columns of a row, scaled by 2^-e: h plane at p, l plane `plane` bytes behind
+__device__ __forceinline__ void put_planes(unsigned char* p, int plane, f32x4 x, int e) {
+  h4 h, l;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const float t = __builtin_amdgcn_ldexpf(x[k], -e);
+    h[k] = (_Float16)t;
+    l[k] = (_Float16)(t - (float)h[k]);
+  }
+  *reinterpret_cast<h4*>(p) = h;
+  *reinterpret_cast<h4*>(p + plane) = l;
+}
+__device__ __forceinline__ float top4(f32x4 x) { return fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))); }
+
+// q, k and v -> planes and scales: HD / 2 lanes per (row, head), four columns each; blocks [0, q_blocks) q, then k, then v
+template <int HD, int MODE>
+__global__ __launch_bounds__(NT) void diff_planes_kernel(Args a, unsigned q_blocks, unsigned kv_blocks) {
+  constexpr int LANES = HD / 2, GROUPS = NT / LANES;
+  const int tid = threadIdx.x, c4 = tid % LANES, hd = a.hd;
+  const int what = blockIdx.x < q_blocks ? 0 : (blockIdx.x < q_blocks + kv_blocks ? 1 : 2);
+  const long long block = what == 0 ? blockIdx.x : (what == 1 ? blockIdx.x - q_blocks : blockIdx.x - q_blocks - kv_blocks);
+  const int heads = what == 0 ? a.H : a.Hkv;
+  const long long N = what == 0 ? a.Nq : a.Nk, at = block * GROUPS + tid / LANES, row = at / heads;
+  const int h = (int)(at % heads);
+  if (row >= N) return;      // (whole lane groups)
+  const bool live = what == 0 || a.key_ids == nullptr || a.key_ids[row] != 0;
+  const long long slot = h * (N + PAD) + row;
+  if (what == 2) {
+    const f32x4 x = live ? get4<MODE>(a.v + row * a.ldv + (long long)h * 2 * hd, 4 * c4, 2 * hd) : f32x4{0.f, 0.f, 0.f, 0.f};
+    const int e = row_exp(group_max<LANES>(top4(x)), -80);
+    put_planes(a.vp + slot * Row<HD>::BYTES + 8 * c4, 4 * HD, x, e);
+    if (c4 == 0) {
+      a.vs[slot] = pow2(e);
+      a.ivs[slot] = pow2(-e);
+      a.lvb[slot] = live ? (float)e : -INFINITY;
+    }
+    return;
+  }
+  const int mp = c4 / (HD / 4), col = (c4 % (HD / 4)) * 4;
+  const float* src = what == 0 ? a.q + row * a.ldq + (long long)(2 * h + mp) * hd : a.k + row * a.ldk + (long long)(2 * h + mp) * hd;
+  const f32x4 x = live ? get4<MODE>(src, col, hd) : f32x4{0.f, 0.f, 0.f, 0.f};
+  const int e = row_exp(group_max<LANES / 2>(top4(x)), -126);
+  put_planes((what == 0 ? a.qp : a.kp) + slot * Row<HD>::BYTES + mp * 4 * HD + 2 * col, 2 * HD, x, e);
+  if (c4 % (HD / 4) == 0) (what == 0 ? a.qs : a.ks)[(2 * h + mp) * (N + PAD) + row] = pow2(e);
+}
+
+// ---- staging -----------------------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ unsigned lds_addr(const void* p) { return (unsigned)(unsigned long long)(RT_LDS const void*)p; }
+__device__ __forceinline__ void dma16(const void* src, unsigned dst) {      // lane i: 16 bytes to dst + 16 i
+  unsigned keep;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0" : "=&s"(keep) : "v"(src), "s"(dst) : "memory");
+}
+__device__ __forceinline__ void dma4(const void* src, unsigned dst) {       // lane i: 4 bytes to dst + 4 i
+  unsigned keep;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %1, off\n\ts_mov_b32 m0, %0" : "=&s"(keep) : "v"(src), "s"(dst) : "memory");
+}
+__device__ __forceinline__ void dma_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ void barrier() {      // LDS writes of this wave are visible behind it; LDS DMA is waited for by dma_done
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+template <int HD> __device__ __forceinline__ void copy_chunk(const unsigned char* src, unsigned dst, int tid) {
+  const unsigned wave0 = __builtin_amdgcn_readfirstlane(tid & ~63);
+#pragma unroll
+  for (int i = 0; i < (Row<HD>::UNITS + NT - 1) / NT; ++i)
+    if (tid + i * NT < Row<HD>::UNITS) dma16(src + (size_t)(tid + i * NT) * 16, dst + (wave0 + i * NT) * 16);
+}
+// rows [left, CH) of two staged images: zeros (they belong to the next session, or to nobody)
+template <int HD> __device__ __forceinline__ void clear_rows(unsigned char* img, int left, int tid) {
+  constexpr int U = Row<HD>::BYTES / 16;
+  for (int u = left * U + tid; u < CH * U; u += NT) {
+    *reinterpret_cast<f32x4*>(img + u * 16) = f32x4{0.f, 0.f, 0.f, 0.f};
+    *reinterpret_cast<f32x4*>(img + Row<HD>::CHUNK + u * 16) = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+}
+
+// ---- products ----------------------------------------------------------------------------------------------------------------------------
+struct P2 { h8 h, l; };
+__device__ __forceinline__ f32x16 mfma3(const P2& A, const P2& B, f32x16 acc) {      // smallest terms first
+  acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(A.l, B.h, acc, 0, 0, 0);
+  acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(A.h, B.l, acc, 0, 0, 0);
+  acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(A.h, B.h, acc, 0, 0, 0);
+  return acc;
+}
+__device__ __forceinline__ int reg_row(int r, int g) { return 8 * (r >> 2) + 4 * g + (r & 3); }
+__device__ __forceinline__ f32x16 zero16() { f32x16 z; for (int r = 0; r < 16; ++r) z[r] = 0.f; return z; }
+
+// columns c0 + 16 s + 8 g .. + 7 of one stored row (l plane `plane` bytes behind h)
+template <int NS> __device__ __forceinline__ void load_own(const unsigned char* row, int c0, int plane, int g, P2 (&out)[NS]) {
+#pragma unroll
+  for (int s = 0; s < NS; ++s) {
+    out[s].h = *reinterpret_cast<const h8*>(row + (c0 + 16 * s + 8 * g) * 2);
+    out[s].l = *reinterpret_cast<const h8*>(row + (c0 + 16 * s + 8 * g) * 2 + plane);
+  }
+}
+// acc[r] += sum_c img[row(r)][c0 + c] * own[c], row(r) = 8 (r / 4) + 4 g + r % 4: the partner rows are the registers, the owner the lane
+template <int HD, int NS>
+__device__ __forceinline__ void rows_dot(const unsigned char* img, int c0, int plane, const P2 (&own)[NS], int i, int g, f32x16& acc) {
+  const unsigned char* p = img + i * Row<HD>::BYTES + c0 * 2 + 16 * g;
+#pragma unroll
+  for (int s = 0; s < NS; ++s) {
+    P2 A;
+    A.h = *reinterpret_cast<const h8*>(p + 32 * s);
+    A.l = *reinterpret_cast<const h8*>(p + 32 * s + plane);
+    acc = mfma3(A, own[s], acc);
+  }
+}
+// acc[cb][r] += sum over the 32 partner rows of img[row][c0 + 32 cb + col(r)] * w[row], the lane's weights in the accumulator order of rows_dot
+// (slot j of step t = register 8 t + j = row 16 t + 8 (j / 4) + 4 g + j % 4): the partner rows are the reduction index, read transposed
+template <int HD, int NB>
+__device__ __forceinline__ void cols_dot(const unsigned char* img, int c0, int plane, const P2 (&w)[2], int lane, f32x16 (&acc)[NB]) {
+  const int g = lane >> 5;
+  const unsigned char* p = img + (4 * g + ((lane & 15) >> 2)) * Row<HD>::BYTES + (c0 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3)) * 2;
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int cb = 0; cb < NB; ++cb) {
+      const unsigned char* a = p + 16 * t * Row<HD>::BYTES + 64 * cb;
+      const unsigned char* b = a + 8 * Row<HD>::BYTES;
+      P2 A;
+      A.h = __builtin_bit_cast(h8, (s16x8v)__builtin_shufflevector(tr_read(a), tr_read(b), 0, 1, 2, 3, 4, 5, 6, 7));
+      A.l = __builtin_bit_cast(h8, (s16x8v)__builtin_shufflevector(tr_read(a + plane), tr_read(b + plane), 0, 1, 2, 3, 4, 5, 6, 7));
+      acc[cb] = mfma3(A, w[t], acc[cb]);
+    }
+}
+__device__ __forceinline__ void split16(const float (&x)[16], P2 (&out)[2]) {
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float v = x[8 * t + j];
+      out[t].h[j] = (_Float16)v;
+      out[t].l[j] = (_Float16)(v - (float)out[t].h[j]);
+    }
+}
+// The same for weights of unknown size (dS; the difference map times dO's scales): the lane's unit follows the largest magnitude it has met, as
+// the running maximum of a softmax does; when it grows, the lane's accumulators are rescaled (powers of two: exact).
+template <int NB>
+__device__ __forceinline__ void split16_scaled(float (&x)[16], float& inv, f32x16 (&acc)[NB], P2 (&out)[2]) {
+  float top = 0.f;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(x[r]));
+  top = fmaxf(top, __shfl_xor(top, 32, 64));
+  const bool grows = top * inv > 32768.f;
+  if (__any(grows)) {
+    const int e = __builtin_amdgcn_frexp_expf(top);      // top < 2^e: it comes to 2^12 .. 2^13
+    const float now = grows ? pow2(min(13 - e, 126)) : inv, ratio = now / inv;
+#pragma unroll
+    for (int cb = 0; cb < NB; ++cb) acc[cb] *= ratio;
+    inv = now;
+  }
+#pragma unroll
+  for (int r = 0; r < 16; ++r) x[r] *= inv;
+  split16(x, out);
+}
+constexpr float NO_UNIT = 0x1p126f;      // before the first weight
 
 // blockIdx -> (owner tile, session, head, split); the LAST tile of a session first where it is the heaviest (causal queries)
 struct Work { int tile, b, h, split; };
@@ -218,15 +306,19 @@ __device__ __forceinline__ Work work_of(int n_tiles, int B1, int H, bool last_fi
 }
 
 // ---- forward ----------------------------------------------------------------------------------------------------------------------------
-template <int HD, int MODE>
+// Values carry their row's scale 2^e: the running maximum is that of s + e, so the weights exp2(s + e - m) stay below one whatever the scales
+// are, and the row sum takes them back by 2^-e.
+template <int HD> constexpr int fwd_stage() { return 2 * Row<HD>::CHUNK + 512; }      // K | V | key scales of the maps | e, 2^-e
+
+template <int HD>
 __global__ __launch_bounds__(NT, 2) void diff_fwd_kernel(Args a) {
-  constexpr int DV = 2 * HD, NS = HD / 16, NB = DV / 32;
+  constexpr int DV = 2 * HD, NS = HD / 16, NB = DV / 32, STAGE = fwd_stage<HD>();
+  constexpr float UP = 14.f;      // weights come to 2^14 at most
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  unsigned char* Kimg = smem;      // the first map's image, the second one's behind it
-  unsigned char* Vimg = smem + 2 * Img<HD>::BYTES;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, mp = wave & 1, rg = wave >> 1, i = lane & 31, g = lane >> 5;
   const Work wk = work_of(a.n_tiles, a.B + (a.cu_q != nullptr ? 1 : 0), a.H, a.causal != 0);
-  const int h = wk.h, hk = h / (a.H / a.Hkv), hd = a.hd, dv = 2 * hd;
+  const int h = wk.h, hk = h / (a.H / a.Hkv), dv = 2 * a.hd;
+  const long long NqP = a.Nq + PAD, NkP = a.Nk + PAD;
 
   if (wk.b == a.B) {      // rows behind the last session: zeros
     if (wk.split != 0) return;
@@ -234,7 +326,7 @@ __global__ __launch_bounds__(NT, 2) void diff_fwd_kernel(Args a) {
     for (long long r = r0 + wk.tile; r < a.Nq; r += a.n_tiles) {
       for (int c = tid; c < dv; c += NT) a.y[r * a.ldy + (long long)h * dv + c] = 0.f;
       if (a.o12 != nullptr) for (int c = tid; c < 2 * dv; c += NT) a.o12[(r * a.H + h) * 2 * dv + c] = 0.f;
-      if (a.lse != nullptr && tid < 2) a.lse[(r * a.H + h) * 2 + tid] = 0.f;
+      if (a.lse != nullptr && tid < 2) a.lse[(2 * h + tid) * NqP + r] = 0.f;
     }
     return;
   }
@@ -242,16 +334,26 @@ __global__ __launch_bounds__(NT, 2) void diff_fwd_kernel(Args a) {
   rows_of(a.cu_q, wk.b, a.Lq, a.Nq, qr0, nq);
   rows_of(a.cu_k, wk.b, a.Lk, a.Nk, kr0, nk);
   const int off = nk - nq;
-  const float qscale = a.scale * LOG2E;
   const float lam = a.lam[h];
+  const unsigned lds0 = lds_addr(smem);
+  const long long krow = hk * NkP + kr0;
+  auto issue = [&](int c, int st) {
+    const unsigned dst = lds0 + st * STAGE;
+    const long long r = krow + c * CH;
+    copy_chunk<HD>(a.kp + r * Row<HD>::BYTES, dst, tid);
+    copy_chunk<HD>(a.vp + r * Row<HD>::BYTES, dst + Row<HD>::CHUNK, tid);
+    const long long at = kr0 + c * CH + i;
+    if (wave == 0) dma4(a.ks + (2 * hk + g) * NkP + at, dst + 2 * Row<HD>::CHUNK);
+    if (wave == 1) dma4((g == 0 ? a.lvb : a.ivs) + hk * NkP + at, dst + 2 * Row<HD>::CHUNK + 256);
+  };
 
   for (int tile = wk.tile; tile * OWN < nq; tile += a.n_tiles) {
     const int q0 = tile * OWN + 32 * rg, qi = q0 + i;
     const bool qok = qi < nq;
-    const float* qrow = a.q + (qr0 + (qok ? qi : 0)) * a.ldq + (long long)(2 * h + mp) * hd;
-    P3 Qp[NS];
-#pragma unroll
-    for (int s = 0; s < NS; ++s) Qp[s] = load_planes<MODE>(qrow, 16 * s + 8 * g, hd, qok, qscale);
+    const long long qrow = qr0 + min(qi, nq - 1);
+    P2 Qp[NS];
+    load_own<NS>(a.qp + (h * NqP + qrow) * Row<HD>::BYTES + mp * 4 * HD, 0, 2 * HD, g, Qp);
+    const float qsc = a.qs[(2 * h + mp) * NqP + qrow] * (a.scale * LOG2E);
     f32x16 O[NB];
 #pragma unroll
     for (int cb = 0; cb < NB; ++cb) O[cb] = zero16();
@@ -264,92 +366,105 @@ __global__ __launch_bounds__(NT, 2) void diff_fwd_kernel(Args a) {
       c_lo = min(c_hi, wk.split * each);
       c_hi = min(c_hi, c_lo + each);
     }
-    for (int c = c_lo; c < c_hi; ++c) {
-      const int t0 = c * CH;
-      const unsigned live = live_keys(a, kr0, t0, nk, lane);
-      if (live == 0u) continue;
-      __syncthreads();
-      {
-        const float* kb = a.k + (kr0 + t0) * a.ldk + (long long)(2 * hk) * hd;
-        stage<HD, MODE>(kb, a.ldk, hd, live, 1.f, Kimg, tid);
-        stage<HD, MODE>(kb + hd, a.ldk, hd, live, 1.f, Kimg + Img<HD>::BYTES, tid);
-        stage<DV, MODE>(a.v + (kr0 + t0) * a.ldv + (long long)hk * dv, a.ldv, dv, live, 1.f, Vimg, tid);
+    barrier();      // (the previous tile's readers are done)
+    if (c_lo < c_hi) issue(c_lo, 0);
+    int st = 0;
+    for (int c = c_lo; c < c_hi; ++c, st ^= 1) {
+      const int t0 = c * CH, left = nk - t0;
+      unsigned char* img = smem + st * STAGE;
+      float* sc = reinterpret_cast<float*>(img + 2 * Row<HD>::CHUNK);
+      dma_done();
+      barrier();                                    // chunk c is here, chunk c - 1 has been read
+      if (c + 1 < c_hi) issue(c + 1, st ^ 1);
+      if (left < CH) {
+        clear_rows<HD>(img, left, tid);
+        if (tid < 128 && (tid & 31) >= left) sc[tid] = 0.f;
+        barrier();
       }
-      __syncthreads();
       if (q0 >= nq || (a.causal && t0 > q0 + 31 + off)) continue;      // (wave-uniform) nothing of the chunk is visible to the row group
       f32x16 S = zero16();
-      rows_dot<HD, NS>(Kimg + mp * Img<HD>::BYTES, 0, Qp, i, g, S);
-      float sc[16];
+      rows_dot<HD, NS>(img + mp * 4 * HD, 0, 2 * HD, Qp, i, g, S);
+      float x[16];
 #pragma unroll
-      for (int r = 0; r < 16; ++r) sc[r] = S[r];
-      if (live != 0xFFFFFFFFu || (a.causal && t0 + 31 > q0 + off)) {
-        const int last = a.causal ? qi + off - t0 : 31;
+      for (int r = 0; r < 4; ++r) {
+        const f32x4 k4 = *reinterpret_cast<const f32x4*>(sc + 32 * mp + 8 * r + 4 * g), e4 = *reinterpret_cast<const f32x4*>(sc + 64 + 8 * r + 4 * g);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int j = reg_row(r, g);
-          sc[r] = (j <= last && ((live >> j) & 1u)) ? sc[r] : -INFINITY;
-        }
+        for (int e = 0; e < 4; ++e) x[4 * r + e] = fmaf(S[4 * r + e] * k4[e], qsc, e4[e]);
       }
-      float mx = sc[0];
+      if (left < CH || (a.causal && t0 + 31 > q0 + off)) {
+        const int last = a.causal ? min(qi + off - t0, left - 1) : left - 1;
 #pragma unroll
-      for (int r = 1; r < 16; ++r) mx = fmaxf(mx, sc[r]);
+        for (int r = 0; r < 16; ++r) x[r] = reg_row(r, g) <= last ? x[r] : -INFINITY;
+      }
+      float mx = x[0];
+#pragma unroll
+      for (int r = 1; r < 16; ++r) mx = fmaxf(mx, x[r]);
       mx = fmaxf(m, fmaxf(mx, __shfl_xor(mx, 32, 64)));
       const float base = mx == -INFINITY ? 0.f : mx;      // a row that has seen no key yet
       const float alpha = __builtin_amdgcn_exp2f(m - base);
-      float ps = 0.f;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) { sc[r] = __builtin_amdgcn_exp2f(sc[r] - base); ps += sc[r]; }
-      lsum = lsum * alpha + ps;
       if (__any(mx != m)) {
+        lsum *= alpha;
 #pragma unroll
         for (int cb = 0; cb < NB; ++cb) O[cb] *= alpha;
       }
       m = mx;
-      P3 Pp[2];
-      split16(sc, Pp);
-      cols_dot<DV, NB>(Vimg, 0, Pp, lane, O);
+      float ps = 0.f;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const f32x4 i4 = *reinterpret_cast<const f32x4*>(sc + 96 + 8 * r + 4 * g);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          x[4 * r + e] = __builtin_amdgcn_exp2f(x[4 * r + e] - (base - UP));
+          ps = fmaf(x[4 * r + e], i4[e], ps);
+        }
+      }
+      lsum += ps;
+      P2 Pp[2];
+      split16(x, Pp);
+      cols_dot<HD, NB>(img + Row<HD>::CHUNK, 0, 4 * HD, Pp, lane, O);
     }
     const float l = lsum + __shfl_xor(lsum, 32, 64);
     if (a.n_split > 1) {      // partial sums as they are; diff_combine_kernel joins the splits
       if (qok) {
         const long long at = (((long long)wk.split * a.Nq + qr0 + qi) * a.H + h) * 2 + mp;
-        if (g == 0) { a.ml[2 * at] = m; a.ml[2 * at + 1] = l; }
+        if (g == 0) { a.ml[2 * at] = m; a.ml[2 * at + 1] = l * 0x1p-14f; }
         float* o = a.part + at * dv;
 #pragma unroll
         for (int cb = 0; cb < NB; ++cb)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) put4<MODE>(o, 32 * cb + 8 * r + 4 * g, dv, f32x4{O[cb][4 * r], O[cb][4 * r + 1], O[cb][4 * r + 2], O[cb][4 * r + 3]});
+          for (int r = 0; r < 4; ++r)
+            put4(o, 32 * cb + 8 * r + 4 * g, dv, f32x4{O[cb][4 * r], O[cb][4 * r + 1], O[cb][4 * r + 2], O[cb][4 * r + 3]} * 0x1p-14f, (dv & 3) == 0);
       }
       continue;
     }
     const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);      // (a NaN sum stays one)
 #pragma unroll
     for (int cb = 0; cb < NB; ++cb) O[cb] *= inv;
-    if (qok && a.lse != nullptr && g == 0) a.lse[((qr0 + qi) * a.H + h) * 2 + mp] = l > 0.f ? m + __builtin_amdgcn_logf(l) : 0.f;
+    if (qok && a.lse != nullptr && g == 0) a.lse[(2 * h + mp) * NqP + qr0 + qi] = l > 0.f ? (m - UP) + __builtin_amdgcn_logf(l) : 0.f;
     if (qok && a.o12 != nullptr) {
       float* o = a.o12 + (((qr0 + qi) * a.H + h) * 2 + mp) * (long long)dv;
 #pragma unroll
       for (int cb = 0; cb < NB; ++cb)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) put4<MODE>(o, 32 * cb + 8 * r + 4 * g, dv, f32x4{O[cb][4 * r], O[cb][4 * r + 1], O[cb][4 * r + 2], O[cb][4 * r + 3]});
+        for (int r = 0; r < 4; ++r) put4(o, 32 * cb + 8 * r + 4 * g, dv, f32x4{O[cb][4 * r], O[cb][4 * r + 1], O[cb][4 * r + 2], O[cb][4 * r + 3]}, (dv & 3) == 0);
     }
     // the second map's wave hands its output over; the first one's subtracts, normalises and writes
-    __syncthreads();
-    f32x4* x = reinterpret_cast<f32x4*>(smem) + rg * (NB * 4 * 64);
+    barrier();
+    f32x4* xo = reinterpret_cast<f32x4*>(smem) + rg * (NB * 4 * 64);
     if (mp == 1) {
 #pragma unroll
       for (int cb = 0; cb < NB; ++cb)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) x[(cb * 4 + r) * 64 + lane] = f32x4{O[cb][4 * r], O[cb][4 * r + 1], O[cb][4 * r + 2], O[cb][4 * r + 3]};
+        for (int r = 0; r < 4; ++r) xo[(cb * 4 + r) * 64 + lane] = f32x4{O[cb][4 * r], O[cb][4 * r + 1], O[cb][4 * r + 2], O[cb][4 * r + 3]};
     }
-    __syncthreads();
+    barrier();
     if (mp == 0) {
       float ss = 0.f;
 #pragma unroll
       for (int cb = 0; cb < NB; ++cb)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const f32x4 o2 = x[(cb * 4 + r) * 64 + lane];
+          const f32x4 o2 = xo[(cb * 4 + r) * 64 + lane];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             O[cb][4 * r + e] -= lam * o2[e];
@@ -368,7 +483,7 @@ __global__ __launch_bounds__(NT, 2) void diff_fwd_kernel(Args a) {
             f32x4 t;
 #pragma unroll
             for (int e = 0; e < 4; ++e) t[e] = O[cb][4 * r + e] * f * ((a.norm_w != nullptr && col + e < dv) ? a.norm_w[col + e] : 1.f);
-            put4<MODE>(o, col, dv, t);
+            put4(o, col, dv, t, a.vec_y != 0);
           }
       }
     }
@@ -389,7 +504,7 @@ __global__ __launch_bounds__(NT) void diff_combine_kernel(Args a) {
     const float m = on ? a.ml[2 * p] : -INFINITY, l = on ? a.ml[2 * p + 1] : 0.f, mx = wave_max(m), base = mx == -INFINITY ? 0.f : mx;
     const float e = on ? __builtin_amdgcn_exp2f(m - base) : 0.f, total = wave_sum(l * e);
     wgt[wave][lane] = e * (total > 0.f ? 1.f / total : (total == 0.f ? 0.f : total));
-    if (a.lse != nullptr && lane == 0) a.lse[at * 2 + wave] = total > 0.f ? mx + __builtin_amdgcn_logf(total) : 0.f;
+    if (a.lse != nullptr && lane == 0) a.lse[(2 * h + wave) * (a.Nq + PAD) + row] = total > 0.f ? mx + __builtin_amdgcn_logf(total) : 0.f;
   }
   const int slots = NT / dv, c = tid % dv, sub = tid / dv;
   for (int mp = 0; mp < 2; ++mp) {
@@ -415,53 +530,27 @@ __global__ __launch_bounds__(NT) void diff_combine_kernel(Args a) {
   if (tid < dv) a.y[row * a.ldy + (long long)h * dv + tid] = o * f * (a.norm_w != nullptr ? a.norm_w[tid] : 1.f);
 }
 
-// ---- backward, in front: gradient of o, delta_m = do . o_m, and the sums behind dlam and dw -----------------------------------------------
+// ---- backward, in front: gradient of o (as planes), delta_m = do . o_m, and the sums behind dlam and dw --------------------------------------
 // HD / 2 lanes per (row, head), four columns each; a lane group keeps its head, so dlam and dw stay in registers over all of its rows.  They
 // are summed in 64 bits, per workgroup, in a fixed order.
 constexpr int PRE_WG = 1024;      // workgroups at most: the partials are [PRE_WG][H + 2 hd] doubles
 
-template <int LANES> __device__ __forceinline__ float group_sum(float v) {      // 16 or 32 neighbouring lanes
-  v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0xB1, 0xF, 0xF, true));
-  v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x4E, 0xF, 0xF, true));
-  v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x141, 0xF, 0xF, true));
-  v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x140, 0xF, 0xF, true));
-  if (LANES == 32) v += __builtin_bit_cast(float, __builtin_amdgcn_ds_swizzle(__builtin_bit_cast(int, v), 0x401F));
-  return v;
-}
-template <bool VEC> __device__ __forceinline__ f32x4 get4(const float* p, int c, int ncol) {
-  f32x4 x{0.f, 0.f, 0.f, 0.f};
-  if (VEC) {
-    if (c < ncol) x = *reinterpret_cast<const f32x4*>(p + c);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (c + e < ncol) x[e] = p[c + e];
-  }
-  return x;
-}
-
-template <int HD, bool VEC>
-__global__ __launch_bounds__(NT) void diff_bwd_pre_kernel(Args a, const float* dy, long long lddy, float* dout, float* delta, double* part) {
+template <int HD, int MODE>
+__global__ __launch_bounds__(NT) void diff_bwd_pre_kernel(Args a, const float* dy, long long lddy, double* part) {
   constexpr int LANES = HD / 2, GROUPS = NT / LANES;
   __shared__ double sw[GROUPS][2 * HD], sl[GROUPS];
   const int tid = threadIdx.x, gid = tid / LANES, c = (tid % LANES) * 4, dv = 2 * a.hd, H = a.H;
-  const long long used = rows_used(a.cu_q, a.B, a.Nq);
+  const long long used = rows_used(a.cu_q, a.B, a.Nq), NqP = a.Nq + PAD;
   const long long gg = (long long)blockIdx.x * GROUPS + gid, n_groups = (long long)gridDim.x * GROUPS;
   const int h = (int)(gg % H);
-  const long long step = n_groups / H;                       // rows are dealt to the step lane groups of a head; leftover groups do nothing
+  const long long step = n_groups / H;                       // rows are dealt to the `step` lane groups of a head; leftover groups do nothing
   const float lam = a.lam[h], inv = 1.f / (float)dv;
-  const f32x4 w = a.norm_w != nullptr ? get4<VEC>(a.norm_w, c, dv) * a.out_scale : f32x4{a.out_scale, a.out_scale, a.out_scale, a.out_scale};
+  const f32x4 w = a.norm_w != nullptr ? get4<MODE>(a.norm_w, c, dv) * a.out_scale : f32x4{a.out_scale, a.out_scale, a.out_scale, a.out_scale};
   double dw[4] = {0.0, 0.0, 0.0, 0.0}, dl = 0.0;
-  for (long long row = gg < step * H ? gg / H : a.Nq; row < a.Nq; row += step) {
+  for (long long row = gg < step * H ? gg / H : used; row < used; row += step) {
     const long long at = row * H + h;
-    float* dst = dout + at * dv;
-    if (row >= used) {
-      put4<VEC ? 1 : 2>(dst, c, dv, f32x4{0.f, 0.f, 0.f, 0.f});
-      if (c == 0) { delta[at * 2] = 0.f; delta[at * 2 + 1] = 0.f; }
-      continue;
-    }
-    const f32x4 o1 = get4<VEC>(a.o12 + at * 2 * dv, c, dv), o2 = get4<VEC>(a.o12 + (at * 2 + 1) * dv, c, dv);
-    const f32x4 g = get4<VEC>(dy + row * lddy + (long long)h * dv, c, dv), e = g * w;
+    const f32x4 o1 = get4<MODE>(a.o12 + at * 2 * dv, c, dv), o2 = get4<MODE>(a.o12 + (at * 2 + 1) * dv, c, dv);
+    const f32x4 g = get4<MODE>(dy + row * lddy + (long long)h * dv, c, dv), e = g * w;
     f32x4 d = e;
     if (a.norm_w != nullptr) {
       const f32x4 x = o1 - o2 * lam;
@@ -474,10 +563,19 @@ __global__ __launch_bounds__(NT) void diff_bwd_pre_kernel(Args a, const float* d
         dw[k] += (double)(a.out_scale * g[k] * u[k]);
       }
     }
-    put4<VEC ? 1 : 2>(dst, c, dv, d);
+    if (MODE != 0) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) d[k] = c + k < dv ? d[k] : 0.f;
+    }
+    const int ex = row_exp(group_max<LANES>(top4(d)), -126);
+    put_planes(a.dp + (h * NqP + row) * Row<HD>::BYTES + 2 * c, 4 * HD, d, ex);
     const float s1 = group_sum<LANES>(d[0] * o1[0] + d[1] * o1[1] + d[2] * o1[2] + d[3] * o1[3]);
     const float s2 = group_sum<LANES>(d[0] * o2[0] + d[1] * o2[1] + d[2] * o2[2] + d[3] * o2[3]);
-    if (c == 0) { delta[at * 2] = s1; delta[at * 2 + 1] = s2; }
+    if (c == 0) {
+      a.ds[h * NqP + row] = pow2(ex);
+      a.delta[2 * h * NqP + row] = s1;
+      a.delta[(2 * h + 1) * NqP + row] = s2;
+    }
     dl -= (double)s2;
   }
 #pragma unroll
@@ -510,16 +608,21 @@ __global__ __launch_bounds__(64) void diff_bwd_sums_kernel(const double* part, i
 }
 
 // ---- backward, dQ: the owner is a query; both maps need G^T = V dO^T, each wave makes it over half of V's columns and they swap halves ------
-template <int HD, int MODE>
+// STAGES: two where two workgroups with two chunk buffers fit a CU's LDS (HD 32), else one: the other workgroup's products run under the copy.
+template <int HD> constexpr int bwd_stages() { return HD == 32 ? 2 : 1; }
+template <int HD> constexpr int dq_lds() { return bwd_stages<HD>() * fwd_stage<HD>() + 4 * 4 * 64 * 16; }
+template <int HD> constexpr int dkv_stage() { return 2 * Row<HD>::CHUNK + 1024; }
+template <int HD> constexpr int dkv_lds() { return bwd_stages<HD>() * dkv_stage<HD>() + 4 * 8 * 64 * 16; }
+
+template <int HD>
 __global__ __launch_bounds__(NT, 2) void diff_bwd_dq_kernel(Args a) {
-  constexpr int DV = 2 * HD, NS = HD / 16, NB = HD / 32;
+  constexpr int NS = HD / 16, NB = HD / 32, STAGE = fwd_stage<HD>(), STAGES = bwd_stages<HD>();
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  unsigned char* Kimg = smem;      // the first map's image, the second one's behind it
-  unsigned char* Vimg = smem + 2 * Img<HD>::BYTES;
-  f32x4* swap = reinterpret_cast<f32x4*>(smem + 2 * Img<HD>::BYTES + Img<DV>::BYTES);      // [wave][4][64]
+  f32x4* swap = reinterpret_cast<f32x4*>(smem + STAGES * STAGE);      // [wave][4][64]
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, mp = wave & 1, rg = wave >> 1, i = lane & 31, g = lane >> 5;
   const Work wk = work_of(a.n_tiles, a.B + (a.cu_q != nullptr ? 1 : 0), a.H, a.causal != 0);
   const int h = wk.h, hk = h / (a.H / a.Hkv), hd = a.hd, dv = 2 * hd;
+  const long long NqP = a.Nq + PAD, NkP = a.Nk + PAD;
   if (wk.b == a.B) {      // rows behind the last session have no gradient
     for (long long r = rows_used(a.cu_q, a.B, a.Nq) + wk.tile; r < a.Nq; r += a.n_tiles)
       for (int c = tid; c < dv; c += NT) a.dq[r * a.lddq + (long long)h * dv + c] = 0.f;
@@ -529,89 +632,112 @@ __global__ __launch_bounds__(NT, 2) void diff_bwd_dq_kernel(Args a) {
   rows_of(a.cu_q, wk.b, a.Lq, a.Nq, qr0, nq);
   rows_of(a.cu_k, wk.b, a.Lk, a.Nk, kr0, nk);
   const int off = nk - nq;
-  const float qscale = a.scale * LOG2E, sign = mp == 0 ? 1.f : -a.lam[h];
+  const float sign = mp == 0 ? 1.f : -a.lam[h];
+  const unsigned lds0 = lds_addr(smem);
+  const long long krow = hk * NkP + kr0;
+  auto issue = [&](int c, int st) {
+    const unsigned dst = lds0 + st * STAGE;
+    const long long r = krow + c * CH;
+    copy_chunk<HD>(a.kp + r * Row<HD>::BYTES, dst, tid);
+    copy_chunk<HD>(a.vp + r * Row<HD>::BYTES, dst + Row<HD>::CHUNK, tid);
+    const long long at = kr0 + c * CH + i;
+    if (wave == 0) dma4(a.ks + (2 * hk + g) * NkP + at, dst + 2 * Row<HD>::CHUNK);
+    if (wave == 1) dma4((g == 0 ? a.lvb : a.vs) + hk * NkP + at, dst + 2 * Row<HD>::CHUNK + 256);
+  };
 
   for (int tile = wk.tile; tile * OWN < nq; tile += a.n_tiles) {
     const int q0 = tile * OWN + 32 * rg, qi = q0 + i;
     const bool qok = qi < nq;
-    const long long grow = qr0 + (qok ? qi : 0);
-    P3 Qp[NS], Dp[NS];      // dO: columns mp * HD .. of the padded 2 HD
-#pragma unroll
-    for (int s = 0; s < NS; ++s) {
-      Qp[s] = load_planes<MODE>(a.q + grow * a.ldq + (long long)(2 * h + mp) * hd, 16 * s + 8 * g, hd, qok, qscale);
-      Dp[s] = load_planes<MODE>(a.dout + grow * a.lddo + (long long)h * dv, mp * HD + 16 * s + 8 * g, dv, qok, 1.f);
-    }
-    const float lse = qok ? a.lse[(grow * a.H + h) * 2 + mp] : 0.f, dl = qok ? a.delta[(grow * a.H + h) * 2 + mp] : 0.f;
+    const long long qrow = qr0 + min(qi, nq - 1);
+    P2 Qp[NS], Dp[NS];      // dO: columns mp * HD .. of the padded 2 HD
+    load_own<NS>(a.qp + (h * NqP + qrow) * Row<HD>::BYTES + mp * 4 * HD, 0, 2 * HD, g, Qp);
+    load_own<NS>(a.dp + (h * NqP + qrow) * Row<HD>::BYTES, mp * HD, 4 * HD, g, Dp);
+    const float qsc = a.qs[(2 * h + mp) * NqP + qrow] * (a.scale * LOG2E), dsc = a.ds[h * NqP + qrow];
+    const float lse = a.lse[(2 * h + mp) * NqP + qrow], dl = a.delta[(2 * h + mp) * NqP + qrow];
     f32x16 dQ[NB];
 #pragma unroll
     for (int cb = 0; cb < NB; ++cb) dQ[cb] = zero16();
+    float unit = NO_UNIT;
     const int k_end = a.causal ? min(nk, tile * OWN + OWN + off) : nk;
     const int n_ch = k_end > 0 ? (k_end + CH - 1) / CH : 0;
-    for (int c = 0; c < n_ch; ++c) {
-      const int t0 = c * CH;
-      const unsigned live = live_keys(a, kr0, t0, nk, lane);
-      if (live == 0u) continue;
-      __syncthreads();
-      {
-        const float* kb = a.k + (kr0 + t0) * a.ldk + (long long)(2 * hk) * hd;
-        stage<HD, MODE>(kb, a.ldk, hd, live, 1.f, Kimg, tid);
-        stage<HD, MODE>(kb + hd, a.ldk, hd, live, 1.f, Kimg + Img<HD>::BYTES, tid);
-        stage<DV, MODE>(a.v + (kr0 + t0) * a.ldv + (long long)hk * dv, a.ldv, dv, live, 1.f, Vimg, tid);
+    barrier();
+    if (STAGES == 2 && n_ch > 0) issue(0, 0);
+    int st = 0;
+    for (int c = 0; c < n_ch; ++c, st ^= STAGES - 1) {
+      const int t0 = c * CH, left = nk - t0;
+      unsigned char* img = smem + st * STAGE;
+      float* sc = reinterpret_cast<float*>(img + 2 * Row<HD>::CHUNK);
+      if (STAGES == 1) {
+        if (c > 0) barrier();      // chunk c - 1 has been read
+        issue(c, 0);
       }
-      __syncthreads();
+      dma_done();
+      barrier();
+      if (STAGES == 2 && c + 1 < n_ch) issue(c + 1, st ^ 1);
+      if (left < CH) {
+        clear_rows<HD>(img, left, tid);
+        if (tid < 128 && (tid & 31) >= left) sc[tid] = 0.f;
+        barrier();
+      }
       const bool on = q0 < nq && !(a.causal && t0 > q0 + 31 + off);      // (the same for the two waves of a row group)
       f32x16 S = zero16(), G = zero16();
       if (on) {
-        rows_dot<HD, NS>(Kimg + mp * Img<HD>::BYTES, 0, Qp, i, g, S);
-        rows_dot<DV, NS>(Vimg, mp * HD, Dp, i, g, G);
+        rows_dot<HD, NS>(img + Row<HD>::CHUNK, mp * HD, 4 * HD, Dp, i, g, G);
 #pragma unroll
         for (int r = 0; r < 4; ++r) swap[(wave * 4 + r) * 64 + lane] = f32x4{G[4 * r], G[4 * r + 1], G[4 * r + 2], G[4 * r + 3]};
+        rows_dot<HD, NS>(img + mp * 4 * HD, 0, 2 * HD, Qp, i, g, S);
       }
-      __syncthreads();
+      barrier();
       if (!on) continue;
-      float ds[16];
-      const bool edge = live != 0xFFFFFFFFu || (a.causal && t0 + 31 > q0 + off);
-      const int last = a.causal ? qi + off - t0 : 31;
+      float x[16];
+      const bool edge = left < CH || (a.causal && t0 + 31 > q0 + off);
+      const int last = a.causal ? min(qi + off - t0, left - 1) : left - 1;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const f32x4 other = swap[((wave ^ 1) * 4 + r) * 64 + lane];
+        const f32x4 k4 = *reinterpret_cast<const f32x4*>(sc + 32 * mp + 8 * r + 4 * g), v4 = *reinterpret_cast<const f32x4*>(sc + 96 + 8 * r + 4 * g);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int j = reg_row(4 * r + e, g);
-          float p = __builtin_amdgcn_exp2f(S[4 * r + e] - lse);
-          if (edge) p = (j <= last && ((live >> j) & 1u)) ? p : 0.f;
-          ds[4 * r + e] = p * ((G[4 * r + e] + other[e]) - dl);
+          float p = __builtin_amdgcn_exp2f(fmaf(S[4 * r + e] * k4[e], qsc, -lse));
+          if (edge) p = reg_row(4 * r + e, g) <= last ? p : 0.f;
+          x[4 * r + e] = p * fmaf((G[4 * r + e] + other[e]) * v4[e], dsc, -dl) * k4[e];
         }
       }
-      P3 dsp[2];
-      split16(ds, dsp);
-      cols_dot<HD, NB>(Kimg + mp * Img<HD>::BYTES, 0, dsp, lane, dQ);
+      if (a.key_ids != nullptr) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const f32x4 b4 = *reinterpret_cast<const f32x4*>(sc + 64 + 8 * r + 4 * g);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[4 * r + e] = b4[e] == -INFINITY ? 0.f : x[4 * r + e];
+        }
+      }
+      P2 w[2];
+      split16_scaled<NB>(x, unit, dQ, w);
+      cols_dot<HD, NB>(img + mp * 4 * HD, 0, 2 * HD, w, lane, dQ);
     }
     if (qok) {
-      float* o = a.dq + grow * a.lddq + (long long)(2 * h + mp) * hd;
-      const float f = a.scale * sign;
+      float* o = a.dq + (qr0 + qi) * a.lddq + (long long)(2 * h + mp) * hd;
+      const float f = a.scale * sign / unit;
 #pragma unroll
       for (int cb = 0; cb < NB; ++cb)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          put4<MODE>(o, 32 * cb + 8 * r + 4 * g, hd, f32x4{dQ[cb][4 * r] * f, dQ[cb][4 * r + 1] * f, dQ[cb][4 * r + 2] * f, dQ[cb][4 * r + 3] * f});
+          put4(o, 32 * cb + 8 * r + 4 * g, hd, f32x4{dQ[cb][4 * r], dQ[cb][4 * r + 1], dQ[cb][4 * r + 2], dQ[cb][4 * r + 3]} * f, a.vec_q != 0);
     }
   }
 }
 
 // ---- backward, dK and dV: the owner is a key; the query heads of its group are summed in a fixed order ---------------------------------------
 // The two waves of a row group swap their halves of G and their probabilities: each makes dK of its map and dV of its half of the columns.
-template <int HD, int MODE>
+template <int HD>
 __global__ __launch_bounds__(NT, 2) void diff_bwd_dkv_kernel(Args a) {
-  constexpr int DV = 2 * HD, NS = HD / 16, NB = HD / 32;
+  constexpr int NS = HD / 16, NB = HD / 32, STAGE = dkv_stage<HD>(), STAGES = bwd_stages<HD>();
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  unsigned char* Qimg = smem;      // the first map's image, the second one's behind it
-  unsigned char* Dimg = smem + 2 * Img<HD>::BYTES;
-  f32x4* swap = reinterpret_cast<f32x4*>(smem + 2 * Img<HD>::BYTES + Img<DV>::BYTES);      // [wave][8][64]: G halves, probabilities
-  float* stat = reinterpret_cast<float*>(swap + 4 * 8 * 64);                               // [map][lse 32 | delta 32]
+  f32x4* swap = reinterpret_cast<f32x4*>(smem + STAGES * STAGE);      // [wave][8][64]: G halves, probabilities
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, mp = wave & 1, rg = wave >> 1, i = lane & 31, g = lane >> 5;
   const Work wk = work_of(a.n_tiles, a.B + (a.cu_k != nullptr ? 1 : 0), a.Hkv, false);
   const int hk = wk.h, rep = a.H / a.Hkv, hd = a.hd, dv = 2 * hd;
+  const long long NqP = a.Nq + PAD, NkP = a.Nk + PAD;
   if (wk.b == a.B) {
     for (long long r = rows_used(a.cu_k, a.B, a.Nk) + wk.tile; r < a.Nk; r += a.n_tiles)
       for (int c = tid; c < dv; c += NT) {
@@ -624,93 +750,108 @@ __global__ __launch_bounds__(NT, 2) void diff_bwd_dkv_kernel(Args a) {
   rows_of(a.cu_q, wk.b, a.Lq, a.Nq, qr0, nq);
   rows_of(a.cu_k, wk.b, a.Lk, a.Nk, kr0, nk);
   const int off = nk - nq;
-  const float kscale = a.scale * LOG2E;
+  const unsigned lds0 = lds_addr(smem);
+  const int c_all = (nq + CH - 1) / CH;
+  // scales behind the images: queries of the maps | log sums | deltas | dO, each [2][32]
+  auto issue = [&](int h, int c, int st) {
+    const unsigned dst = lds0 + st * STAGE;
+    const long long r = h * NqP + qr0 + c * CH;
+    copy_chunk<HD>(a.qp + r * Row<HD>::BYTES, dst, tid);
+    copy_chunk<HD>(a.dp + r * Row<HD>::BYTES, dst + Row<HD>::CHUNK, tid);
+    const long long at = (2 * h + g) * NqP + qr0 + c * CH + i;
+    const float* src = wave == 0 ? a.qs + at : wave == 1 ? a.lse + at : wave == 2 ? a.delta + at : a.ds + h * NqP + qr0 + c * CH + i;
+    dma4(src, dst + 2 * Row<HD>::CHUNK + __builtin_amdgcn_readfirstlane(wave) * 256);
+  };
 
   for (int tile = wk.tile; tile * OWN < nk; tile += a.n_tiles) {
     const int k0 = tile * OWN + 32 * rg, ki = k0 + i;
     const bool kin = ki < nk;
-    const bool kok = kin && (a.key_ids == nullptr || a.key_ids[kr0 + ki] != 0);
-    const long long grow = kr0 + (kin ? ki : 0);
-    P3 Kp[NS], Vp[NS];
-#pragma unroll
-    for (int s = 0; s < NS; ++s) {
-      Kp[s] = load_planes<MODE>(a.k + grow * a.ldk + (long long)(2 * hk + mp) * hd, 16 * s + 8 * g, hd, kok, kscale);
-      Vp[s] = load_planes<MODE>(a.v + grow * a.ldv + (long long)hk * dv, mp * HD + 16 * s + 8 * g, dv, kok, 1.f);
-    }
+    const long long krow = kr0 + min(ki, nk - 1);
+    const bool kok = kin && a.lvb[hk * NkP + krow] != -INFINITY;
+    P2 Kp[NS], Vp[NS];
+    load_own<NS>(a.kp + (hk * NkP + krow) * Row<HD>::BYTES + mp * 4 * HD, 0, 2 * HD, g, Kp);
+    load_own<NS>(a.vp + (hk * NkP + krow) * Row<HD>::BYTES, mp * HD, 4 * HD, g, Vp);
+    const float ksc = a.ks[(2 * hk + mp) * NkP + krow] * (a.scale * LOG2E), vsc = a.vs[hk * NkP + krow];
     f32x16 dK[NB], dV[NB];
 #pragma unroll
     for (int cb = 0; cb < NB; ++cb) { dK[cb] = zero16(); dV[cb] = zero16(); }
-    const int c_lo = a.causal ? max(0, tile * OWN - off) / CH : 0, c_hi = (nq + CH - 1) / CH;
-    for (int hh = 0; hh < rep; ++hh) {
-      const int h = hk * rep + hh;
-      const float lam = a.lam[h], sign = mp == 0 ? 1.f : -lam;
-      for (int c = c_lo; c < c_hi; ++c) {
-        const int t0 = c * CH, left = nq - t0;
-        const unsigned rows = left >= 32 ? 0xFFFFFFFFu : (1u << left) - 1u;
-        __syncthreads();
-        {
-          const float* qb = a.q + (qr0 + t0) * a.ldq + (long long)(2 * h) * hd;
-          stage<HD, MODE>(qb, a.ldq, hd, rows, 1.f, Qimg, tid);
-          stage<HD, MODE>(qb + hd, a.ldq, hd, rows, 1.f, Qimg + Img<HD>::BYTES, tid);
-          stage<DV, MODE>(a.dout + (qr0 + t0) * a.lddo + (long long)h * dv, a.lddo, dv, rows, 1.f, Dimg, tid);
-          if (tid < 128) {      // a row behind the session's end: exp2(-inf) = 0
-            const int m = tid >> 6, what = (tid >> 5) & 1, r = tid & 31;
-            const long long at = ((qr0 + t0 + r) * a.H + h) * 2 + m;
-            stat[tid] = r < left ? (what == 0 ? a.lse[at] : a.delta[at]) : (what == 0 ? INFINITY : 0.f);
-          }
-        }
-        __syncthreads();
-        const bool on = k0 < nk && !(a.causal && t0 + 31 + off < k0);
-        f32x16 S = zero16(), G = zero16();
-        float p[16];
-        if (on) {
-          rows_dot<HD, NS>(Qimg + mp * Img<HD>::BYTES, 0, Kp, i, g, S);
-          rows_dot<DV, NS>(Dimg, mp * HD, Vp, i, g, G);
-          const bool edge = a.causal && t0 + off < k0 + 31;
-          const int first = a.causal ? ki - off - t0 : -1;      // the first row of the chunk that sees this key
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const f32x4 ls = *reinterpret_cast<const f32x4*>(stat + mp * 64 + 8 * r + 4 * g);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float x = __builtin_amdgcn_exp2f(S[4 * r + e] - ls[e]);
-              p[4 * r + e] = (kok && (!edge || reg_row(4 * r + e, g) >= first)) ? x : 0.f;
-            }
-            swap[(wave * 8 + r) * 64 + lane] = f32x4{G[4 * r], G[4 * r + 1], G[4 * r + 2], G[4 * r + 3]};
-            swap[(wave * 8 + 4 + r) * 64 + lane] = f32x4{p[4 * r], p[4 * r + 1], p[4 * r + 2], p[4 * r + 3]};
-          }
-        }
-        __syncthreads();
-        if (!on) continue;
-        float ds[16], d[16];
+    float unit_k = NO_UNIT, unit_v = NO_UNIT;
+    const int c_lo = a.causal ? min(c_all, max(0, tile * OWN - off) / CH) : 0, n_ch = c_all - c_lo, n_all = n_ch * rep;      // chunks of the heads one after another
+    barrier();
+    if (STAGES == 2 && n_all > 0) issue(hk * rep, c_lo, 0);
+    int st = 0;
+    for (int n = 0; n < n_all; ++n, st ^= STAGES - 1) {
+      const int h = hk * rep + n / n_ch, c = c_lo + n % n_ch, t0 = c * CH, left = nq - t0;
+      const float lam = a.lam[h];
+      unsigned char* img = smem + st * STAGE;
+      float* sc = reinterpret_cast<float*>(img + 2 * Row<HD>::CHUNK);
+      if (STAGES == 1) {
+        if (n > 0) barrier();
+        issue(h, c, 0);
+      }
+      dma_done();
+      barrier();
+      if (STAGES == 2 && n + 1 < n_all) issue(hk * rep + (n + 1) / n_ch, c_lo + (n + 1) % n_ch, st ^ 1);
+      if (left < CH) {      // rows behind the session's end: a log sum of infinity, so that exp2 gives 0
+        clear_rows<HD>(img, left, tid);
+        if ((tid & 31) >= left) sc[tid] = (tid >> 6) == 1 ? INFINITY : 0.f;
+        barrier();
+      }
+      const bool on = k0 < nk && !(a.causal && t0 + 31 + off < k0);
+      f32x16 S = zero16(), G = zero16();
+      float p[16];
+      if (on) {
+        rows_dot<HD, NS>(img + mp * 4 * HD, 0, 2 * HD, Kp, i, g, S);
+        rows_dot<HD, NS>(img + Row<HD>::CHUNK, mp * HD, 4 * HD, Vp, i, g, G);
+        const bool edge = a.causal && t0 + off < k0 + 31;
+        const int first = a.causal ? ki - off - t0 : -1;      // the first row of the chunk that sees this key
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const f32x4 og = swap[((wave ^ 1) * 8 + r) * 64 + lane], op = swap[((wave ^ 1) * 8 + 4 + r) * 64 + lane];
-          const f32x4 dl = *reinterpret_cast<const f32x4*>(stat + mp * 64 + 32 + 8 * r + 4 * g);
+          const f32x4 q4 = *reinterpret_cast<const f32x4*>(sc + 32 * mp + 8 * r + 4 * g), l4 = *reinterpret_cast<const f32x4*>(sc + 64 + 32 * mp + 8 * r + 4 * g);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int x = 4 * r + e;
-            ds[x] = sign * p[x] * ((G[x] + og[e]) - dl[e]);
-            d[x] = mp == 0 ? p[x] - lam * op[e] : op[e] - lam * p[x];
+            const float x = __builtin_amdgcn_exp2f(fmaf(S[4 * r + e] * q4[e], ksc, -l4[e]));
+            p[4 * r + e] = (kok && (!edge || reg_row(4 * r + e, g) >= first)) ? x : 0.f;
           }
+          swap[(wave * 8 + r) * 64 + lane] = f32x4{G[4 * r], G[4 * r + 1], G[4 * r + 2], G[4 * r + 3]};
+          swap[(wave * 8 + 4 + r) * 64 + lane] = f32x4{p[4 * r], p[4 * r + 1], p[4 * r + 2], p[4 * r + 3]};
         }
-        P3 w[2];
-        split16(ds, w);
-        cols_dot<HD, NB>(Qimg + mp * Img<HD>::BYTES, 0, w, lane, dK);
-        split16(d, w);
-        cols_dot<DV, NB>(Dimg, mp * HD, w, lane, dV);
       }
+      barrier();
+      if (!on) continue;
+      const float sign = mp == 0 ? 1.f : -lam;
+      float x[16];
+      P2 w[2];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const f32x4 og = swap[((wave ^ 1) * 8 + r) * 64 + lane];
+        const f32x4 q4 = *reinterpret_cast<const f32x4*>(sc + 32 * mp + 8 * r + 4 * g), dl = *reinterpret_cast<const f32x4*>(sc + 128 + 32 * mp + 8 * r + 4 * g),
+                    d4 = *reinterpret_cast<const f32x4*>(sc + 192 + 8 * r + 4 * g);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[4 * r + e] = sign * p[4 * r + e] * fmaf((G[4 * r + e] + og[e]) * d4[e], vsc, -dl[e]) * q4[e];
+      }
+      split16_scaled<NB>(x, unit_k, dK, w);
+      cols_dot<HD, NB>(img + mp * 4 * HD, 0, 2 * HD, w, lane, dK);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const f32x4 op = swap[((wave ^ 1) * 8 + 4 + r) * 64 + lane], d4 = *reinterpret_cast<const f32x4*>(sc + 192 + 8 * r + 4 * g);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[4 * r + e] = (mp == 0 ? p[4 * r + e] - lam * op[e] : op[e] - lam * p[4 * r + e]) * d4[e];
+      }
+      split16_scaled<NB>(x, unit_v, dV, w);
+      cols_dot<HD, NB>(img + Row<HD>::CHUNK, mp * HD, 4 * HD, w, lane, dV);
     }
     if (kin) {
-      float* ok = a.dk + grow * a.lddk + (long long)(2 * hk + mp) * hd;
-      float* ov = a.dv + grow * a.lddv + (long long)hk * dv;
+      float* ok = a.dk + (kr0 + ki) * a.lddk + (long long)(2 * hk + mp) * hd;
+      float* ov = a.dv + (kr0 + ki) * a.lddv + (long long)hk * dv;
+      const float fk = a.scale / unit_k, fv = 1.f / unit_v;
 #pragma unroll
       for (int cb = 0; cb < NB; ++cb)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int col = 32 * cb + 8 * r + 4 * g;
-          put4<MODE>(ok, col, hd, f32x4{dK[cb][4 * r] * a.scale, dK[cb][4 * r + 1] * a.scale, dK[cb][4 * r + 2] * a.scale, dK[cb][4 * r + 3] * a.scale});
-          put4<MODE>(ov, mp * HD + col, dv, f32x4{dV[cb][4 * r], dV[cb][4 * r + 1], dV[cb][4 * r + 2], dV[cb][4 * r + 3]});
+          put4(ok, col, hd, f32x4{dK[cb][4 * r], dK[cb][4 * r + 1], dK[cb][4 * r + 2], dK[cb][4 * r + 3]} * fk, a.vec_kv != 0);
+          put4(ov, mp * HD + col, dv, f32x4{dV[cb][4 * r], dV[cb][4 * r + 1], dV[cb][4 * r + 2], dV[cb][4 * r + 3]} * fv, a.vec_kv != 0);
         }
     }
   }
@@ -723,19 +864,9 @@ __global__ __launch_bounds__(NT, 2) void diff_bwd_dkv_kernel(Args a) {
 // keeps its own running maximum and sum; no barrier in the loop, 16 loads of 16 bytes in flight per lane.
 constexpr int MAXR = 8;
 
-template <int CTRL> __device__ __forceinline__ float dpp(float v) {
-  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, true));
-}
-template <int HD> __device__ __forceinline__ float map_sum(float v) {      // over the HD / 4 lanes of a key's map
-  v += dpp<0xB1>(v);       // lane ^ 1
-  v += dpp<0x4E>(v);       // lane ^ 2
-  v += dpp<0x141>(v);      // mirrored in 8 lanes
-  if (HD == 64) v += dpp<0x140>(v);      // mirrored in 16 lanes
-  return v;
-}
 template <int HD> __device__ __forceinline__ float other_map(float v) {
   if (HD == 32) return dpp<0x128>(v);      // rotated by 8 in 16 lanes
-  return __builtin_bit_cast(float, __builtin_amdgcn_ds_swizzle(__builtin_bit_cast(int, v), 0x401F));      // lane ^ 16
+  return lane_xor16(v);
 }
 template <int HD> __device__ __forceinline__ float keys_max(float v) {      // over the keys of one load
   if (HD == 32) v = fmaxf(v, __shfl_xor(v, 16, 64));
@@ -748,7 +879,7 @@ template <int HD> __device__ __forceinline__ float keys_sum(float v) {
 constexpr int decode_keys(int HDP) { return HDP == 32 ? 32 : 16; }      // TK
 
 template <int HD, int MODE, int R>
-__global__ __launch_bounds__(NT, 2) void diff_decode_kernel(Args a) {
+__global__ __launch_bounds__(NT, R > 4 ? 1 : 2) void diff_decode_kernel(Args a) {
   constexpr int DV = 2 * HD, LPK = HD / 2, KPL = 64 / LPK, NL = 8, TK = KPL * NL;
   __shared__ float wstat[4][R][2][2], wacc[4][R][2][DV];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, kk = lane / LPK, c4 = lane % LPK, mp = c4 / (HD / 4), col = (c4 % (HD / 4)) * 4;
@@ -813,7 +944,7 @@ __global__ __launch_bounds__(NT, 2) void diff_decode_kernel(Args a) {
         float s[NL], mx = m[w];
 #pragma unroll
         for (int u = 0; u < NL; ++u) {
-          s[u] = map_sum<HD>(fmaf(qv[w][0], kf[u][0], qv[w][1] * kf[u][1]) + fmaf(qv[w][2], kf[u][2], qv[w][3] * kf[u][3]));
+          s[u] = group_sum<HD / 4>(fmaf(qv[w][0], kf[u][0], qv[w][1] * kf[u][1]) + fmaf(qv[w][2], kf[u][2], qv[w][3] * kf[u][3]));
           if (((live >> u) & 1u) == 0u || t * TK + u * KPL + kk > last) s[u] = -INFINITY;
           mx = fmaxf(mx, s[u]);
         }
@@ -950,6 +1081,46 @@ int check(int B, int H, int Hkv, int hd, int Lq, int Lk, long long Nq, long long
 }
 bool grid_ok(long long blocks) { return blocks > 0 && blocks <= 0x7FFFFFFFLL; }
 
+// consecutive 256-byte aligned pieces of a buffer (base null: sizes only)
+struct Carve {
+  unsigned char* base; size_t at = 0;
+  template <typename T> void take(T*& p, size_t n) {
+    if (base != nullptr) p = reinterpret_cast<T*>(base + at);
+    at += (n * sizeof(T) + 255) & ~(size_t)255;
+  }
+};
+size_t carve_planes(Args& a, void* base, bool train) {      // what diff_planes_kernel writes; train: and what the forward keeps for the backward
+  Carve c{static_cast<unsigned char*>(base)};
+  const size_t row = 8 * (size_t)pad_hd(a.hd) + 16, nq = (size_t)a.Nq + PAD, nk = (size_t)a.Nk + PAD, H = a.H, G = a.Hkv;
+  c.take(a.qp, H * nq * row);
+  c.take(a.kp, G * nk * row);
+  c.take(a.vp, G * nk * row);
+  c.take(a.qs, 2 * H * nq);
+  c.take(a.ks, 2 * G * nk);
+  c.take(a.vs, G * nk);
+  c.take(a.ivs, G * nk);
+  c.take(a.lvb, G * nk);
+  if (train) {
+    c.take(a.lse, 2 * H * nq);
+    c.take(a.o12, (size_t)a.Nq * H * 4 * a.hd);
+  }
+  return c.at;
+}
+size_t carve_backward(Args& a, void* base, double*& part) {
+  Carve c{static_cast<unsigned char*>(base)};
+  const size_t row = 8 * (size_t)pad_hd(a.hd) + 16, nq = (size_t)a.Nq + PAD, H = a.H;
+  c.take(a.dp, H * nq * row);
+  c.take(a.ds, H * nq);
+  c.take(a.delta, 2 * H * nq);
+  c.take(part, (size_t)PRE_WG * (H + 2 * a.hd));
+  return c.at;
+}
+Args sizes(int H, int Hkv, int hd, long long Nq, long long Nk) {
+  Args a{};
+  a.H = H; a.Hkv = Hkv; a.hd = hd; a.Nq = Nq; a.Nk = Nk;
+  return a;
+}
+
 template <typename K>
 int start(K kernel, dim3 grid, size_t lds, hipStream_t stream, const Args& a) {
   if (lds > 65536) RT_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
@@ -958,71 +1129,101 @@ int start(K kernel, dim3 grid, size_t lds, hipStream_t stream, const Args& a) {
   return RT_OK;
 }
 // mode: 0 the head fills its tile and rows are 16-byte aligned, 1 aligned, columns checked, 2 single columns, checked
-#define RT_DIFF_START(KERNEL, HDP, MODE, ...)                                                                                        \
-  ((HDP) == 32 ? ((MODE) == 0 ? start(KERNEL<32, 0>, __VA_ARGS__) : (MODE) == 1 ? start(KERNEL<32, 1>, __VA_ARGS__) : start(KERNEL<32, 2>, __VA_ARGS__)) \
-               : ((MODE) == 0 ? start(KERNEL<64, 0>, __VA_ARGS__) : (MODE) == 1 ? start(KERNEL<64, 1>, __VA_ARGS__) : start(KERNEL<64, 2>, __VA_ARGS__)))
+int mode_of(bool vec, int hd) { return !vec ? 2 : (hd == pad_hd(hd) ? 0 : 1); }
 
-template <int R>
-int start_decode(int HDP, int mode, dim3 grid, hipStream_t stream, const Args& a) {
-  if (HDP == 32)
-    return mode == 0 ? start(diff_decode_kernel<32, 0, R>, grid, 0, stream, a) : mode == 1 ? start(diff_decode_kernel<32, 1, R>, grid, 0, stream, a)
-                                                                                           : start(diff_decode_kernel<32, 2, R>, grid, 0, stream, a);
-  return mode == 0 ? start(diff_decode_kernel<64, 0, R>, grid, 0, stream, a) : mode == 1 ? start(diff_decode_kernel<64, 1, R>, grid, 0, stream, a)
-                                                                                         : start(diff_decode_kernel<64, 2, R>, grid, 0, stream, a);
+template <int HD, int R>
+int start_decode(int mode, dim3 grid, hipStream_t stream, const Args& a) {
+  return mode == 0 ? start(diff_decode_kernel<HD, 0, R>, grid, 0, stream, a) : mode == 1 ? start(diff_decode_kernel<HD, 1, R>, grid, 0, stream, a)
+                                                                                         : start(diff_decode_kernel<HD, 2, R>, grid, 0, stream, a);
 }
-
-size_t img_bytes(int HDP) { return HDP == 32 ? 2 * Img<32>::BYTES + Img<64>::BYTES : 2 * Img<64>::BYTES + Img<128>::BYTES; }
+template <int HD>
+int start_decode(long long queries, int mode, dim3 grid, hipStream_t stream, const Args& a) {
+  return queries <= 1 ? start_decode<HD, 1>(mode, grid, stream, a) : queries <= 2 ? start_decode<HD, 2>(mode, grid, stream, a)
+         : queries <= 4 ? start_decode<HD, 4>(mode, grid, stream, a) : start_decode<HD, 8>(mode, grid, stream, a);
+}
+template <int HD>
+int start_planes(const Args& a, int mode, hipStream_t stream) {
+  constexpr int GROUPS = NT / (HD / 2);
+  const long long qb = (a.Nq * a.H + GROUPS - 1) / GROUPS, kb = (a.Nk * a.Hkv + GROUPS - 1) / GROUPS, n = qb + 2 * kb;
+  if (!grid_ok(n)) return RT_ERR_INVALID_ARG;
+  if (mode == 0) diff_planes_kernel<HD, 0><<<(unsigned)n, NT, 0, stream>>>(a, (unsigned)qb, (unsigned)kb);
+  else if (mode == 1) diff_planes_kernel<HD, 1><<<(unsigned)n, NT, 0, stream>>>(a, (unsigned)qb, (unsigned)kb);
+  else diff_planes_kernel<HD, 2><<<(unsigned)n, NT, 0, stream>>>(a, (unsigned)qb, (unsigned)kb);
+  RT_CHECK_LAUNCH();
+  return RT_OK;
+}
+template <int HD>
+int start_pre(const Args& a, int mode, unsigned n, const float* dy, long long lddy, double* part, hipStream_t stream) {
+  if (mode == 0) diff_bwd_pre_kernel<HD, 0><<<n, NT, 0, stream>>>(a, dy, lddy, part);
+  else if (mode == 1) diff_bwd_pre_kernel<HD, 1><<<n, NT, 0, stream>>>(a, dy, lddy, part);
+  else diff_bwd_pre_kernel<HD, 2><<<n, NT, 0, stream>>>(a, dy, lddy, part);
+  RT_CHECK_LAUNCH();
+  return RT_OK;
+}
+#define RT_TRY(call)                 \
+  do {                               \
+    const int rc__ = (call);         \
+    if (rc__ != RT_OK) return rc__;  \
+  } while (0)
 
 }  // namespace
 
 extern "C" {
 
-size_t rt_diffattn_fwd_workspace_bytes(int32_t B, int32_t H, int32_t Hkv, int32_t hd, int32_t Lq, int32_t Lk, int64_t Nq, int32_t train) {
-  if (B <= 0 || H <= 0 || Hkv <= 0 || hd <= 0 || hd > 64 || Lq <= 0 || Lk <= 0 || Nq <= 0 || H % Hkv != 0) return 0;
-  return part_floats(plan_of(B, H, Hkv, hd, Lq, Lk, train != 0), Nq, H, hd) * sizeof(float);
+size_t rt_diffattn_saved_bytes(int32_t H, int32_t Hkv, int32_t hd, int64_t Nq, int64_t Nk) {
+  if (H <= 0 || Hkv <= 0 || hd <= 0 || hd > 64 || Nq < 0 || Nk < 0) return 0;
+  Args a = sizes(H, Hkv, hd, Nq, Nk);
+  return carve_planes(a, nullptr, true);
+}
+
+size_t rt_diffattn_fwd_workspace_bytes(int32_t B, int32_t H, int32_t Hkv, int32_t hd, int32_t Lq, int32_t Lk, int64_t Nq, int64_t Nk, int32_t train) {
+  if (B <= 0 || H <= 0 || Hkv <= 0 || hd <= 0 || hd > 64 || Lq < 0 || Lk < 0 || Nq <= 0 || Nk < 0 || H % Hkv != 0) return 0;
+  const Plan p = plan_of(B, H, Hkv, hd, Lq, Lk, train != 0);
+  Args a = sizes(H, Hkv, hd, Nq, Nk);
+  return part_floats(p, Nq, H, hd) * sizeof(float) + (train == 0 && !p.decode ? carve_planes(a, nullptr, false) + 256 : 0);
 }
 
 int rt_diffattn_fwd(const float* q, int64_t ldq, const float* k, int64_t ldk, const float* v, int64_t ldv, const float* lam, const int64_t* cu_q,
                     const int64_t* cu_k, const int64_t* key_ids, int32_t B, int32_t H, int32_t Hkv, int32_t hd, int32_t Lq, int32_t Lk, int64_t Nq,
-                    int64_t Nk, float scale, int32_t causal, const float* norm_w, float out_scale, float eps, float* y, int64_t ldy, float* o12,
-                    float* lse, void* ws, size_t ws_bytes, hipStream_t stream) {
-  const int rc = check(B, H, Hkv, hd, Lq, Lk, Nq, Nk, cu_q, cu_k);
-  if (rc != RT_OK) return rc;
-  if (Nq == 0) return RT_OK;
+                    int64_t Nk, float scale, int32_t causal, const float* norm_w, float out_scale, float eps, float* y, int64_t ldy, void* saved,
+                    size_t saved_bytes, void* ws, size_t ws_bytes, hipStream_t stream) {
+  RT_TRY(check(B, H, Hkv, hd, Lq, Lk, Nq, Nk, cu_q, cu_k));
   const long long wq = 2LL * H * hd, wk = 2LL * Hkv * hd;
-  if (q == nullptr || lam == nullptr || y == nullptr || ldq < wq || ldy < wq || (o12 == nullptr) != (lse == nullptr)) return RT_ERR_INVALID_ARG;
+  if (lam == nullptr || (Nq > 0 && (q == nullptr || y == nullptr || ldq < wq || ldy < wq))) return RT_ERR_INVALID_ARG;
   if (Nk > 0 && (k == nullptr || v == nullptr || ldk < wk || ldv < wk)) return RT_ERR_INVALID_ARG;
-  Args a{};
+  if (saved != nullptr && (saved_bytes < rt_diffattn_saved_bytes(H, Hkv, hd, Nq, Nk) || ((uintptr_t)saved & 15u) != 0)) return RT_ERR_WORKSPACE;
+  if (Nq == 0) return RT_OK;
+  Args a = sizes(H, Hkv, hd, Nq, Nk);
   a.q = q; a.k = k; a.v = v; a.ldq = ldq; a.ldk = ldk; a.ldv = ldv; a.lam = lam;
   a.cu_q = (const long long*)cu_q; a.cu_k = (const long long*)cu_k; a.key_ids = (const long long*)key_ids;
-  a.B = B; a.H = H; a.Hkv = Hkv; a.hd = hd; a.Lq = Lq; a.Lk = Lk; a.Nq = Nq; a.Nk = Nk;
+  a.B = B; a.Lq = Lq; a.Lk = Lk;
   a.scale = scale > 0.f ? scale : 1.f / sqrtf((float)hd); a.causal = causal;
-  a.norm_w = norm_w; a.out_scale = out_scale; a.eps = eps; a.y = y; a.ldy = ldy; a.o12 = o12; a.lse = lse;
-  const Plan p = plan_of(B > 0 ? B : 1, H, Hkv, hd, Lq > 0 ? Lq : 1, Lk, o12 != nullptr);
+  a.norm_w = norm_w; a.out_scale = out_scale; a.eps = eps; a.y = y; a.ldy = ldy;
+  const Plan p = plan_of(B > 0 ? B : 1, H, Hkv, hd, Lq, Lk, saved != nullptr);
   a.n_split = p.n_split;
+  const size_t part_bytes = part_floats(p, Nq, H, hd) * sizeof(float);
+  const size_t need = part_bytes + (saved == nullptr && !p.decode ? carve_planes(a, nullptr, false) + 256 : 0);
+  if (need > 0 && (ws == nullptr || ws_bytes < need || ((uintptr_t)ws & 15u) != 0)) return RT_ERR_WORKSPACE;
   if (p.n_split > 1) {
-    const size_t need = part_floats(p, Nq, H, hd) * sizeof(float);
-    if (ws == nullptr || ws_bytes < need) return RT_ERR_WORKSPACE;
     a.part = (float*)ws;
-    a.ml = a.part + (size_t)p.n_split * Nq * H * 2 * 2 * hd;
+    a.ml = a.part + (size_t)p.n_split * Nq * H * 4 * hd;
   }
   const int HDP = pad_hd(hd);
-  const bool vec = hd % 4 == 0 && vec_ok(q, ldq) && vec_ok(k, ldk) && vec_ok(v, ldv) && vec_ok(y, ldy) && (o12 == nullptr || vec_ok(o12, 4)) &&
-                   (ws == nullptr || vec_ok(ws, 4));
-  const int mode = !vec ? 2 : (hd == HDP ? 0 : 1);
+  const int mode = mode_of(hd % 4 == 0 && vec_ok(q, ldq) && vec_ok(k, ldk) && vec_ok(v, ldv), hd);
+  a.vec_y = hd % 2 == 0 && vec_ok(y, ldy);
   const long long B1 = B + (cu_q != nullptr ? 1 : 0);
   if (p.decode) {
     if (!grid_ok(B1 * Hkv)) return RT_ERR_INVALID_ARG;
     const long long queries = (long long)(H / Hkv) * (Lq > 0 ? Lq : 1);
     const dim3 grid((unsigned)(B1 * Hkv), p.n_split);
-    const int rc2 = queries <= 1 ? start_decode<1>(HDP, mode, grid, stream, a) : queries <= 2 ? start_decode<2>(HDP, mode, grid, stream, a)
-                    : queries <= 4 ? start_decode<4>(HDP, mode, grid, stream, a) : start_decode<8>(HDP, mode, grid, stream, a);
-    if (rc2 != RT_OK) return rc2;
+    RT_TRY(HDP == 32 ? start_decode<32>(queries, mode, grid, stream, a) : start_decode<64>(queries, mode, grid, stream, a));
   } else {
-    a.n_tiles = (Lq + OWN - 1) / OWN > 0 ? (Lq + OWN - 1) / OWN : 1;
+    a.n_tiles = Lq > 0 ? (Lq + OWN - 1) / OWN : 1;
     if (!grid_ok(B1 * H * a.n_tiles)) return RT_ERR_INVALID_ARG;
-    const int rc2 = RT_DIFF_START(diff_fwd_kernel, HDP, mode, dim3((unsigned)(B1 * H * a.n_tiles), p.n_split), img_bytes(HDP), stream, a);
-    if (rc2 != RT_OK) return rc2;
+    carve_planes(a, saved != nullptr ? saved : (unsigned char*)ws + ((part_bytes + 255) & ~(size_t)255), saved != nullptr);
+    RT_TRY(HDP == 32 ? start_planes<32>(a, mode, stream) : start_planes<64>(a, mode, stream));
+    const dim3 grid((unsigned)(B1 * H * a.n_tiles), p.n_split);
+    RT_TRY(HDP == 32 ? start(diff_fwd_kernel<32>, grid, 2 * fwd_stage<32>(), stream, a) : start(diff_fwd_kernel<64>, grid, 2 * fwd_stage<64>(), stream, a));
   }
   if (p.n_split > 1) {
     if (!grid_ok(Nq * H)) return RT_ERR_INVALID_ARG;
@@ -1033,69 +1234,58 @@ int rt_diffattn_fwd(const float* q, int64_t ldq, const float* k, int64_t ldk, co
 }
 
 size_t rt_diffattn_bwd_workspace_bytes(int32_t H, int32_t hd, int64_t Nq) {
-  if (H <= 0 || hd <= 0 || Nq <= 0) return 0;
-  return sizeof(float) * ((size_t)Nq * H * 2 * hd + (size_t)Nq * H * 2) + sizeof(double) * (size_t)PRE_WG * (H + 2 * hd) + 16;
+  if (H <= 0 || hd <= 0 || hd > 64 || Nq < 0) return 0;
+  Args a = sizes(H, 1, hd, Nq, 0);
+  double* part = nullptr;
+  return carve_backward(a, nullptr, part);
 }
 
-int rt_diffattn_bwd(const float* q, int64_t ldq, const float* k, int64_t ldk, const float* v, int64_t ldv, const float* lam, const int64_t* cu_q,
-                    const int64_t* cu_k, const int64_t* key_ids, int32_t B, int32_t H, int32_t Hkv, int32_t hd, int32_t Lq, int32_t Lk, int64_t Nq,
-                    int64_t Nk, float scale, int32_t causal, const float* norm_w, float out_scale, float eps, const float* o12, const float* lse,
-                    const float* dy, int64_t lddy, float* dq, int64_t lddq, float* dk, int64_t lddk, float* dv, int64_t lddv, float* dlam,
-                    float* dw, void* ws, size_t ws_bytes, hipStream_t stream) {
-  const int rc = check(B, H, Hkv, hd, Lq, Lk, Nq, Nk, cu_q, cu_k);
-  if (rc != RT_OK) return rc;
+int rt_diffattn_bwd(const void* saved, size_t saved_bytes, const float* lam, const int64_t* cu_q, const int64_t* cu_k, const int64_t* key_ids, int32_t B,
+                    int32_t H, int32_t Hkv, int32_t hd, int32_t Lq, int32_t Lk, int64_t Nq, int64_t Nk, float scale, int32_t causal, const float* norm_w,
+                    float out_scale, float eps, const float* dy, int64_t lddy, float* dq, int64_t lddq, float* dk, int64_t lddk, float* dv, int64_t lddv,
+                    float* dlam, float* dw, void* ws, size_t ws_bytes, hipStream_t stream) {
+  RT_TRY(check(B, H, Hkv, hd, Lq, Lk, Nq, Nk, cu_q, cu_k));
   const long long wq = 2LL * H * hd, wk = 2LL * Hkv * hd;
   if (lam == nullptr || dlam == nullptr || (norm_w != nullptr) != (dw != nullptr)) return RT_ERR_INVALID_ARG;
-  if (Nq > 0 && (q == nullptr || o12 == nullptr || lse == nullptr || dy == nullptr || dq == nullptr || ldq < wq || lddy < wq || lddq < wq)) return RT_ERR_INVALID_ARG;
-  if (Nk > 0 && (k == nullptr || v == nullptr || dk == nullptr || dv == nullptr || ldk < wk || ldv < wk || lddk < wk || lddv < wk)) return RT_ERR_INVALID_ARG;
-  if (ws == nullptr || ws_bytes < rt_diffattn_bwd_workspace_bytes(H, hd, Nq > 0 ? Nq : 1) || ((uintptr_t)ws & 15u) != 0) return RT_ERR_WORKSPACE;
-  Args a{};
-  a.q = q; a.k = k; a.v = v; a.ldq = ldq; a.ldk = ldk; a.ldv = ldv; a.lam = lam;
-  a.cu_q = (const long long*)cu_q; a.cu_k = (const long long*)cu_k; a.key_ids = (const long long*)key_ids;
-  a.B = B; a.H = H; a.Hkv = Hkv; a.hd = hd; a.Lq = Lq; a.Lk = Lk; a.Nq = Nq; a.Nk = Nk;
+  if (Nq > 0 && (dy == nullptr || dq == nullptr || lddy < wq || lddq < wq)) return RT_ERR_INVALID_ARG;
+  if (Nk > 0 && (dk == nullptr || dv == nullptr || lddk < wk || lddv < wk)) return RT_ERR_INVALID_ARG;
+  if (saved == nullptr || saved_bytes < rt_diffattn_saved_bytes(H, Hkv, hd, Nq, Nk) || ((uintptr_t)saved & 15u) != 0) return RT_ERR_WORKSPACE;
+  if (ws == nullptr || ws_bytes < rt_diffattn_bwd_workspace_bytes(H, hd, Nq) || ((uintptr_t)ws & 15u) != 0) return RT_ERR_WORKSPACE;
+  Args a = sizes(H, Hkv, hd, Nq, Nk);
+  a.lam = lam; a.cu_q = (const long long*)cu_q; a.cu_k = (const long long*)cu_k; a.key_ids = (const long long*)key_ids;
+  a.B = B; a.Lq = Lq; a.Lk = Lk;
   a.scale = scale > 0.f ? scale : 1.f / sqrtf((float)hd); a.causal = causal;
-  a.norm_w = norm_w; a.out_scale = out_scale; a.eps = eps; a.o12 = const_cast<float*>(o12); a.lse = const_cast<float*>(lse);
+  a.norm_w = norm_w; a.out_scale = out_scale; a.eps = eps;
   a.dq = dq; a.dk = dk; a.dv = dv; a.lddq = lddq; a.lddk = lddk; a.lddv = lddv;
-  double* part = (double*)ws;
-  float* dout = (float*)(part + (size_t)PRE_WG * (H + 2 * hd));
-  dout = (float*)(((uintptr_t)dout + 15u) & ~(uintptr_t)15u);
-  float* delta = dout + (size_t)Nq * H * 2 * hd;
-  a.dout = dout; a.lddo = wq; a.delta = delta;
-  hipStream_t s = stream;
+  a.vec_q = hd % 4 == 0 && vec_ok(dq, lddq);
+  a.vec_kv = hd % 4 == 0 && vec_ok(dk, lddk) && vec_ok(dv, lddv);
+  double* part = nullptr;
+  carve_planes(a, const_cast<void*>(saved), true);
+  carve_backward(a, ws, part);
 
   const int HDP = pad_hd(hd), groups = NT / (HDP / 2);
-  long long n_pre = (Nq * H + groups - 1) / groups, least = (H + groups - 1) / groups;      // (one lane group per head at least)
+  const long long least = (H + groups - 1) / groups;      // (one lane group per head at least)
+  long long n_pre = (Nq * H + groups - 1) / groups;
   n_pre = n_pre > PRE_WG ? PRE_WG : n_pre;
   n_pre = n_pre < least ? least : n_pre;
   if (n_pre > PRE_WG) return RT_ERR_UNSUPPORTED;
-  const bool pre_vec = hd % 2 == 0 && vec_ok(dy, lddy) && vec_ok(o12, 4) && (norm_w == nullptr || vec_ok(norm_w, 4));
-  if (HDP == 32) {
-    if (pre_vec) diff_bwd_pre_kernel<32, true><<<(unsigned)n_pre, NT, 0, s>>>(a, dy, lddy, dout, delta, part);
-    else diff_bwd_pre_kernel<32, false><<<(unsigned)n_pre, NT, 0, s>>>(a, dy, lddy, dout, delta, part);
-  } else {
-    if (pre_vec) diff_bwd_pre_kernel<64, true><<<(unsigned)n_pre, NT, 0, s>>>(a, dy, lddy, dout, delta, part);
-    else diff_bwd_pre_kernel<64, false><<<(unsigned)n_pre, NT, 0, s>>>(a, dy, lddy, dout, delta, part);
-  }
+  const int mode = mode_of(hd % 2 == 0 && vec_ok(dy, lddy) && (norm_w == nullptr || vec_ok(norm_w, 4)), hd);
+  RT_TRY(HDP == 32 ? start_pre<32>(a, mode, (unsigned)n_pre, dy, lddy, part, stream) : start_pre<64>(a, mode, (unsigned)n_pre, dy, lddy, part, stream));
+  diff_bwd_sums_kernel<<<H + 2 * hd, 64, 0, stream>>>(part, (int)n_pre, H, 2 * hd, dlam, dw);
   RT_CHECK_LAUNCH();
-  diff_bwd_sums_kernel<<<H + 2 * hd, 64, 0, s>>>(part, (int)n_pre, H, 2 * hd, dlam, dw);
-  RT_CHECK_LAUNCH();
-
-  const bool vec = hd % 4 == 0 && vec_ok(q, ldq) && vec_ok(k, ldk) && vec_ok(v, ldv) && vec_ok(dq, lddq) && vec_ok(dk, lddk) && vec_ok(dv, lddv);
-  const int mode = !vec ? 2 : (hd == HDP ? 0 : 1);
-  const size_t img = img_bytes(HDP);
   if (Nq > 0) {
     const long long B1 = B + (cu_q != nullptr ? 1 : 0);
     a.n_tiles = Lq > 0 ? (Lq + OWN - 1) / OWN : 1;
     if (!grid_ok(B1 * H * a.n_tiles)) return RT_ERR_INVALID_ARG;
-    const int rc2 = RT_DIFF_START(diff_bwd_dq_kernel, HDP, mode, dim3((unsigned)(B1 * H * a.n_tiles)), img + 4 * 4 * 64 * 16, s, a);
-    if (rc2 != RT_OK) return rc2;
+    const dim3 grid((unsigned)(B1 * H * a.n_tiles));
+    RT_TRY(HDP == 32 ? start(diff_bwd_dq_kernel<32>, grid, dq_lds<32>(), stream, a) : start(diff_bwd_dq_kernel<64>, grid, dq_lds<64>(), stream, a));
   }
   if (Nk > 0) {
     const long long B1 = B + (cu_k != nullptr ? 1 : 0);
     a.n_tiles = Lk > 0 ? (Lk + OWN - 1) / OWN : 1;
     if (!grid_ok(B1 * Hkv * a.n_tiles)) return RT_ERR_INVALID_ARG;
-    const int rc2 = RT_DIFF_START(diff_bwd_dkv_kernel, HDP, mode, dim3((unsigned)(B1 * Hkv * a.n_tiles)), img + 4 * 8 * 64 * 16 + 512, s, a);
-    if (rc2 != RT_OK) return rc2;
+    const dim3 grid((unsigned)(B1 * Hkv * a.n_tiles));
+    RT_TRY(HDP == 32 ? start(diff_bwd_dkv_kernel<32>, grid, dkv_lds<32>(), stream, a) : start(diff_bwd_dkv_kernel<64>, grid, dkv_lds<64>(), stream, a));
   }
   return RT_OK;
 }

@@ -27,6 +27,7 @@ struct Lib {
   decltype(&rt_rotary) rotary = nullptr;
   decltype(&rt_diff_lambda_fwd) lambda_fwd = nullptr;
   decltype(&rt_diff_lambda_bwd) lambda_bwd = nullptr;
+  decltype(&rt_diffattn_saved_bytes) attn_saved = nullptr;
   decltype(&rt_diffattn_fwd_workspace_bytes) attn_fwd_ws = nullptr;
   decltype(&rt_diffattn_fwd) attn_fwd = nullptr;
   decltype(&rt_diffattn_bwd_workspace_bytes) attn_bwd_ws = nullptr;
@@ -47,6 +48,7 @@ void bind(uintptr_t handle, py::object library_error) {
   RT_BIND(rotary, rt_rotary);
   RT_BIND(lambda_fwd, rt_diff_lambda_fwd);
   RT_BIND(lambda_bwd, rt_diff_lambda_bwd);
+  RT_BIND(attn_saved, rt_diffattn_saved_bytes);
   RT_BIND(attn_fwd_ws, rt_diffattn_fwd_workspace_bytes);
   RT_BIND(attn_fwd, rt_diffattn_fwd);
   RT_BIND(attn_bwd_ws, rt_diffattn_bwd_workspace_bytes);
@@ -243,19 +245,20 @@ Tensor diff_lambda(const Tensor& q1_in, const Tensor& k1_in, const Tensor& q2_in
 // ---- differential attention -----------------------------------------------------------------------------------------------------------------
 struct AttnMeta { int64_t B, H, Hkv, hd, Lq, Lk, causal; double scale, out_scale, eps; };
 Tensor attention_call(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& lam, const Tensor& cu_q, const Tensor& cu_k, const Tensor& ids, const Tensor& w,
-                      const AttnMeta& m, Tensor* o12, Tensor* lse) {
+                      const AttnMeta& m, Tensor* saved) {
   c10::DeviceGuard guard(q.device());
   const int64_t Nq = q.size(0), Nk = k.size(0);
   const Tensor y = at::empty({Nq, 2 * m.H * m.hd}, q.options());
-  if (o12 != nullptr) {
-    *o12 = at::empty({Nq, m.H, 2, 2 * m.hd}, q.options());
-    *lse = at::empty({Nq, m.H, 2}, q.options());
+  size_t kept = 0;
+  if (saved != nullptr) {
+    kept = L.attn_saved(m.H, m.Hkv, m.hd, Nq, Nk);
+    *saved = scratch(kept, q);
   }
-  const size_t n = L.attn_fwd_ws(m.B, m.H, m.Hkv, m.hd, m.Lq, m.Lk, Nq, o12 != nullptr);
+  const size_t n = L.attn_fwd_ws(m.B, m.H, m.Hkv, m.hd, m.Lq, m.Lk, Nq, Nk, saved != nullptr);
   const Tensor ws = scratch(n, q);
   status(L.attn_fwd(f(q), ld(q), f(k), ld(k), f(v), ld(v), f(lam), i64(cu_q), i64(cu_k), i64(ids), m.B, m.H, m.Hkv, m.hd, m.Lq, m.Lk, Nq, Nk, (float)m.scale, m.causal, f(w),
-                    (float)m.out_scale, (float)m.eps, f(y), y.size(1), o12 != nullptr ? f(*o12) : nullptr, lse != nullptr ? f(*lse) : nullptr,
-                    ws.defined() ? ws.data_ptr() : nullptr, n, stream_of(q)),
+                    (float)m.out_scale, (float)m.eps, f(y), y.size(1), saved != nullptr ? saved->data_ptr() : nullptr, kept, ws.defined() ? ws.data_ptr() : nullptr, n,
+                    stream_of(q)),
          "rt_diffattn_fwd", true);
   return y;
 }
@@ -264,9 +267,11 @@ struct AttentionNode : torch::autograd::Function<AttentionNode> {
                         const OptTensor& cu_k_opt, const OptTensor& ids_opt, std::vector<int64_t> sizes, double scale, double out_scale, double eps) {
     const AttnMeta m{sizes[0], sizes[1], sizes[2], sizes[3], sizes[4], sizes[5], sizes[6], scale, out_scale, eps};
     const Tensor w = got(w_opt), cu_q = got(cu_q_opt), cu_k = got(cu_k_opt), ids = got(ids_opt);
-    Tensor o12, lse;
-    const Tensor y = attention_call(q, k, v, lam, cu_q, cu_k, ids, w, m, &o12, &lse);
-    ctx->save_for_backward({q, k, v, lam, w, cu_q, cu_k, ids, o12, lse});
+    Tensor saved;
+    const Tensor y = attention_call(q, k, v, lam, cu_q, cu_k, ids, w, m, &saved);
+    ctx->save_for_backward({lam, w, cu_q, cu_k, ids, saved});      // (not q, k, v: their planes are in `saved`)
+    sizes.push_back(q.size(0));
+    sizes.push_back(k.size(0));
     ctx->saved_data["s"] = std::move(sizes);
     ctx->saved_data["f"] = std::vector<double>{scale, out_scale, eps};
     return y;
@@ -274,23 +279,23 @@ struct AttentionNode : torch::autograd::Function<AttentionNode> {
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     once("diff_attention");
     const auto s = ctx->get_saved_variables();
-    const Tensor &q = s[0], &k = s[1], &v = s[2], &lam = s[3], &w = s[4];
+    const Tensor &lam = s[0], &w = s[1], &saved = s[5];
     const auto z = ctx->saved_data["s"].toIntVector();
     const auto x = ctx->saved_data["f"].toDoubleVector();
-    c10::DeviceGuard guard(q.device());
+    c10::DeviceGuard guard(lam.device());
     const Tensor dy = dense_rows(g[0]);
+    const int64_t H = z[1], Hkv = z[2], hd = z[3], Nq = z[7], Nk = z[8];
     variable_list out(12);
-    out[0] = like(q);
-    out[1] = like(k);
-    out[2] = like(v);
+    out[0] = at::empty({Nq, 2 * H * hd}, lam.options());
+    out[1] = at::empty({Nk, 2 * Hkv * hd}, lam.options());
+    out[2] = at::empty({Nk, 2 * Hkv * hd}, lam.options());
     out[3] = like(lam);
     out[4] = like(w);
-    const int64_t Nq = q.size(0), Nk = k.size(0);
-    const size_t n = L.attn_bwd_ws(z[1], z[3], Nq > 0 ? Nq : 1);
-    const Tensor ws = scratch(n, q);
-    status(L.attn_bwd(f(q), ld(q), f(k), ld(k), f(v), ld(v), f(lam), i64(s[5]), i64(s[6]), i64(s[7]), z[0], z[1], z[2], z[3], z[4], z[5], Nq, Nk, (float)x[0], z[6], f(w),
-                      (float)x[1], (float)x[2], f(s[8]), f(s[9]), f(dy), ld(dy), f(out[0]), q.size(1), f(out[1]), k.size(1), f(out[2]), v.size(1), f(out[3]), f(out[4]),
-                      ws.data_ptr(), n, stream_of(q)),
+    const size_t n = L.attn_bwd_ws(H, hd, Nq);
+    const Tensor ws = scratch(n, lam);
+    status(L.attn_bwd(saved.data_ptr(), saved.numel(), f(lam), i64(s[2]), i64(s[3]), i64(s[4]), z[0], H, Hkv, hd, z[4], z[5], Nq, Nk, (float)x[0], z[6], f(w), (float)x[1],
+                      (float)x[2], f(dy), ld(dy), f(out[0]), out[0].size(1), f(out[1]), out[1].size(1), f(out[2]), out[2].size(1), f(out[3]), f(out[4]), ws.data_ptr(), n,
+                      stream_of(lam)),
            "rt_diffattn_bwd", false);
     return out;
   }
@@ -318,7 +323,7 @@ Tensor diff_attention(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in
   const AttnMeta m{B, H, Hkv, hd, Lq, Lk, causal, scale.value_or(0.0), out_scale, eps};
   if (on_tape({&q, &k, &v, &lam, &w}))
     return AttentionNode::apply(q, k, v, lam, opt(w), opt(cu_q), opt(cu_k), opt(ids), std::vector<int64_t>{B, H, Hkv, hd, Lq, Lk, causal}, m.scale, out_scale, eps);
-  return attention_call(q, k, v, lam, cu_q, cu_k, ids, w, m, nullptr, nullptr);
+  return attention_call(q, k, v, lam, cu_q, cu_k, ids, w, m, nullptr);
 }
 
 // ---- norms, gate, residual scale ---------------------------------------------------------------------------------------------------------

@@ -38,29 +38,34 @@ def test_rotary_refuses():
     assert call(M=0) == 0 and call(n=0, kv=0) == 0
 
 
-def _fwd(B=2, H=2, Hkv=2, hd=16, Lq=4, Lk=4, Nq=8, Nk=8, cu_q=None, cu_k=None, q=P, k=P, lam=P, y=P, ld=64, ldk=64, o12=None, lse=None, ws=None, n=0):
-    return _lib.load().rt_diffattn_fwd(q, ld, k, ldk, P, ldk, lam, cu_q, cu_k, None, B, H, Hkv, hd, Lq, Lk, Nq, Nk, 0.0, 1, None, 1.0, 1e-5, y, ld, o12, lse, ws, n, None)
+def _fwd(B=2, H=2, Hkv=2, hd=16, Lq=4, Lk=4, Nq=8, Nk=8, cu_q=None, cu_k=None, q=P, k=P, lam=P, y=P, ld=64, ldk=64, saved=None, sn=0, ws=None, n=0):
+    return _lib.load().rt_diffattn_fwd(q, ld, k, ldk, P, ldk, lam, cu_q, cu_k, None, B, H, Hkv, hd, Lq, Lk, Nq, Nk, 0.0, 1, None, 1.0, 1e-5, y, ld, saved, sn, ws, n, None)
 
 
 def test_attention_refuses():
     for kw in (dict(H=3), dict(H=0), dict(Hkv=0), dict(hd=0), dict(B=-1), dict(Nq=7), dict(Nk=9), dict(q=None), dict(k=None), dict(lam=None), dict(y=None),
-               dict(ld=63), dict(ldk=63), dict(o12=P), dict(lse=P), dict(Lq=-1), dict(Nq=-8)):
+               dict(ld=63), dict(ldk=63), dict(Lq=-1), dict(Nq=-8)):
         assert _fwd(**kw) == INVALID, kw
     assert _fwd(hd=65, ld=260, ldk=260) == UNSUPPORTED
     assert _fwd(B=0, Nq=0, Nk=0) == 0
     lib = _lib.load()
-    need = lib.rt_diffattn_fwd_workspace_bytes(1, 2, 2, 16, 1, 100_000, 1, 0)
-    assert need > 0 and lib.rt_diffattn_fwd_workspace_bytes(64, 2, 2, 16, 200, 200, 12_800, 1) == 0
+    saved = lib.rt_diffattn_saved_bytes(2, 2, 16, 8, 8)
+    assert saved > 0 and lib.rt_diffattn_saved_bytes(2, 2, 65, 8, 8) == 0
+    for kw in (dict(saved=P, sn=saved - 1), dict(saved=P + 4, sn=saved)):
+        assert _fwd(**kw) == WORKSPACE, kw
+    need = lib.rt_diffattn_fwd_workspace_bytes(1, 2, 2, 16, 1, 100_000, 1, 100_000, 0)
+    assert 0 < need < 100_000 * 64 and lib.rt_diffattn_fwd_workspace_bytes(64, 2, 2, 16, 200, 200, 12_800, 12_800, 1) == 0      # (one query: no planes)
+    assert lib.rt_diffattn_fwd_workspace_bytes(64, 2, 2, 16, 200, 200, 12_800, 12_800, 0) > 12_800 * 2 * 3 * 128
     big = dict(B=1, Lq=1, Lk=100_000, Nq=1, Nk=100_000)
     assert _fwd(**big) == WORKSPACE and _fwd(**big, ws=P, n=need - 1) == WORKSPACE
-    assert lib.rt_diffattn_fwd_workspace_bytes(0, 2, 2, 16, 1, 1, 1, 0) == 0 and lib.rt_diffattn_fwd_workspace_bytes(1, 3, 2, 16, 1, 1, 1, 0) == 0
+    assert lib.rt_diffattn_fwd_workspace_bytes(0, 2, 2, 16, 1, 1, 1, 1, 0) == 0 and lib.rt_diffattn_fwd_workspace_bytes(1, 3, 2, 16, 1, 1, 1, 1, 0) == 0
 
-    def bwd(ws=P, n=1 << 30, Nq=8, norm_w=None, dw=None, dlam=P, o12=P, dq=P):
-        return lib.rt_diffattn_bwd(P, 64, P, 64, P, 64, P, None, None, None, 2, 2, 2, 16, 4, 4, Nq, 8, 0.0, 1, norm_w, 1.0, 1e-5, o12, P, P, 64, dq, 64, P, 64, P, 64, dlam,
-                                   dw, ws, n, None)
+    def bwd(sv=P, sn=1 << 30, ws=P, n=1 << 30, Nq=8, norm_w=None, dw=None, dlam=P, dy=P, dq=P, dk=P):
+        return lib.rt_diffattn_bwd(sv, sn, P, None, None, None, 2, 2, 2, 16, 4, 4, Nq, 8, 0.0, 1, norm_w, 1.0, 1e-5, dy, 64, dq, 64, dk, 64, P, 64, dlam, dw, ws, n, None)
 
-    assert bwd(ws=None) == WORKSPACE and bwd(ws=P + 8) == WORKSPACE and bwd(n=lib.rt_diffattn_bwd_workspace_bytes(2, 16, 8) - 1) == WORKSPACE
-    for kw in (dict(Nq=7), dict(norm_w=P), dict(dw=P), dict(dlam=None), dict(o12=None), dict(dq=None)):
+    for kw in (dict(ws=None), dict(ws=P + 8), dict(n=lib.rt_diffattn_bwd_workspace_bytes(2, 16, 8) - 1), dict(sv=None), dict(sn=saved - 1), dict(sv=P + 4)):
+        assert bwd(**kw) == WORKSPACE, kw
+    for kw in (dict(Nq=7), dict(norm_w=P), dict(dw=P), dict(dlam=None), dict(dy=None), dict(dq=None), dict(dk=None)):
         assert bwd(**kw) == INVALID, kw
 
 
