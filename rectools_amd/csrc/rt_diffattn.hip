@@ -19,8 +19,9 @@
 // in the dK/dV pass a key) is the lane, the partner rows are the registers, so probabilities and dS feed the next product from the
 // registers they were made in.  One wave per map rather than one wave for both: its operands and accumulators are half as many registers, which
 // leaves two waves on a SIMD (one's softmax runs under the other's products).  Partner rows stream through LDS 32 at a time, copied as they
-// lie by LDS DMA (global_load_lds: no registers, no address arithmetic): the planes are stored head-major with 16 bytes behind every row,
-// so rows lie an odd number of 16-byte units apart and both read patterns (32 rows of 16 bytes; 4-row transpose blocks) spread over the banks.
+// lie by LDS DMA (global_load_lds: no registers, no address arithmetic): the planes are stored head-major with 48 bytes behind every row, so
+// rows lie 3 sixteen-byte units apart modulo the 256 bytes of the banks: 32 rows of 16 bytes without a conflict, 4-row transpose blocks two-way (with 16
+// bytes behind them: four-way, 192 conflict cycles per wave and chunk of the forward pass).
 #include "rt_attn_planes.h"
 
 namespace {
@@ -37,6 +38,9 @@ constexpr int OWN = 64;    // owner rows per workgroup
 constexpr int CH = 32;     // partner rows per staged chunk
 constexpr int PAD = 32;    // rows behind the last one that a chunk may copy (never used)
 
+// Work of a matrix launch: owner tiles per session (longer sessions loop), (session, head) pairs as they are counted, order (work_of)
+struct Grid { int n_tiles, bhs, paired, blocks; };
+
 struct Args {
   const float* q; const float* k; const float* v; long long ldq, ldk, ldv;
   const float* lam;                      // [H]
@@ -46,16 +50,16 @@ struct Args {
   float scale; int causal;
   const float* norm_w; float out_scale, eps;
   float* y; long long ldy;
-  // planes: rows of [map 1: h | l][map 2: h | l] (q, k) or [h | l] (v, dO), 8 HD bytes + 16, head-major with N + PAD rows per head; scales 2^e
+  // planes: rows of [map 1: h | l][map 2: h | l] (q, k) or [h | l] (v, dO), 8 HD bytes + 48, head-major with N + PAD rows per head; scales 2^e
   unsigned char* qp; unsigned char* kp; unsigned char* vp; unsigned char* dp;
   float* qs; float* ks;                  // [H][2][Nq + PAD], [Hkv][2][Nk + PAD]
   float* vs; float* ivs; float* lvb;     // [Hkv][Nk + PAD]: 2^e, 2^-e, e (minus infinity: the key is masked)
   float* ds;                             // [H][Nq + PAD]
   float* o12;                            // [Nq, H, 2, 2 hd] normalised outputs of the two maps (training)
-  float* lse;                            // [H][2][Nq + PAD] log2-sum-exp2 of the two maps (training)
+  float* lse; float* lsf;                // [H][2][Nq + PAD] of the two maps (training): probability = exp2(s - lse) lsf, lse a whole number
   float* part; float* ml;                // split keys: [n_split, Nq, H, 2, 2 hd] and [n_split, Nq, H, 2, 2] (maximum, sum)
   int n_split;
-  int n_tiles;                           // owner tiles per session in the grid (longer sessions loop)
+  Grid own_q, own_k;                     // launches whose owner rows are queries / keys
   // backward
   float* delta;                          // [H][2][Nq + PAD]
   float* dq; float* dk; float* dv; long long lddq, lddk, lddv; int vec_q, vec_kv;
@@ -124,7 +128,7 @@ __device__ __forceinline__ void put4(float* row, int c, int ncol, f32x4 x, bool 
 
 // ---- the planes --------------------------------------------------------------------------------------------------------------------------
 template <int HD> struct Row {
-  static constexpr int BYTES = 8 * HD + 16, CHUNK = CH * BYTES, UNITS = CHUNK / 16;      // UNITS of 16 bytes per chunk
+  static constexpr int BYTES = 8 * HD + 48, CHUNK = CH * BYTES, UNITS = CHUNK / 16;      // UNITS of 16 bytes per chunk
 };
 // exponent of the row's scale: its largest magnitude comes to 2^13 .. 2^14 (2 x below the fp16 range; what is 2^-18 of it keeps all 22 bits)
 // `least`: values below 2^(least + 14) lose bits.  -126 keeps 2^e a normal number; v takes -80, so that a row sum of weights that carry 2^-e
@@ -232,34 +236,45 @@ template <int NS> __device__ __forceinline__ void load_own(const unsigned char* 
   }
 }
 // acc[r] += sum_c img[row(r)][c0 + c] * own[c], row(r) = 8 (r / 4) + 4 g + r % 4: the partner rows are the registers, the owner the lane
+// All fragments are read in front of the products (the compiler reads each in front of the instruction that needs it: an LDS latency per step).
 template <int HD, int NS>
 __device__ __forceinline__ void rows_dot(const unsigned char* img, int c0, int plane, const P2 (&own)[NS], int i, int g, f32x16& acc) {
   const unsigned char* p = img + i * Row<HD>::BYTES + c0 * 2 + 16 * g;
+  P2 A[NS];
 #pragma unroll
   for (int s = 0; s < NS; ++s) {
-    P2 A;
-    A.h = *reinterpret_cast<const h8*>(p + 32 * s);
-    A.l = *reinterpret_cast<const h8*>(p + 32 * s + plane);
-    acc = mfma3(A, own[s], acc);
+    A[s].h = *reinterpret_cast<const h8*>(p + 32 * s);
+    A[s].l = *reinterpret_cast<const h8*>(p + 32 * s + plane);
   }
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int s = 0; s < NS; ++s) acc = mfma3(A[s], own[s], acc);
 }
 // acc[cb][r] += sum over the 32 partner rows of img[row][c0 + 32 cb + col(r)] * w[row], the lane's weights in the accumulator order of rows_dot
 // (slot j of step t = register 8 t + j = row 16 t + 8 (j / 4) + 4 g + j % 4): the partner rows are the reduction index, read transposed
+// The next fragment is read under the products of the one before.
 template <int HD, int NB>
 __device__ __forceinline__ void cols_dot(const unsigned char* img, int c0, int plane, const P2 (&w)[2], int lane, f32x16 (&acc)[NB]) {
   const int g = lane >> 5;
   const unsigned char* p = img + (4 * g + ((lane & 15) >> 2)) * Row<HD>::BYTES + (c0 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3)) * 2;
+  auto read = [&](int n) {
+    const unsigned char* a = p + 16 * (n / NB) * Row<HD>::BYTES + 64 * (n % NB);
+    const unsigned char* b = a + 8 * Row<HD>::BYTES;
+    P2 A;
+    A.h = __builtin_bit_cast(h8, (s16x8v)__builtin_shufflevector(tr_read(a), tr_read(b), 0, 1, 2, 3, 4, 5, 6, 7));
+    A.l = __builtin_bit_cast(h8, (s16x8v)__builtin_shufflevector(tr_read(a + plane), tr_read(b + plane), 0, 1, 2, 3, 4, 5, 6, 7));
+    return A;
+  };
+  constexpr int AHEAD = 2;
+  P2 A[AHEAD + 1];
 #pragma unroll
-  for (int t = 0; t < 2; ++t)
+  for (int n = 0; n < AHEAD; ++n) A[n] = read(n);
 #pragma unroll
-    for (int cb = 0; cb < NB; ++cb) {
-      const unsigned char* a = p + 16 * t * Row<HD>::BYTES + 64 * cb;
-      const unsigned char* b = a + 8 * Row<HD>::BYTES;
-      P2 A;
-      A.h = __builtin_bit_cast(h8, (s16x8v)__builtin_shufflevector(tr_read(a), tr_read(b), 0, 1, 2, 3, 4, 5, 6, 7));
-      A.l = __builtin_bit_cast(h8, (s16x8v)__builtin_shufflevector(tr_read(a + plane), tr_read(b + plane), 0, 1, 2, 3, 4, 5, 6, 7));
-      acc[cb] = mfma3(A, w[t], acc[cb]);
-    }
+  for (int n = 0; n < 2 * NB; ++n) {
+    if (n + AHEAD < 2 * NB) A[(n + AHEAD) % (AHEAD + 1)] = read(n + AHEAD);
+    __builtin_amdgcn_sched_barrier(0);
+    acc[n % NB] = mfma3(A[n % (AHEAD + 1)], w[n / NB], acc[n % NB]);
+  }
 }
 __device__ __forceinline__ void split16(const float (&x)[16], P2 (&out)[2]) {
 #pragma unroll
@@ -293,16 +308,47 @@ __device__ __forceinline__ void split16_scaled(float (&x)[16], float& inv, f32x1
 }
 constexpr float NO_UNIT = 0x1p126f;      // before the first weight
 
-// blockIdx -> (owner tile, session, head, split); the LAST tile of a session first where it is the heaviest (causal queries)
-struct Work { int tile, b, h, split; };
-__device__ __forceinline__ Work work_of(int n_tiles, int B1, int H, bool last_first) {
-  const int per = B1 * H, o = (int)blockIdx.x / per, bh = (int)blockIdx.x % per;
+// The backward pass recomputes a probability as exp2(s - n) f: n the nearest whole number to the row's log2-sum-exp2, f in 0.7 .. 1.5 the rest.  The log
+// itself, 10 to 30 in magnitude, would be rounded to 2^-20 and make every probability of the row wrong by that (it did: dq, dk, dv were off by
+// 7e-7 in one direction).  base: what was taken from the scores; total: the sum of exp2(s - base).
+__device__ __forceinline__ void row_norm(float base, float total, float& n, float& f) {
+  if (!(total > 0.f)) { n = 0.f; f = total; return; }      // an empty row: every probability 0 (a NaN sum stays one)
+  const float whole = floorf(base);
+  n = rintf(base + __builtin_amdgcn_logf(total));
+  f = __builtin_amdgcn_ldexpf(__builtin_amdgcn_exp2f(whole - base) / total, (int)(n - whole));
+}
+
+// blockIdx -> (owner tile, session, head, split): the tiles of the real sessions, then (b == B) the rows behind the last one.
+// Heavy tiles first (causal: a session's last queries, its first keys): where the launch is many times the machine, the light ones fill the gaps
+// at its end.  Where all workgroups are resident at once (two per CU), each CU keeps the two it is given: then (`paired`) the second half of the
+// tiles comes in the opposite order, a light one to every heavy one.
+// Workgroups go to the eight dies in turn and each die has its own 4 MB of L2: with the (session, head) pairs counted in a multiple of eight (`bhs`:
+// rounded up where there are many), all tiles of a pair, which stream the same chunks, meet on one die.
+struct Work { int tile, b, h, split; bool any; };
+__device__ __forceinline__ Work work_of(const Args& a, const Grid& n, int blk, int H, bool last_first) {
+  const int real = n.bhs * n.n_tiles, half = n.n_tiles / 2, bh = blk % n.bhs;
   Work w;
-  w.tile = last_first ? n_tiles - 1 - o : o;
+  w.split = blockIdx.y;
+  if (blk >= real) {
+    w.b = a.B;
+    w.h = (blk - real) % H;
+    w.tile = (blk - real) / H;
+    w.any = true;
+    return w;
+  }
+  int o = blk / n.bhs;
+  if (n.paired && o >= n.n_tiles - half) o = n.n_tiles - 1 - (o - (n.n_tiles - half));
+  w.tile = last_first ? n.n_tiles - 1 - o : o;
   w.b = bh / H;
   w.h = bh % H;
-  w.split = blockIdx.y;
+  w.any = bh < a.B * H;
   return w;
+}
+// A value that the optimiser takes for new at this point: comparisons with it stay here, instead of being made once per column in front of the
+// loops and kept in hundreds of spilled scalar registers.
+__device__ __forceinline__ int fresh(int x) {
+  asm volatile("" : "+s"(x));
+  return x;
 }
 
 // ---- forward ----------------------------------------------------------------------------------------------------------------------------
@@ -311,22 +357,22 @@ __device__ __forceinline__ Work work_of(int n_tiles, int B1, int H, bool last_fi
 template <int HD> constexpr int fwd_stage() { return 2 * Row<HD>::CHUNK + 512; }      // K | V | key scales of the maps | e, 2^-e
 
 template <int HD>
-__global__ __launch_bounds__(NT, 2) void diff_fwd_kernel(Args a) {
+__global__ __launch_bounds__(NT, HD == 32 ? 3 : 2) void diff_fwd_kernel(Args a) {
   constexpr int DV = 2 * HD, NS = HD / 16, NB = DV / 32, STAGE = fwd_stage<HD>();
   constexpr float UP = 14.f;      // weights come to 2^14 at most
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, mp = wave & 1, rg = wave >> 1, i = lane & 31, g = lane >> 5;
-  const Work wk = work_of(a.n_tiles, a.B + (a.cu_q != nullptr ? 1 : 0), a.H, a.causal != 0);
+  const Work wk = work_of(a, a.own_q, blockIdx.x, a.H, a.causal != 0);
+  if (!wk.any) return;
   const int h = wk.h, hk = h / (a.H / a.Hkv), dv = 2 * a.hd;
   const long long NqP = a.Nq + PAD, NkP = a.Nk + PAD;
 
   if (wk.b == a.B) {      // rows behind the last session: zeros
     if (wk.split != 0) return;
     const long long r0 = rows_used(a.cu_q, a.B, a.Nq);
-    for (long long r = r0 + wk.tile; r < a.Nq; r += a.n_tiles) {
+    for (long long r = r0 + wk.tile; r < a.Nq; r += a.own_q.n_tiles) {
       for (int c = tid; c < dv; c += NT) a.y[r * a.ldy + (long long)h * dv + c] = 0.f;
       if (a.o12 != nullptr) for (int c = tid; c < 2 * dv; c += NT) a.o12[(r * a.H + h) * 2 * dv + c] = 0.f;
-      if (a.lse != nullptr && tid < 2) a.lse[(2 * h + tid) * NqP + r] = 0.f;
     }
     return;
   }
@@ -347,7 +393,7 @@ __global__ __launch_bounds__(NT, 2) void diff_fwd_kernel(Args a) {
     if (wave == 1) dma4((g == 0 ? a.lvb : a.ivs) + hk * NkP + at, dst + 2 * Row<HD>::CHUNK + 256);
   };
 
-  for (int tile = wk.tile; tile * OWN < nq; tile += a.n_tiles) {
+  for (int tile = wk.tile; tile * OWN < nq; tile += a.own_q.n_tiles) {
     const int q0 = tile * OWN + 32 * rg, qi = q0 + i;
     const bool qok = qi < nq;
     const long long qrow = qr0 + min(qi, nq - 1);
@@ -426,6 +472,7 @@ __global__ __launch_bounds__(NT, 2) void diff_fwd_kernel(Args a) {
     const float l = lsum + __shfl_xor(lsum, 32, 64);
     if (a.n_split > 1) {      // partial sums as they are; diff_combine_kernel joins the splits
       if (qok) {
+        const int n = fresh(dv);
         const long long at = (((long long)wk.split * a.Nq + qr0 + qi) * a.H + h) * 2 + mp;
         if (g == 0) { a.ml[2 * at] = m; a.ml[2 * at + 1] = l * 0x1p-14f; }
         float* o = a.part + at * dv;
@@ -433,20 +480,21 @@ __global__ __launch_bounds__(NT, 2) void diff_fwd_kernel(Args a) {
         for (int cb = 0; cb < NB; ++cb)
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            put4(o, 32 * cb + 8 * r + 4 * g, dv, f32x4{O[cb][4 * r], O[cb][4 * r + 1], O[cb][4 * r + 2], O[cb][4 * r + 3]} * 0x1p-14f, (dv & 3) == 0);
+            put4(o, 32 * cb + 8 * r + 4 * g, n, f32x4{O[cb][4 * r], O[cb][4 * r + 1], O[cb][4 * r + 2], O[cb][4 * r + 3]} * 0x1p-14f, (n & 3) == 0);
       }
       continue;
     }
     const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);      // (a NaN sum stays one)
 #pragma unroll
     for (int cb = 0; cb < NB; ++cb) O[cb] *= inv;
-    if (qok && a.lse != nullptr && g == 0) a.lse[(2 * h + mp) * NqP + qr0 + qi] = l > 0.f ? (m - UP) + __builtin_amdgcn_logf(l) : 0.f;
+    if (qok && a.lse != nullptr && g == 0) row_norm(m - UP, l, a.lse[(2 * h + mp) * NqP + qr0 + qi], a.lsf[(2 * h + mp) * NqP + qr0 + qi]);
     if (qok && a.o12 != nullptr) {
-      float* o = a.o12 + (((qr0 + qi) * a.H + h) * 2 + mp) * (long long)dv;
+      const int n = fresh(dv);
+      float* o = a.o12 + (((qr0 + qi) * a.H + h) * 2 + mp) * (long long)n;
 #pragma unroll
       for (int cb = 0; cb < NB; ++cb)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) put4(o, 32 * cb + 8 * r + 4 * g, dv, f32x4{O[cb][4 * r], O[cb][4 * r + 1], O[cb][4 * r + 2], O[cb][4 * r + 3]}, (dv & 3) == 0);
+        for (int r = 0; r < 4; ++r) put4(o, 32 * cb + 8 * r + 4 * g, n, f32x4{O[cb][4 * r], O[cb][4 * r + 1], O[cb][4 * r + 2], O[cb][4 * r + 3]}, (n & 3) == 0);
     }
     // the second map's wave hands its output over; the first one's subtracts, normalises and writes
     barrier();
@@ -474,7 +522,8 @@ __global__ __launch_bounds__(NT, 2) void diff_fwd_kernel(Args a) {
       ss += __shfl_xor(ss, 32, 64);
       const float f = a.norm_w != nullptr ? a.out_scale / sqrtf(ss / (float)dv + a.eps) : a.out_scale;
       if (qok) {
-        float* o = a.y + (qr0 + qi) * a.ldy + (long long)h * dv;
+        const int n = fresh(dv), vec = fresh(a.vec_y);
+        float* o = a.y + (qr0 + qi) * a.ldy + (long long)h * n;
 #pragma unroll
         for (int cb = 0; cb < NB; ++cb)
 #pragma unroll
@@ -482,8 +531,8 @@ __global__ __launch_bounds__(NT, 2) void diff_fwd_kernel(Args a) {
             const int col = 32 * cb + 8 * r + 4 * g;
             f32x4 t;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) t[e] = O[cb][4 * r + e] * f * ((a.norm_w != nullptr && col + e < dv) ? a.norm_w[col + e] : 1.f);
-            put4(o, col, dv, t, a.vec_y != 0);
+            for (int e = 0; e < 4; ++e) t[e] = O[cb][4 * r + e] * f * ((a.norm_w != nullptr && col + e < n) ? a.norm_w[col + e] : 1.f);
+            put4(o, col, n, t, vec != 0);
           }
       }
     }
@@ -504,14 +553,23 @@ __global__ __launch_bounds__(NT) void diff_combine_kernel(Args a) {
     const float m = on ? a.ml[2 * p] : -INFINITY, l = on ? a.ml[2 * p + 1] : 0.f, mx = wave_max(m), base = mx == -INFINITY ? 0.f : mx;
     const float e = on ? __builtin_amdgcn_exp2f(m - base) : 0.f, total = wave_sum(l * e);
     wgt[wave][lane] = e * (total > 0.f ? 1.f / total : (total == 0.f ? 0.f : total));
-    if (a.lse != nullptr && lane == 0) a.lse[(2 * h + wave) * (a.Nq + PAD) + row] = total > 0.f ? mx + __builtin_amdgcn_logf(total) : 0.f;
+    if (a.lse != nullptr && lane == 0) row_norm(mx, total, a.lse[(2 * h + wave) * (a.Nq + PAD) + row], a.lsf[(2 * h + wave) * (a.Nq + PAD) + row]);
   }
   const int slots = NT / dv, c = tid % dv, sub = tid / dv;
   for (int mp = 0; mp < 2; ++mp) {
     __syncthreads();
     float x = 0.f;
     if (sub < slots)
-      for (int s = sub; s < a.n_split; s += slots) x = fmaf(a.part[(((long long)s * plane + at) * 2 + mp) * dv + c], wgt[mp][s], x);
+      for (int s0 = sub; s0 < a.n_split; s0 += 8 * slots) {      // eight loads in flight
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int s = s0 + k * slots;
+          v[k] = s < a.n_split ? a.part[(((long long)s * plane + at) * 2 + mp) * dv + c] : 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x = fmaf(v[k], wgt[mp][min(s0 + k * slots, 63)], x);
+      }
     sums[tid] = x;
     __syncthreads();
     if (tid < dv) {
@@ -610,21 +668,20 @@ __global__ __launch_bounds__(64) void diff_bwd_sums_kernel(const double* part, i
 // ---- backward, dQ: the owner is a query; both maps need G^T = V dO^T, each wave makes it over half of V's columns and they swap halves ------
 // STAGES: two where two workgroups with two chunk buffers fit a CU's LDS (HD 32), else one: the other workgroup's products run under the copy.
 template <int HD> constexpr int bwd_stages() { return HD == 32 ? 2 : 1; }
-template <int HD> constexpr int dq_lds() { return bwd_stages<HD>() * fwd_stage<HD>() + 4 * 4 * 64 * 16; }
-template <int HD> constexpr int dkv_stage() { return 2 * Row<HD>::CHUNK + 1024; }
-template <int HD> constexpr int dkv_lds() { return bwd_stages<HD>() * dkv_stage<HD>() + 4 * 8 * 64 * 16; }
+template <int HD> constexpr int dkv_stage() { return 2 * Row<HD>::CHUNK + 1280; }
+template <int HD> constexpr int bwd_lds() { return bwd_stages<HD>() * dkv_stage<HD>() + 4 * 8 * 64 * 16; }      // (dQ needs less)
 
 template <int HD>
-__global__ __launch_bounds__(NT, 2) void diff_bwd_dq_kernel(Args a) {
+__device__ __forceinline__ void bwd_dq(const Args& a, unsigned char* smem, int blk) {
   constexpr int NS = HD / 16, NB = HD / 32, STAGE = fwd_stage<HD>(), STAGES = bwd_stages<HD>();
-  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   f32x4* swap = reinterpret_cast<f32x4*>(smem + STAGES * STAGE);      // [wave][4][64]
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, mp = wave & 1, rg = wave >> 1, i = lane & 31, g = lane >> 5;
-  const Work wk = work_of(a.n_tiles, a.B + (a.cu_q != nullptr ? 1 : 0), a.H, a.causal != 0);
+  const Work wk = work_of(a, a.own_q, blk, a.H, a.causal != 0);
+  if (!wk.any) return;
   const int h = wk.h, hk = h / (a.H / a.Hkv), hd = a.hd, dv = 2 * hd;
   const long long NqP = a.Nq + PAD, NkP = a.Nk + PAD;
   if (wk.b == a.B) {      // rows behind the last session have no gradient
-    for (long long r = rows_used(a.cu_q, a.B, a.Nq) + wk.tile; r < a.Nq; r += a.n_tiles)
+    for (long long r = rows_used(a.cu_q, a.B, a.Nq) + wk.tile; r < a.Nq; r += a.own_q.n_tiles)
       for (int c = tid; c < dv; c += NT) a.dq[r * a.lddq + (long long)h * dv + c] = 0.f;
     return;
   }
@@ -645,7 +702,7 @@ __global__ __launch_bounds__(NT, 2) void diff_bwd_dq_kernel(Args a) {
     if (wave == 1) dma4((g == 0 ? a.lvb : a.vs) + hk * NkP + at, dst + 2 * Row<HD>::CHUNK + 256);
   };
 
-  for (int tile = wk.tile; tile * OWN < nq; tile += a.n_tiles) {
+  for (int tile = wk.tile; tile * OWN < nq; tile += a.own_q.n_tiles) {
     const int q0 = tile * OWN + 32 * rg, qi = q0 + i;
     const bool qok = qi < nq;
     const long long qrow = qr0 + min(qi, nq - 1);
@@ -653,7 +710,7 @@ __global__ __launch_bounds__(NT, 2) void diff_bwd_dq_kernel(Args a) {
     load_own<NS>(a.qp + (h * NqP + qrow) * Row<HD>::BYTES + mp * 4 * HD, 0, 2 * HD, g, Qp);
     load_own<NS>(a.dp + (h * NqP + qrow) * Row<HD>::BYTES, mp * HD, 4 * HD, g, Dp);
     const float qsc = a.qs[(2 * h + mp) * NqP + qrow] * (a.scale * LOG2E), dsc = a.ds[h * NqP + qrow];
-    const float lse = a.lse[(2 * h + mp) * NqP + qrow], dl = a.delta[(2 * h + mp) * NqP + qrow];
+    const float lse = a.lse[(2 * h + mp) * NqP + qrow], lsf = a.lsf[(2 * h + mp) * NqP + qrow], dl = a.delta[(2 * h + mp) * NqP + qrow];
     f32x16 dQ[NB];
 #pragma unroll
     for (int cb = 0; cb < NB; ++cb) dQ[cb] = zero16();
@@ -716,13 +773,14 @@ __global__ __launch_bounds__(NT, 2) void diff_bwd_dq_kernel(Args a) {
       cols_dot<HD, NB>(img + mp * 4 * HD, 0, 2 * HD, w, lane, dQ);
     }
     if (qok) {
-      float* o = a.dq + (qr0 + qi) * a.lddq + (long long)(2 * h + mp) * hd;
-      const float f = a.scale * sign / unit;
+      const int n = fresh(hd), vec = fresh(a.vec_q);
+      float* o = a.dq + (qr0 + qi) * a.lddq + (long long)(2 * h + mp) * n;
+      const float f = a.scale * sign * lsf / unit;      // (lsf belongs to the row: it waits until here)
 #pragma unroll
       for (int cb = 0; cb < NB; ++cb)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          put4(o, 32 * cb + 8 * r + 4 * g, hd, f32x4{dQ[cb][4 * r], dQ[cb][4 * r + 1], dQ[cb][4 * r + 2], dQ[cb][4 * r + 3]} * f, a.vec_q != 0);
+          put4(o, 32 * cb + 8 * r + 4 * g, n, f32x4{dQ[cb][4 * r], dQ[cb][4 * r + 1], dQ[cb][4 * r + 2], dQ[cb][4 * r + 3]} * f, vec != 0);
     }
   }
 }
@@ -730,16 +788,16 @@ __global__ __launch_bounds__(NT, 2) void diff_bwd_dq_kernel(Args a) {
 // ---- backward, dK and dV: the owner is a key; the query heads of its group are summed in a fixed order ---------------------------------------
 // The two waves of a row group swap their halves of G and their probabilities: each makes dK of its map and dV of its half of the columns.
 template <int HD>
-__global__ __launch_bounds__(NT, 2) void diff_bwd_dkv_kernel(Args a) {
+__device__ __forceinline__ void bwd_dkv(const Args& a, unsigned char* smem, int blk) {
   constexpr int NS = HD / 16, NB = HD / 32, STAGE = dkv_stage<HD>(), STAGES = bwd_stages<HD>();
-  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   f32x4* swap = reinterpret_cast<f32x4*>(smem + STAGES * STAGE);      // [wave][8][64]: G halves, probabilities
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, mp = wave & 1, rg = wave >> 1, i = lane & 31, g = lane >> 5;
-  const Work wk = work_of(a.n_tiles, a.B + (a.cu_k != nullptr ? 1 : 0), a.Hkv, false);
+  const Work wk = work_of(a, a.own_k, blk, a.Hkv, false);
+  if (!wk.any) return;
   const int hk = wk.h, rep = a.H / a.Hkv, hd = a.hd, dv = 2 * hd;
   const long long NqP = a.Nq + PAD, NkP = a.Nk + PAD;
   if (wk.b == a.B) {
-    for (long long r = rows_used(a.cu_k, a.B, a.Nk) + wk.tile; r < a.Nk; r += a.n_tiles)
+    for (long long r = rows_used(a.cu_k, a.B, a.Nk) + wk.tile; r < a.Nk; r += a.own_k.n_tiles)
       for (int c = tid; c < dv; c += NT) {
         a.dk[r * a.lddk + (long long)hk * dv + c] = 0.f;
         a.dv[r * a.lddv + (long long)hk * dv + c] = 0.f;
@@ -752,7 +810,7 @@ __global__ __launch_bounds__(NT, 2) void diff_bwd_dkv_kernel(Args a) {
   const int off = nk - nq;
   const unsigned lds0 = lds_addr(smem);
   const int c_all = (nq + CH - 1) / CH;
-  // scales behind the images: queries of the maps | log sums | deltas | dO, each [2][32]
+  // row values behind the images: scales of the maps' queries | lse | delta | scale of dO | lsf, each [2][32]
   auto issue = [&](int h, int c, int st) {
     const unsigned dst = lds0 + st * STAGE;
     const long long r = h * NqP + qr0 + c * CH;
@@ -761,9 +819,10 @@ __global__ __launch_bounds__(NT, 2) void diff_bwd_dkv_kernel(Args a) {
     const long long at = (2 * h + g) * NqP + qr0 + c * CH + i;
     const float* src = wave == 0 ? a.qs + at : wave == 1 ? a.lse + at : wave == 2 ? a.delta + at : a.ds + h * NqP + qr0 + c * CH + i;
     dma4(src, dst + 2 * Row<HD>::CHUNK + __builtin_amdgcn_readfirstlane(wave) * 256);
+    if (wave == 0) dma4(a.lsf + at, dst + 2 * Row<HD>::CHUNK + 1024);
   };
 
-  for (int tile = wk.tile; tile * OWN < nk; tile += a.n_tiles) {
+  for (int tile = wk.tile; tile * OWN < nk; tile += a.own_k.n_tiles) {
     const int k0 = tile * OWN + 32 * rg, ki = k0 + i;
     const bool kin = ki < nk;
     const long long krow = kr0 + min(ki, nk - 1);
@@ -792,9 +851,12 @@ __global__ __launch_bounds__(NT, 2) void diff_bwd_dkv_kernel(Args a) {
       dma_done();
       barrier();
       if (STAGES == 2 && n + 1 < n_all) issue(hk * rep + (n + 1) / n_ch, c_lo + (n + 1) % n_ch, st ^ 1);
-      if (left < CH) {      // rows behind the session's end: a log sum of infinity, so that exp2 gives 0
+      if (left < CH) {      // rows behind the session's end have no probabilities
         clear_rows<HD>(img, left, tid);
-        if ((tid & 31) >= left) sc[tid] = (tid >> 6) == 1 ? INFINITY : 0.f;
+        if ((tid & 31) >= left) {
+          sc[tid] = 0.f;
+          if (tid < 64) sc[256 + tid] = 0.f;
+        }
         barrier();
       }
       const bool on = k0 < nk && !(a.causal && t0 + 31 + off < k0);
@@ -807,10 +869,11 @@ __global__ __launch_bounds__(NT, 2) void diff_bwd_dkv_kernel(Args a) {
         const int first = a.causal ? ki - off - t0 : -1;      // the first row of the chunk that sees this key
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const f32x4 q4 = *reinterpret_cast<const f32x4*>(sc + 32 * mp + 8 * r + 4 * g), l4 = *reinterpret_cast<const f32x4*>(sc + 64 + 32 * mp + 8 * r + 4 * g);
+          const f32x4 q4 = *reinterpret_cast<const f32x4*>(sc + 32 * mp + 8 * r + 4 * g), l4 = *reinterpret_cast<const f32x4*>(sc + 64 + 32 * mp + 8 * r + 4 * g),
+                      f4 = *reinterpret_cast<const f32x4*>(sc + 256 + 32 * mp + 8 * r + 4 * g);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float x = __builtin_amdgcn_exp2f(fmaf(S[4 * r + e] * q4[e], ksc, -l4[e]));
+            const float x = __builtin_amdgcn_exp2f(fmaf(S[4 * r + e] * q4[e], ksc, -l4[e])) * f4[e];
             p[4 * r + e] = (kok && (!edge || reg_row(4 * r + e, g) >= first)) ? x : 0.f;
           }
           swap[(wave * 8 + r) * 64 + lane] = f32x4{G[4 * r], G[4 * r + 1], G[4 * r + 2], G[4 * r + 3]};
@@ -842,26 +905,36 @@ __global__ __launch_bounds__(NT, 2) void diff_bwd_dkv_kernel(Args a) {
       cols_dot<HD, NB>(img + Row<HD>::CHUNK, mp * HD, 4 * HD, w, lane, dV);
     }
     if (kin) {
-      float* ok = a.dk + (kr0 + ki) * a.lddk + (long long)(2 * hk + mp) * hd;
-      float* ov = a.dv + (kr0 + ki) * a.lddv + (long long)hk * dv;
+      const int n = fresh(hd), vec = fresh(a.vec_kv);
+      float* ok = a.dk + (kr0 + ki) * a.lddk + (long long)(2 * hk + mp) * n;
+      float* ov = a.dv + (kr0 + ki) * a.lddv + (long long)hk * 2 * n;
       const float fk = a.scale / unit_k, fv = 1.f / unit_v;
 #pragma unroll
       for (int cb = 0; cb < NB; ++cb)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int col = 32 * cb + 8 * r + 4 * g;
-          put4(ok, col, hd, f32x4{dK[cb][4 * r], dK[cb][4 * r + 1], dK[cb][4 * r + 2], dK[cb][4 * r + 3]} * fk, a.vec_kv != 0);
-          put4(ov, mp * HD + col, dv, f32x4{dV[cb][4 * r], dV[cb][4 * r + 1], dV[cb][4 * r + 2], dV[cb][4 * r + 3]} * fv, a.vec_kv != 0);
+          put4(ok, col, n, f32x4{dK[cb][4 * r], dK[cb][4 * r + 1], dK[cb][4 * r + 2], dK[cb][4 * r + 3]} * fk, vec != 0);
+          put4(ov, mp * HD + col, 2 * n, f32x4{dV[cb][4 * r], dV[cb][4 * r + 1], dV[cb][4 * r + 2], dV[cb][4 * r + 3]} * fv, vec != 0);
         }
     }
   }
+}
+
+// Both passes in one launch, the dK/dV workgroups (one and a half times the work of the others) first: they share no data, and each alone ends with
+// a few of its longest workgroups on an empty machine.  One launch after the other took 309 + 445 us (two sessions of 4,096, 4 heads of hd 64, causal).
+template <int HD>
+__global__ __launch_bounds__(NT, 2) void diff_bwd_kernel(Args a) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  if ((int)blockIdx.x < a.own_k.blocks) bwd_dkv<HD>(a, smem, blockIdx.x);
+  else bwd_dq<HD>(a, smem, (int)blockIdx.x - a.own_k.blocks);
 }
 
 // ---- few query rows: the products are matrix-vector products, the keys and values are read once and the loads are the work ---------------------
 // A workgroup takes the R queries (rows x heads) that share a key head through its share of the keys.  A wave reads TK keys at a time straight
 // into registers: a key's two maps (and its value row) lie across 2 HD / 4 lanes, four columns each, so every load is whole cache lines; a
 // dot product is four multiply-adds and a sum over the lanes of its map (cross-lane adds, no LDS), the value sums stay with the lanes' columns.  Every wave
-// keeps its own running maximum and sum; no barrier in the loop, 16 loads of 16 bytes in flight per lane.
+// keeps its own running maximum and sum; no barrier in the loop, the next TK keys are read while these are taken.
 constexpr int MAXR = 8;
 
 template <int HD> __device__ __forceinline__ float other_map(float v) {
@@ -876,11 +949,11 @@ template <int HD> __device__ __forceinline__ float keys_sum(float v) {
   if (HD == 32) v += __shfl_xor(v, 16, 64);
   return v + __shfl_xor(v, 32, 64);
 }
-constexpr int decode_keys(int HDP) { return HDP == 32 ? 32 : 16; }      // TK
+constexpr int decode_keys(int HDP) { return HDP == 32 ? 16 : 8; }      // TK
 
 template <int HD, int MODE, int R>
 __global__ __launch_bounds__(NT, R > 4 ? 1 : 2) void diff_decode_kernel(Args a) {
-  constexpr int DV = 2 * HD, LPK = HD / 2, KPL = 64 / LPK, NL = 8, TK = KPL * NL;
+  constexpr int DV = 2 * HD, LPK = HD / 2, KPL = 64 / LPK, NL = 4, TK = KPL * NL;
   __shared__ float wstat[4][R][2][2], wacc[4][R][2][DV];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, kk = lane / LPK, c4 = lane % LPK, mp = c4 / (HD / 4), col = (c4 % (HD / 4)) * 4;
   const int b = blockIdx.x / a.Hkv, hk = blockIdx.x % a.Hkv, rep = a.H / a.Hkv, hd = a.hd, dv = 2 * hd;
@@ -914,29 +987,23 @@ __global__ __launch_bounds__(NT, R > 4 ? 1 : 2) void diff_decode_kernel(Args a) 
     }
     const int k_end = a.causal ? max(0, min(nk, first + rows + off)) : nk;
     const int n_t = (k_end + TK - 1) / TK, each = (n_t + a.n_split - 1) / a.n_split, t_lo = min(n_t, (int)blockIdx.y * each), t_hi = min(n_t, t_lo + each);
-    for (int t = t_lo + wave; t < t_hi; t += 4) {
-      f32x4 kf[NL], vf[NL];
-      unsigned live = 0u;
+    const float* kbase = a.k + kr0 * a.ldk + (long long)(2 * hk + mp) * hd;
+    const float* vbase = a.v + kr0 * a.ldv + (long long)hk * dv;
+    struct Tile { f32x4 k[NL], v[NL]; unsigned live; };
+    auto read = [&](int t, Tile& x) {
+      x.live = 0u;
 #pragma unroll
       for (int u = 0; u < NL; ++u) {
         const int key = t * TK + u * KPL + kk;
-        kf[u] = vf[u] = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (key < k_end && (a.key_ids == nullptr || a.key_ids[kr0 + key] != 0)) {
-          live |= 1u << u;
-          const float* kp = a.k + (kr0 + key) * a.ldk + (long long)(2 * hk + mp) * hd + col;
-          const float* vp = a.v + (kr0 + key) * a.ldv + (long long)hk * dv + 4 * c4;
-          if (MODE < 2) {
-            if (MODE == 0 || col < hd) kf[u] = *reinterpret_cast<const f32x4*>(kp);
-            if (MODE == 0 || 4 * c4 < dv) vf[u] = *reinterpret_cast<const f32x4*>(vp);
-          } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              if (col + e < hd) kf[u][e] = kp[e];
-              if (4 * c4 + e < dv) vf[u][e] = vp[e];
-            }
-          }
+        x.k[u] = x.v[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (t < t_hi && key < k_end && (a.key_ids == nullptr || a.key_ids[kr0 + key] != 0)) {
+          x.live |= 1u << u;
+          x.k[u] = get4<MODE>(kbase + (long long)key * a.ldk, col, hd);
+          x.v[u] = get4<MODE>(vbase + (long long)key * a.ldv, 4 * c4, dv);
         }
       }
+    };
+    auto take = [&](int t, const Tile& x) {
 #pragma unroll
       for (int w = 0; w < R; ++w) {
         if (w >= rows * rep) break;
@@ -944,8 +1011,8 @@ __global__ __launch_bounds__(NT, R > 4 ? 1 : 2) void diff_decode_kernel(Args a) 
         float s[NL], mx = m[w];
 #pragma unroll
         for (int u = 0; u < NL; ++u) {
-          s[u] = group_sum<HD / 4>(fmaf(qv[w][0], kf[u][0], qv[w][1] * kf[u][1]) + fmaf(qv[w][2], kf[u][2], qv[w][3] * kf[u][3]));
-          if (((live >> u) & 1u) == 0u || t * TK + u * KPL + kk > last) s[u] = -INFINITY;
+          s[u] = group_sum<HD / 4>(fmaf(qv[w][0], x.k[u][0], qv[w][1] * x.k[u][1]) + fmaf(qv[w][2], x.k[u][2], qv[w][3] * x.k[u][3]));
+          if (((x.live >> u) & 1u) == 0u || t * TK + u * KPL + kk > last) s[u] = -INFINITY;
           mx = fmaxf(mx, s[u]);
         }
         mx = keys_max<HD>(mx);
@@ -961,12 +1028,21 @@ __global__ __launch_bounds__(NT, R > 4 ? 1 : 2) void diff_decode_kernel(Args a) 
           ps += p;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            acc[w][0][e] = fmaf(p0, vf[u][e], acc[w][0][e]);
-            acc[w][1][e] = fmaf(p1, vf[u][e], acc[w][1][e]);
+            acc[w][0][e] = fmaf(p0, x.v[u][e], acc[w][0][e]);
+            acc[w][1][e] = fmaf(p1, x.v[u][e], acc[w][1][e]);
           }
         }
         l[w] = l[w] * alpha + ps;
       }
+    };
+    Tile x, y;      // one is read while the other is taken
+    read(t_lo + wave, x);
+    for (int t = t_lo + wave; t < t_hi; t += 8) {
+      read(t + 4, y);
+      take(t, x);
+      if (t + 4 >= t_hi) break;
+      read(t + 8, x);
+      take(t + 4, y);
     }
     __syncthreads();      // (the previous pass's readers are done)
 #pragma unroll
@@ -1079,6 +1155,13 @@ int check(int B, int H, int Hkv, int hd, int Lq, int Lk, long long Nq, long long
   if (cu_k == nullptr && Nk != (long long)B * Lk) return RT_ERR_INVALID_ARG;
   return RT_OK;
 }
+// work of B sessions x H heads x tiles of L owner rows (tail: and the rows behind the last session)
+bool plan_grid(Grid& g, int B, int H, int L, bool tail) {
+  const long long bhs = (long long)B * H, counted = bhs >= 64 ? (bhs + 7) / 8 * 8 : (bhs > 0 ? bhs : 1), tiles = L > 0 ? (L + OWN - 1) / OWN : 1;
+  const long long blocks = (counted + (tail ? H : 0)) * tiles;
+  g = Grid{(int)tiles, (int)counted, 0, (int)blocks};
+  return blocks <= 0x3FFFFFFF;
+}
 bool grid_ok(long long blocks) { return blocks > 0 && blocks <= 0x7FFFFFFFLL; }
 
 // consecutive 256-byte aligned pieces of a buffer (base null: sizes only)
@@ -1091,7 +1174,7 @@ struct Carve {
 };
 size_t carve_planes(Args& a, void* base, bool train) {      // what diff_planes_kernel writes; train: and what the forward keeps for the backward
   Carve c{static_cast<unsigned char*>(base)};
-  const size_t row = 8 * (size_t)pad_hd(a.hd) + 16, nq = (size_t)a.Nq + PAD, nk = (size_t)a.Nk + PAD, H = a.H, G = a.Hkv;
+  const size_t row = 8 * (size_t)pad_hd(a.hd) + 48, nq = (size_t)a.Nq + PAD, nk = (size_t)a.Nk + PAD, H = a.H, G = a.Hkv;
   c.take(a.qp, H * nq * row);
   c.take(a.kp, G * nk * row);
   c.take(a.vp, G * nk * row);
@@ -1102,13 +1185,14 @@ size_t carve_planes(Args& a, void* base, bool train) {      // what diff_planes_
   c.take(a.lvb, G * nk);
   if (train) {
     c.take(a.lse, 2 * H * nq);
+    c.take(a.lsf, 2 * H * nq);
     c.take(a.o12, (size_t)a.Nq * H * 4 * a.hd);
   }
   return c.at;
 }
 size_t carve_backward(Args& a, void* base, double*& part) {
   Carve c{static_cast<unsigned char*>(base)};
-  const size_t row = 8 * (size_t)pad_hd(a.hd) + 16, nq = (size_t)a.Nq + PAD, H = a.H;
+  const size_t row = 8 * (size_t)pad_hd(a.hd) + 48, nq = (size_t)a.Nq + PAD, H = a.H;
   c.take(a.dp, H * nq * row);
   c.take(a.ds, H * nq);
   c.take(a.delta, 2 * H * nq);
@@ -1218,11 +1302,11 @@ int rt_diffattn_fwd(const float* q, int64_t ldq, const float* k, int64_t ldk, co
     const dim3 grid((unsigned)(B1 * Hkv), p.n_split);
     RT_TRY(HDP == 32 ? start_decode<32>(queries, mode, grid, stream, a) : start_decode<64>(queries, mode, grid, stream, a));
   } else {
-    a.n_tiles = Lq > 0 ? (Lq + OWN - 1) / OWN : 1;
-    if (!grid_ok(B1 * H * a.n_tiles)) return RT_ERR_INVALID_ARG;
+    if (!plan_grid(a.own_q, B, H, Lq, cu_q != nullptr)) return RT_ERR_INVALID_ARG;
+    a.own_q.paired = causal && (long long)B * H * a.own_q.n_tiles * p.n_split <= 2LL * rt_num_cus();
     carve_planes(a, saved != nullptr ? saved : (unsigned char*)ws + ((part_bytes + 255) & ~(size_t)255), saved != nullptr);
     RT_TRY(HDP == 32 ? start_planes<32>(a, mode, stream) : start_planes<64>(a, mode, stream));
-    const dim3 grid((unsigned)(B1 * H * a.n_tiles), p.n_split);
+    const dim3 grid((unsigned)a.own_q.blocks, p.n_split);
     RT_TRY(HDP == 32 ? start(diff_fwd_kernel<32>, grid, 2 * fwd_stage<32>(), stream, a) : start(diff_fwd_kernel<64>, grid, 2 * fwd_stage<64>(), stream, a));
   }
   if (p.n_split > 1) {
@@ -1273,19 +1357,11 @@ int rt_diffattn_bwd(const void* saved, size_t saved_bytes, const float* lam, con
   RT_TRY(HDP == 32 ? start_pre<32>(a, mode, (unsigned)n_pre, dy, lddy, part, stream) : start_pre<64>(a, mode, (unsigned)n_pre, dy, lddy, part, stream));
   diff_bwd_sums_kernel<<<H + 2 * hd, 64, 0, stream>>>(part, (int)n_pre, H, 2 * hd, dlam, dw);
   RT_CHECK_LAUNCH();
-  if (Nq > 0) {
-    const long long B1 = B + (cu_q != nullptr ? 1 : 0);
-    a.n_tiles = Lq > 0 ? (Lq + OWN - 1) / OWN : 1;
-    if (!grid_ok(B1 * H * a.n_tiles)) return RT_ERR_INVALID_ARG;
-    const dim3 grid((unsigned)(B1 * H * a.n_tiles));
-    RT_TRY(HDP == 32 ? start(diff_bwd_dq_kernel<32>, grid, dq_lds<32>(), stream, a) : start(diff_bwd_dq_kernel<64>, grid, dq_lds<64>(), stream, a));
-  }
-  if (Nk > 0) {
-    const long long B1 = B + (cu_k != nullptr ? 1 : 0);
-    a.n_tiles = Lk > 0 ? (Lk + OWN - 1) / OWN : 1;
-    if (!grid_ok(B1 * Hkv * a.n_tiles)) return RT_ERR_INVALID_ARG;
-    const dim3 grid((unsigned)(B1 * Hkv * a.n_tiles));
-    RT_TRY(HDP == 32 ? start(diff_bwd_dkv_kernel<32>, grid, dkv_lds<32>(), stream, a) : start(diff_bwd_dkv_kernel<64>, grid, dkv_lds<64>(), stream, a));
+  if ((Nq > 0 && !plan_grid(a.own_q, B, H, Lq, cu_q != nullptr)) || (Nk > 0 && !plan_grid(a.own_k, B, Hkv, Lk, cu_k != nullptr))) return RT_ERR_INVALID_ARG;
+  const long long blocks = (long long)a.own_q.blocks + a.own_k.blocks;
+  if (blocks > 0) {
+    const dim3 grid((unsigned)blocks);
+    RT_TRY(HDP == 32 ? start(diff_bwd_kernel<32>, grid, bwd_lds<32>(), stream, a) : start(diff_bwd_kernel<64>, grid, bwd_lds<64>(), stream, a));
   }
   return RT_OK;
 }
