@@ -933,8 +933,9 @@ __global__ __launch_bounds__(NT, 2) void diff_bwd_kernel(Args a) {
 // ---- few query rows: the products are matrix-vector products, the keys and values are read once and the loads are the work ---------------------
 // A workgroup takes the R queries (rows x heads) that share a key head through its share of the keys.  A wave reads TK keys at a time straight
 // into registers: a key's two maps (and its value row) lie across 2 HD / 4 lanes, four columns each, so every load is whole cache lines; a
-// dot product is four multiply-adds and a sum over the lanes of its map (cross-lane adds, no LDS), the value sums stay with the lanes' columns.  Every wave
-// keeps its own running maximum and sum; no barrier in the loop, the next TK keys are read while these are taken.
+// dot product is four multiply-adds and a sum over the lanes of its map (cross-lane adds, no LDS), the two maps' lanes swap their probabilities, the value
+// sums stay with the lanes' columns.  Every lane group keeps its own running maximum and sum until the end; no barrier in the loop, and the
+// next TK keys are read while these are taken.
 constexpr int MAXR = 8;
 
 template <int HD> __device__ __forceinline__ float other_map(float v) {
@@ -955,7 +956,7 @@ template <int HD, int MODE, int R>
 __global__ __launch_bounds__(NT, R > 4 ? 1 : 2) void diff_decode_kernel(Args a) {
   constexpr int DV = 2 * HD, LPK = HD / 2, KPL = 64 / LPK, NL = 4, TK = KPL * NL;
   __shared__ float wstat[4][R][2][2], wacc[4][R][2][DV];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, kk = lane / LPK, c4 = lane % LPK, mp = c4 / (HD / 4), col = (c4 % (HD / 4)) * 4;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, kk = lane / LPK, c4 = lane % LPK, mp = c4 / (HD / 4), cm = c4 % (HD / 4), col = cm * 4;
   const int b = blockIdx.x / a.Hkv, hk = blockIdx.x % a.Hkv, rep = a.H / a.Hkv, hd = a.hd, dv = 2 * hd;
   if (b == a.B) {      // rows behind the last session: zeros
     if (blockIdx.y != 0) return;
@@ -970,7 +971,7 @@ __global__ __launch_bounds__(NT, R > 4 ? 1 : 2) void diff_decode_kernel(Args a) 
   const float qscale = a.scale * LOG2E;
   for (int first = 0; first < nq; first += per) {
     const int rows = min(per, nq - first);
-    f32x4 qv[R], acc[R][2];
+    f32x4 qv[R], acc[R][2];                        // acc: value columns 4 c4 .. + 3 under the two maps
     float m[R], l[R];
 #pragma unroll
     for (int w = 0; w < R; ++w) {                  // query w = (row w / rep, head w % rep)
@@ -1004,35 +1005,40 @@ __global__ __launch_bounds__(NT, R > 4 ? 1 : 2) void diff_decode_kernel(Args a) 
       }
     };
     auto take = [&](int t, const Tile& x) {
+      const bool edge = __any(x.live != (1u << NL) - 1u) || (a.causal && t * TK + TK - 1 > first + off);
 #pragma unroll
       for (int w = 0; w < R; ++w) {
         if (w >= rows * rep) break;
-        const int last = a.causal ? first + w / rep + off : 0x7FFFFFFF;
         float s[NL], mx = m[w];
 #pragma unroll
-        for (int u = 0; u < NL; ++u) {
+        for (int u = 0; u < NL; ++u)
           s[u] = group_sum<HD / 4>(fmaf(qv[w][0], x.k[u][0], qv[w][1] * x.k[u][1]) + fmaf(qv[w][2], x.k[u][2], qv[w][3] * x.k[u][3]));
-          if (((x.live >> u) & 1u) == 0u || t * TK + u * KPL + kk > last) s[u] = -INFINITY;
-          mx = fmaxf(mx, s[u]);
+        if (edge) {
+          const int last = a.causal ? first + w / rep + off : 0x7FFFFFFF;
+#pragma unroll
+          for (int u = 0; u < NL; ++u) s[u] = (((x.live >> u) & 1u) == 0u || t * TK + u * KPL + kk > last) ? -INFINITY : s[u];
         }
-        mx = keys_max<HD>(mx);
-        const float base = mx == -INFINITY ? 0.f : mx, alpha = __builtin_amdgcn_exp2f(m[w] - base);
-        m[w] = mx;
-        const float alpha_o = other_map<HD>(alpha);
-        acc[w][0] *= mp == 0 ? alpha : alpha_o;
-        acc[w][1] *= mp == 0 ? alpha_o : alpha;
-        float ps = 0.f;
+#pragma unroll
+        for (int u = 0; u < NL; ++u) mx = fmaxf(mx, s[u]);
+        if (__any(mx != m[w])) {
+          const float alpha = __builtin_amdgcn_exp2f(m[w] - (mx == -INFINITY ? 0.f : mx));
+          const float other = other_map<HD>(alpha);
+          m[w] = mx;
+          l[w] *= alpha;
+          acc[w][0] *= mp == 0 ? alpha : other;
+          acc[w][1] *= mp == 0 ? other : alpha;
+        }
+        const float base = mx == -INFINITY ? 0.f : mx;
 #pragma unroll
         for (int u = 0; u < NL; ++u) {
           const float p = __builtin_amdgcn_exp2f(s[u] - base), po = other_map<HD>(p), p0 = mp == 0 ? p : po, p1 = mp == 0 ? po : p;
-          ps += p;
+          l[w] += p;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             acc[w][0][e] = fmaf(p0, x.v[u][e], acc[w][0][e]);
             acc[w][1][e] = fmaf(p1, x.v[u][e], acc[w][1][e]);
           }
         }
-        l[w] = l[w] * alpha + ps;
       }
     };
     Tile x, y;      // one is read while the other is taken
@@ -1046,14 +1052,16 @@ __global__ __launch_bounds__(NT, R > 4 ? 1 : 2) void diff_decode_kernel(Args a) 
     }
     __syncthreads();      // (the previous pass's readers are done)
 #pragma unroll
-    for (int w = 0; w < R; ++w) {
-      const float lt = keys_sum<HD>(l[w]);
+    for (int w = 0; w < R; ++w) {                  // the lane groups of the wave meet
+      const float mx = keys_max<HD>(m[w]), e = __builtin_amdgcn_exp2f(m[w] - (mx == -INFINITY ? 0.f : mx)), lt = keys_sum<HD>(l[w] * e);
+      const float eo = other_map<HD>(e);
 #pragma unroll
-      for (int q = 0; q < 2; ++q)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[w][q][e] = keys_sum<HD>(acc[w][q][e]);
+      for (int k = 0; k < 4; ++k) {
+        acc[w][0][k] = keys_sum<HD>(acc[w][0][k] * (mp == 0 ? e : eo));
+        acc[w][1][k] = keys_sum<HD>(acc[w][1][k] * (mp == 0 ? eo : e));
+      }
       if (kk == 0) {
-        if (c4 % (HD / 4) == 0) { wstat[wave][w][mp][0] = m[w]; wstat[wave][w][mp][1] = lt; }
+        if (cm == 0) { wstat[wave][w][mp][0] = mx; wstat[wave][w][mp][1] = lt; }
         *reinterpret_cast<f32x4*>(&wacc[wave][w][0][4 * c4]) = acc[w][0];
         *reinterpret_cast<f32x4*>(&wacc[wave][w][1][4 * c4]) = acc[w][1];
       }
