@@ -196,6 +196,7 @@ __device__ __forceinline__ void dma4(const void* src, unsigned dst) {       // l
   asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %1, off\n\ts_mov_b32 m0, %0" : "=&s"(keep) : "v"(src), "s"(dst) : "memory");
 }
 __device__ __forceinline__ void dma_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+template <int N> __device__ __forceinline__ void dma_left() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void barrier() {      // LDS writes of this wave are visible behind it; LDS DMA is waited for by dma_done
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   __builtin_amdgcn_s_barrier();
@@ -206,6 +207,17 @@ template <int HD> __device__ __forceinline__ void copy_chunk(const unsigned char
 #pragma unroll
   for (int i = 0; i < (Row<HD>::UNITS + NT - 1) / NT; ++i)
     if (tid + i * NT < Row<HD>::UNITS) dma16(src + (size_t)(tid + i * NT) * 16, dst + (wave0 + i * NT) * 16);
+}
+// Copies of a chunk pair a wave issues (two images; row values by waves 0 and 1), and the wait that leaves `later` chunk pairs in flight: copies
+// land in the order of their issue
+template <int HD> constexpr int copies(bool first_waves) {
+  return 2 * (Row<HD>::UNITS / NT + (first_waves && Row<HD>::UNITS % NT > 0 ? 1 : 0)) + (first_waves ? 1 : 0);
+}
+template <int HD> __device__ __forceinline__ void dma_left_chunks(int later, bool first_waves) {
+  static_assert(Row<HD>::UNITS % NT <= 128, "the tail of an image is copied by waves 0 and 1");
+  if (later <= 0) dma_left<0>();
+  else if (later == 1) { if (first_waves) dma_left<copies<HD>(true)>(); else dma_left<copies<HD>(false)>(); }
+  else { if (first_waves) dma_left<2 * copies<HD>(true)>(); else dma_left<2 * copies<HD>(false)>(); }
 }
 // rows [left, CH) of two staged images: zeros (they belong to the next session, or to nobody)
 template <int HD> __device__ __forceinline__ void clear_rows(unsigned char* img, int left, int tid) {
@@ -354,11 +366,12 @@ __device__ __forceinline__ int fresh(int x) {
 // ---- forward ----------------------------------------------------------------------------------------------------------------------------
 // Values carry their row's scale 2^e: the running maximum is that of s + e, so the weights exp2(s + e - m) stay below one whatever the scales
 // are, and the row sum takes them back by 2^-e.
+template <int HD> constexpr int fwd_stages() { return 2; }
 template <int HD> constexpr int fwd_stage() { return 2 * Row<HD>::CHUNK + 512; }      // K | V | key scales of the maps | e, 2^-e
 
 template <int HD>
 __global__ __launch_bounds__(NT, HD == 32 ? 3 : 2) void diff_fwd_kernel(Args a) {
-  constexpr int DV = 2 * HD, NS = HD / 16, NB = DV / 32, STAGE = fwd_stage<HD>();
+  constexpr int DV = 2 * HD, NS = HD / 16, NB = DV / 32, STAGE = fwd_stage<HD>(), STAGES = fwd_stages<HD>();
   constexpr float UP = 14.f;      // weights come to 2^14 at most
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, mp = wave & 1, rg = wave >> 1, i = lane & 31, g = lane >> 5;
@@ -413,15 +426,18 @@ __global__ __launch_bounds__(NT, HD == 32 ? 3 : 2) void diff_fwd_kernel(Args a) 
       c_hi = min(c_hi, c_lo + each);
     }
     barrier();      // (the previous tile's readers are done)
-    if (c_lo < c_hi) issue(c_lo, 0);
+#pragma unroll
+    for (int k = 0; k < STAGES - 1; ++k)
+      if (c_lo + k < c_hi) issue(c_lo + k, k);
     int st = 0;
-    for (int c = c_lo; c < c_hi; ++c, st ^= 1) {
+    for (int c = c_lo; c < c_hi; ++c) {
       const int t0 = c * CH, left = nk - t0;
       unsigned char* img = smem + st * STAGE;
       float* sc = reinterpret_cast<float*>(img + 2 * Row<HD>::CHUNK);
-      dma_done();
+      dma_left_chunks<HD>(min(STAGES - 2, c_hi - 1 - c), wave < 2);
       barrier();                                    // chunk c is here, chunk c - 1 has been read
-      if (c + 1 < c_hi) issue(c + 1, st ^ 1);
+      if (c + STAGES - 1 < c_hi) issue(c + STAGES - 1, st == 0 ? STAGES - 1 : st - 1);
+      st = st == STAGES - 1 ? 0 : st + 1;
       if (left < CH) {
         clear_rows<HD>(img, left, tid);
         if (tid < 128 && (tid & 31) >= left) sc[tid] = 0.f;
@@ -1315,7 +1331,7 @@ int rt_diffattn_fwd(const float* q, int64_t ldq, const float* k, int64_t ldk, co
     carve_planes(a, saved != nullptr ? saved : (unsigned char*)ws + ((part_bytes + 255) & ~(size_t)255), saved != nullptr);
     RT_TRY(HDP == 32 ? start_planes<32>(a, mode, stream) : start_planes<64>(a, mode, stream));
     const dim3 grid((unsigned)a.own_q.blocks, p.n_split);
-    RT_TRY(HDP == 32 ? start(diff_fwd_kernel<32>, grid, 2 * fwd_stage<32>(), stream, a) : start(diff_fwd_kernel<64>, grid, 2 * fwd_stage<64>(), stream, a));
+    RT_TRY(HDP == 32 ? start(diff_fwd_kernel<32>, grid, fwd_stages<32>() * fwd_stage<32>(), stream, a) : start(diff_fwd_kernel<64>, grid, fwd_stages<64>() * fwd_stage<64>(), stream, a));
   }
   if (p.n_split > 1) {
     if (!grid_ok(Nq * H)) return RT_ERR_INVALID_ARG;
