@@ -259,8 +259,10 @@ __device__ __forceinline__ void rows_dot(const unsigned char* img, int c0, int p
     A[s].l = *reinterpret_cast<const h8*>(p + 32 * s + plane);
   }
   __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_setprio(1);
 #pragma unroll
   for (int s = 0; s < NS; ++s) acc = mfma3(A[s], own[s], acc);
+  __builtin_amdgcn_s_setprio(0);
 }
 // acc[cb][r] += sum over the 32 partner rows of img[row][c0 + 32 cb + col(r)] * w[row], the lane's weights in the accumulator order of rows_dot
 // (slot j of step t = register 8 t + j = row 16 t + 8 (j / 4) + 4 g + j % 4): the partner rows are the reduction index, read transposed
@@ -281,12 +283,14 @@ __device__ __forceinline__ void cols_dot(const unsigned char* img, int c0, int p
   P2 A[AHEAD + 1];
 #pragma unroll
   for (int n = 0; n < AHEAD; ++n) A[n] = read(n);
+  __builtin_amdgcn_s_setprio(1);
 #pragma unroll
   for (int n = 0; n < 2 * NB; ++n) {
     if (n + AHEAD < 2 * NB) A[(n + AHEAD) % (AHEAD + 1)] = read(n + AHEAD);
     __builtin_amdgcn_sched_barrier(0);
     acc[n % NB] = mfma3(A[n % (AHEAD + 1)], w[n / NB], acc[n % NB]);
   }
+  __builtin_amdgcn_s_setprio(0);
 }
 __device__ __forceinline__ void split16(const float (&x)[16], P2 (&out)[2]) {
 #pragma unroll
