@@ -894,8 +894,15 @@ __device__ __forceinline__ void bwd_dkv(const Args& a, unsigned char* smem, int 
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const float x = __builtin_amdgcn_exp2f(fmaf(S[4 * r + e] * q4[e], ksc, -l4[e])) * f4[e];
-            p[4 * r + e] = (kok && (!edge || reg_row(4 * r + e, g) >= first)) ? x : 0.f;
+            p[4 * r + e] = x;
           }
+        }
+        if (edge) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) p[r] = reg_row(r, g) >= first ? p[r] : 0.f;
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
           swap[(wave * 8 + r) * 64 + lane] = f32x4{G[4 * r], G[4 * r + 1], G[4 * r + 2], G[4 * r + 3]};
           swap[(wave * 8 + 4 + r) * 64 + lane] = f32x4{p[4 * r], p[4 * r + 1], p[4 * r + 2], p[4 * r + 3]};
         }
@@ -924,7 +931,7 @@ __device__ __forceinline__ void bwd_dkv(const Args& a, unsigned char* smem, int 
       split16_scaled<NB>(x, unit_v, dV, w);
       cols_dot<HD, NB>(img + Row<HD>::CHUNK, mp * HD, 4 * HD, w, lane, dV);
     }
-    if (kin) {
+    if (kin) {      // a masked key's lane holds whatever its zeroed row made of the probabilities: its gradients are zero
       const int n = fresh(hd), vec = fresh(a.vec_kv);
       float* ok = a.dk + (kr0 + ki) * a.lddk + (long long)(2 * hk + mp) * n;
       float* ov = a.dv + (kr0 + ki) * a.lddv + (long long)hk * 2 * n;
@@ -934,8 +941,11 @@ __device__ __forceinline__ void bwd_dkv(const Args& a, unsigned char* smem, int 
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int col = 32 * cb + 8 * r + 4 * g;
-          put4(ok, col, n, f32x4{dK[cb][4 * r], dK[cb][4 * r + 1], dK[cb][4 * r + 2], dK[cb][4 * r + 3]} * fk, vec != 0);
-          put4(ov, mp * HD + col, 2 * n, f32x4{dV[cb][4 * r], dV[cb][4 * r + 1], dV[cb][4 * r + 2], dV[cb][4 * r + 3]} * fv, vec != 0);
+          f32x4 tk = f32x4{dK[cb][4 * r], dK[cb][4 * r + 1], dK[cb][4 * r + 2], dK[cb][4 * r + 3]} * fk;
+          f32x4 tv = f32x4{dV[cb][4 * r], dV[cb][4 * r + 1], dV[cb][4 * r + 2], dV[cb][4 * r + 3]} * fv;
+          if (!kok) tk = tv = f32x4{0.f, 0.f, 0.f, 0.f};
+          put4(ok, col, n, tk, vec != 0);
+          put4(ov, mp * HD + col, 2 * n, tv, vec != 0);
         }
     }
   }
@@ -1155,16 +1165,23 @@ bool vec_ok(const void* p, long long ld) { return ((uintptr_t)p & 15u) == 0 && l
 int pad_hd(int hd) { return hd <= 32 ? 32 : 64; }
 
 struct Plan { bool decode; int n_split; };
-// Training keeps the outputs of both maps and always takes the matrix kernel.  Otherwise queries that share a key head and are few
-// (<= MAXR of them per session) go through diff_decode_kernel.  Keys are split over workgroups until the launch has about 4 (decode) or 2
-// workgroups per CU, at least 2 (decode) or 4 chunks each.
+// Training keeps the outputs of both maps and always takes the matrix kernels.  Otherwise few queries to a key head (rows x heads of its group) go
+// through diff_decode_kernel, up to twelve of them, in two passes over the keys behind eight.  Decode against matrix, causal, hd 64, 2 key heads:
+//   1 query   8 x 65,536 keys 185 | 763 us   256 x 200 19 | 62     1 x 8,192 17 | 29
+//   8         8 x 65,536      370 | 1158     256 x 200 60 | 128    1 x 8,192 30 | 35
+//   10        8 x 65,536      555 | 837      256 x 200 84 | 88     1 x 8,192 39 | 31
+//   16        8 x 65,536      729 | 837      256 x 200 114 | 89    1 x 8,192 48 | 31
+// Keys are split over workgroups until the launch has what the machine holds at once, two per CU (decode of more than four queries: its registers
+// leave one), with 2 (decode) or 4 chunks each at least.  Decode, 64 sessions of 2,048 keys: 4 queries 52 us (1 per CU: 68, 4 per CU: 58), 8 queries
+// 105 (2: 114, 4: 133); matrix, 8 x 1,024 rows of 4 heads: 82 (1: 84, 4: 134).
 Plan plan_of(int B, int H, int Hkv, int hd, int Lq, int Lk, bool train) {
   Plan p;
   const int rep = H / Hkv;
-  p.decode = !train && (long long)rep * Lq <= MAXR;
+  const long long queries = (long long)rep * Lq;
+  p.decode = !train && rep <= MAXR && queries <= MAXR + MAXR / 2;
   const long long wgs = p.decode ? (long long)B * Hkv : (long long)B * H * ((Lq + OWN - 1) / OWN);
   const int chunk = p.decode ? 4 * decode_keys(pad_hd(hd)) : CH;      // keys a workgroup takes at once
-  const long long want = (long long)rt_num_cus() * (p.decode ? 4 : 2);
+  const long long want = (long long)rt_num_cus() * (p.decode && queries > 4 ? 1 : 2);
   long long s = wgs > 0 ? want / wgs : 1;
   const long long most = Lk / (p.decode ? 2 * chunk : 4 * chunk);
   if (s > most) s = most;
@@ -1176,9 +1193,10 @@ size_t part_floats(const Plan& p, long long Nq, int H, int hd) {
   return p.n_split > 1 ? (size_t)p.n_split * (size_t)Nq * H * 2 * (2 * (size_t)hd + 2) : 0;
 }
 
+constexpr long long MAX_ROWS = 0x3FFFFFFF;      // rows within a session are counted in 32 bits; offsets into q, k, v are 64 bits everywhere
 int check(int B, int H, int Hkv, int hd, int Lq, int Lk, long long Nq, long long Nk, const void* cu_q, const void* cu_k) {
   if (B < 0 || H <= 0 || Hkv <= 0 || hd <= 0 || Lq < 0 || Lk < 0 || Nq < 0 || Nk < 0 || H % Hkv != 0) return RT_ERR_INVALID_ARG;
-  if (hd > 64) return RT_ERR_UNSUPPORTED;
+  if (hd > 64 || Nq > MAX_ROWS || Nk > MAX_ROWS) return RT_ERR_UNSUPPORTED;
   if (cu_q == nullptr && Nq != (long long)B * Lq) return RT_ERR_INVALID_ARG;
   if (cu_k == nullptr && Nk != (long long)B * Lk) return RT_ERR_INVALID_ARG;
   return RT_OK;
