@@ -1201,14 +1201,16 @@ int check(int B, int H, int Hkv, int hd, int Lq, int Lk, long long Nq, long long
   if (cu_k == nullptr && Nk != (long long)B * Lk) return RT_ERR_INVALID_ARG;
   return RT_OK;
 }
+// a launch dimension holds less than 2^32 threads
+bool grid_ok(long long blocks) { return blocks > 0 && blocks <= 0xFFFFFFFFLL / NT; }
 // work of B sessions x H heads x tiles of L owner rows (tail: and the rows behind the last session)
 bool plan_grid(Grid& g, int B, int H, int L, bool tail) {
   const long long bhs = (long long)B * H, counted = bhs >= 64 ? (bhs + 7) / 8 * 8 : (bhs > 0 ? bhs : 1), tiles = L > 0 ? (L + OWN - 1) / OWN : 1;
   const long long blocks = (counted + (tail ? H : 0)) * tiles;
   g = Grid{(int)tiles, (int)counted, 0, (int)blocks};
-  return blocks <= 0x3FFFFFFF;
+  return grid_ok(blocks);
 }
-bool grid_ok(long long blocks) { return blocks > 0 && blocks <= 0x7FFFFFFFLL; }
+
 
 // consecutive 256-byte aligned pieces of a buffer (base null: sizes only)
 struct Carve {
@@ -1275,7 +1277,7 @@ template <int HD>
 int start_planes(const Args& a, int mode, hipStream_t stream) {
   constexpr int GROUPS = NT / (HD / 2);
   const long long qb = (a.Nq * a.H + GROUPS - 1) / GROUPS, kb = (a.Nk * a.Hkv + GROUPS - 1) / GROUPS, n = qb + 2 * kb;
-  if (!grid_ok(n)) return RT_ERR_INVALID_ARG;
+  if (!grid_ok(n)) return RT_ERR_UNSUPPORTED;
   if (mode == 0) diff_planes_kernel<HD, 0><<<(unsigned)n, NT, 0, stream>>>(a, (unsigned)qb, (unsigned)kb);
   else if (mode == 1) diff_planes_kernel<HD, 1><<<(unsigned)n, NT, 0, stream>>>(a, (unsigned)qb, (unsigned)kb);
   else diff_planes_kernel<HD, 2><<<(unsigned)n, NT, 0, stream>>>(a, (unsigned)qb, (unsigned)kb);
@@ -1307,8 +1309,8 @@ size_t rt_diffattn_saved_bytes(int32_t H, int32_t Hkv, int32_t hd, int64_t Nq, i
 }
 
 size_t rt_diffattn_fwd_workspace_bytes(int32_t B, int32_t H, int32_t Hkv, int32_t hd, int32_t Lq, int32_t Lk, int64_t Nq, int64_t Nk, int32_t train) {
-  if (B <= 0 || H <= 0 || Hkv <= 0 || hd <= 0 || hd > 64 || Lq < 0 || Lk < 0 || Nq <= 0 || Nk < 0 || H % Hkv != 0) return 0;
-  const Plan p = plan_of(B, H, Hkv, hd, Lq, Lk, train != 0);
+  if (B < 0 || H <= 0 || Hkv <= 0 || hd <= 0 || hd > 64 || Lq < 0 || Lk < 0 || Nq <= 0 || Nk < 0 || H % Hkv != 0) return 0;
+  const Plan p = plan_of(B > 0 ? B : 1, H, Hkv, hd, Lq, Lk, train != 0);
   Args a = sizes(H, Hkv, hd, Nq, Nk);
   return part_floats(p, Nq, H, hd) * sizeof(float) + (train == 0 && !p.decode ? carve_planes(a, nullptr, false) + 256 : 0);
 }
@@ -1319,7 +1321,7 @@ int rt_diffattn_fwd(const float* q, int64_t ldq, const float* k, int64_t ldk, co
                     size_t saved_bytes, void* ws, size_t ws_bytes, hipStream_t stream) {
   RT_TRY(check(B, H, Hkv, hd, Lq, Lk, Nq, Nk, cu_q, cu_k));
   const long long wq = 2LL * H * hd, wk = 2LL * Hkv * hd;
-  if (lam == nullptr || (Nq > 0 && (q == nullptr || y == nullptr || ldq < wq || ldy < wq))) return RT_ERR_INVALID_ARG;
+  if (lam == nullptr || (norm_w != nullptr && !(eps > 0.f)) || (Nq > 0 && (q == nullptr || y == nullptr || ldq < wq || ldy < wq))) return RT_ERR_INVALID_ARG;
   if (Nk > 0 && (k == nullptr || v == nullptr || ldk < wk || ldv < wk)) return RT_ERR_INVALID_ARG;
   if (saved != nullptr && (saved_bytes < rt_diffattn_saved_bytes(H, Hkv, hd, Nq, Nk) || ((uintptr_t)saved & 15u) != 0)) return RT_ERR_WORKSPACE;
   if (Nq == 0) return RT_OK;
@@ -1343,12 +1345,12 @@ int rt_diffattn_fwd(const float* q, int64_t ldq, const float* k, int64_t ldk, co
   a.vec_y = hd % 2 == 0 && vec_ok(y, ldy);
   const long long B1 = B + (cu_q != nullptr ? 1 : 0);
   if (p.decode) {
-    if (!grid_ok(B1 * Hkv)) return RT_ERR_INVALID_ARG;
+    if (!grid_ok(B1 * Hkv)) return RT_ERR_UNSUPPORTED;
     const long long queries = (long long)(H / Hkv) * (Lq > 0 ? Lq : 1);
     const dim3 grid((unsigned)(B1 * Hkv), p.n_split);
     RT_TRY(HDP == 32 ? start_decode<32>(queries, mode, grid, stream, a) : start_decode<64>(queries, mode, grid, stream, a));
   } else {
-    if (!plan_grid(a.own_q, B, H, Lq, cu_q != nullptr)) return RT_ERR_INVALID_ARG;
+    if (!plan_grid(a.own_q, B, H, Lq, cu_q != nullptr)) return RT_ERR_UNSUPPORTED;
     a.own_q.paired = causal && (long long)B * H * a.own_q.n_tiles * p.n_split <= 2LL * rt_num_cus();
     carve_planes(a, saved != nullptr ? saved : (unsigned char*)ws + ((part_bytes + 255) & ~(size_t)255), saved != nullptr);
     RT_TRY(HDP == 32 ? start_planes<32>(a, mode, stream) : start_planes<64>(a, mode, stream));
@@ -1356,7 +1358,7 @@ int rt_diffattn_fwd(const float* q, int64_t ldq, const float* k, int64_t ldk, co
     RT_TRY(HDP == 32 ? start(diff_fwd_kernel<32>, grid, fwd_stages<32>() * fwd_stage<32>(), stream, a) : start(diff_fwd_kernel<64>, grid, fwd_stages<64>() * fwd_stage<64>(), stream, a));
   }
   if (p.n_split > 1) {
-    if (!grid_ok(Nq * H)) return RT_ERR_INVALID_ARG;
+    if (!grid_ok(Nq * H)) return RT_ERR_UNSUPPORTED;
     diff_combine_kernel<<<(unsigned)(Nq * H), NT, 0, stream>>>(a);
     RT_CHECK_LAUNCH();
   }
@@ -1403,8 +1405,9 @@ int rt_diffattn_bwd(const void* saved, size_t saved_bytes, const float* lam, con
   RT_TRY(HDP == 32 ? start_pre<32>(a, mode, (unsigned)n_pre, dy, lddy, part, stream) : start_pre<64>(a, mode, (unsigned)n_pre, dy, lddy, part, stream));
   diff_bwd_sums_kernel<<<H + 2 * hd, 64, 0, stream>>>(part, (int)n_pre, H, 2 * hd, dlam, dw);
   RT_CHECK_LAUNCH();
-  if ((Nq > 0 && !plan_grid(a.own_q, B, H, Lq, cu_q != nullptr)) || (Nk > 0 && !plan_grid(a.own_k, B, Hkv, Lk, cu_k != nullptr))) return RT_ERR_INVALID_ARG;
+  if ((Nq > 0 && !plan_grid(a.own_q, B, H, Lq, cu_q != nullptr)) || (Nk > 0 && !plan_grid(a.own_k, B, Hkv, Lk, cu_k != nullptr))) return RT_ERR_UNSUPPORTED;
   const long long blocks = (long long)a.own_q.blocks + a.own_k.blocks;
+  if (blocks > 0 && !grid_ok(blocks)) return RT_ERR_UNSUPPORTED;
   if (blocks > 0) {
     const dim3 grid((unsigned)blocks);
     RT_TRY(HDP == 32 ? start(diff_bwd_kernel<32>, grid, bwd_lds<32>(), stream, a) : start(diff_bwd_kernel<64>, grid, bwd_lds<64>(), stream, a));

@@ -57,6 +57,12 @@ __device__ __forceinline__ float drop_factor(const NgArgs& a, long long i, unsig
   return (((i & 1) ? (w >> 16) : (w & 0xFFFFu)) >= thr) ? inv_keep : 0.f;
 }
 __device__ __forceinline__ float sigmoid(float z) { return 1.f / (1.f + expf(-z)); }
+// and one minus it, without the cancellation behind large z
+__device__ __forceinline__ float sigmoid(float z, float& rest) {
+  const float e = expf(-fabsf(z)), near = 1.f / (1.f + e), far = e * near;
+  rest = z > 0.f ? far : near;
+  return z > 0.f ? near : far;
+}
 
 // mean (LayerNorm) and 1 / deviation of a row held in registers; v becomes the normalised row
 template <int TPR, int NE, bool LAYER>
@@ -217,11 +223,12 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_gate_bwd_kernel(Ng
         o[e] = a.alpha * g[i];
         const float uu = a.post ? (u[i] - sv[0]) * sv[1] : u[i];
         float n = a.post ? uu * pw[i] + pb[i] : uu;
-        const float gate = a.z != nullptr ? sigmoid(z[i]) : 1.f;
+        float rest = 0.f;
+        const float gate = a.z != nullptr ? sigmoid(z[i], rest) : 1.f;
         const float keep = a.p > 0.f ? drop_factor(a, base + col[k] + e, thr, inv_keep) : 1.f;
         n *= keep;
         const float gs = g[i] * s[i];
-        oz[e] = gs * n * gate * (1.f - gate);
+        oz[e] = gs * n * gate * rest;
         const float gn = gs * gate * keep;
         if (on[i]) {
           acc[0][i] += g[i] * gate * n;
@@ -373,7 +380,7 @@ int rt_norm_gate_fwd(const float* x, const float* f, const float* z, const float
   const int rc = check(M, d, post_w, post_b, pre_w, pre_b, p);
   if (rc != RT_OK) return rc;
   if (M == 0) return RT_OK;
-  if (x == nullptr || f == nullptr || y == nullptr || (pre_w != nullptr) != (h != nullptr) || ((uintptr_t)stat & 15u) != 0) return RT_ERR_INVALID_ARG;
+  if (!(eps > 0.f) || x == nullptr || f == nullptr || y == nullptr || (pre_w != nullptr) != (h != nullptr) || ((uintptr_t)stat & 15u) != 0) return RT_ERR_INVALID_ARG;
   NgArgs a{};
   a.x = x; a.f = f; a.z = z; a.s = scale; a.pw = post_w; a.pb = post_b; a.nw = pre_w; a.nb = pre_b; a.y = y; a.h = h; a.stat = stat;
   a.M = M; a.d = d; a.post = post_w != nullptr; a.pre = pre_w != nullptr; a.alpha = alpha; a.eps = eps; a.p = p; a.seed = seed; a.stream = stream_id;
@@ -381,7 +388,7 @@ int rt_norm_gate_fwd(const float* x, const float* f, const float* z, const float
   const int vw = vec_of(d, ps, 10);
   const int rpw = rows_per_wg(shape_of(d));
   const long long need = (M + rpw - 1) / rpw;
-  return launch(a, vw, layer != 0, false, (unsigned)(need < 0x7FFFFFFFLL ? need : 0x7FFFFFFFLL), stream);
+  return launch(a, vw, layer != 0, false, (unsigned)(need < (1LL << 20) ? need : 1LL << 20), stream);      // (a launch holds less than 2^32 threads; workgroups loop)
 }
 
 size_t rt_norm_gate_bwd_workspace_bytes(int64_t M, int32_t d) {

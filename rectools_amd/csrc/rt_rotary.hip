@@ -28,61 +28,61 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotArgs a) {
   const int T = a.groups * a.units, half = a.rot / 2, turn_units = (half + V - 1) / V, heads = a.s[0].heads + a.s[1].heads;
   const int in_row = T <= 256 ? (int)threadIdx.x / T : 0;
   if (in_row >= a.rows_per_wg) return;
-  const long long row = (long long)blockIdx.x * a.rows_per_wg + in_row;
-  if (row >= a.M) return;
-  for (int t = T <= 256 ? (int)threadIdx.x % T : (int)threadIdx.x; t < T; t += 256) {
-    const int unit = t % a.units, hg = t / a.units;
-    const bool turns = unit < turn_units;
-    float cs[V], sn[V];
-    const int j0 = unit * V;
-    if (turns) {
-      const double p = (double)a.pos[row];
+  for (long long row = (long long)blockIdx.x * a.rows_per_wg + in_row; row < a.M; row += (long long)gridDim.x * a.rows_per_wg) {
+    for (int t = T <= 256 ? (int)threadIdx.x % T : (int)threadIdx.x; t < T; t += 256) {
+      const int unit = t % a.units, hg = t / a.units;
+      const bool turns = unit < turn_units;
+      float cs[V], sn[V];
+      const int j0 = unit * V;
+      if (turns) {
+        const double p = (double)a.pos[row];
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const double rev = (p * a.freq[min(j0 + e, half - 1)]) * 0.15915494309189533577;      // 1 / (2 pi)
-        float s, c;
-        sincospif(2.f * (float)(rev - rint(rev)), &s, &c);
-        cs[e] = c * a.gain;
-        sn[e] = s * a.gain * a.sign;
-      }
-    }
-    for (int h = hg; h < heads; h += a.groups) {
-      const Seg& s = a.s[h < a.s[0].heads ? 0 : 1];
-      const int hh = h < a.s[0].heads ? h : h - a.s[0].heads;
-      const float* x = s.x + row * s.ldx + (long long)hh * a.hd;
-      float* y = s.y + row * s.ldy + (long long)hh * a.hd;
-      if (!turns) {
-        const int c0 = a.rot + (unit - turn_units) * V;
-        if (V == 4) {
-          *reinterpret_cast<f32x4*>(y + c0) = *reinterpret_cast<const f32x4*>(x + c0);
-        } else {
-          y[c0] = x[c0];
+        for (int e = 0; e < V; ++e) {
+          const double rev = (p * a.freq[min(j0 + e, half - 1)]) * 0.15915494309189533577;      // 1 / (2 pi)
+          float s, c;
+          sincospif(2.f * (float)(rev - rint(rev)), &s, &c);
+          cs[e] = c * a.gain;
+          sn[e] = s * a.gain * a.sign;
         }
-        continue;
       }
-      if (V == 4) {
-        if (INTER) {
-          f32x4 u = *reinterpret_cast<const f32x4*>(x + 2 * j0), v = *reinterpret_cast<const f32x4*>(x + 2 * j0 + 4);
-          *reinterpret_cast<f32x4*>(y + 2 * j0) = f32x4{u[0] * cs[0] - u[1] * sn[0], u[0] * sn[0] + u[1] * cs[0],
-                                                        u[2] * cs[1 % V] - u[3] * sn[1 % V], u[2] * sn[1 % V] + u[3] * cs[1 % V]};
-          *reinterpret_cast<f32x4*>(y + 2 * j0 + 4) = f32x4{v[0] * cs[2 % V] - v[1] * sn[2 % V], v[0] * sn[2 % V] + v[1] * cs[2 % V],
-                                                            v[2] * cs[3 % V] - v[3] * sn[3 % V], v[2] * sn[3 % V] + v[3] * cs[3 % V]};
-        } else {
-          const f32x4 u = *reinterpret_cast<const f32x4*>(x + j0), v = *reinterpret_cast<const f32x4*>(x + half + j0);
-          f32x4 p, q;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            p[e] = u[e] * cs[e % V] - v[e] * sn[e % V];
-            q[e] = u[e] * sn[e % V] + v[e] * cs[e % V];
+      for (int h = hg; h < heads; h += a.groups) {
+        const Seg& s = a.s[h < a.s[0].heads ? 0 : 1];
+        const int hh = h < a.s[0].heads ? h : h - a.s[0].heads;
+        const float* x = s.x + row * s.ldx + (long long)hh * a.hd;
+        float* y = s.y + row * s.ldy + (long long)hh * a.hd;
+        if (!turns) {
+          const int c0 = a.rot + (unit - turn_units) * V;
+          if (V == 4) {
+            *reinterpret_cast<f32x4*>(y + c0) = *reinterpret_cast<const f32x4*>(x + c0);
+          } else {
+            y[c0] = x[c0];
           }
-          *reinterpret_cast<f32x4*>(y + j0) = p;
-          *reinterpret_cast<f32x4*>(y + half + j0) = q;
+          continue;
         }
-      } else {
-        const int ia = INTER ? 2 * j0 : j0, ib = INTER ? 2 * j0 + 1 : half + j0;
-        const float u = x[ia], v = x[ib];
-        y[ia] = u * cs[0] - v * sn[0];
-        y[ib] = u * sn[0] + v * cs[0];
+        if (V == 4) {
+          if (INTER) {
+            f32x4 u = *reinterpret_cast<const f32x4*>(x + 2 * j0), v = *reinterpret_cast<const f32x4*>(x + 2 * j0 + 4);
+            *reinterpret_cast<f32x4*>(y + 2 * j0) = f32x4{u[0] * cs[0] - u[1] * sn[0], u[0] * sn[0] + u[1] * cs[0],
+                                                          u[2] * cs[1 % V] - u[3] * sn[1 % V], u[2] * sn[1 % V] + u[3] * cs[1 % V]};
+            *reinterpret_cast<f32x4*>(y + 2 * j0 + 4) = f32x4{v[0] * cs[2 % V] - v[1] * sn[2 % V], v[0] * sn[2 % V] + v[1] * cs[2 % V],
+                                                              v[2] * cs[3 % V] - v[3] * sn[3 % V], v[2] * sn[3 % V] + v[3] * cs[3 % V]};
+          } else {
+            const f32x4 u = *reinterpret_cast<const f32x4*>(x + j0), v = *reinterpret_cast<const f32x4*>(x + half + j0);
+            f32x4 p, q;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              p[e] = u[e] * cs[e % V] - v[e] * sn[e % V];
+              q[e] = u[e] * sn[e % V] + v[e] * cs[e % V];
+            }
+            *reinterpret_cast<f32x4*>(y + j0) = p;
+            *reinterpret_cast<f32x4*>(y + half + j0) = q;
+          }
+        } else {
+          const int ia = INTER ? 2 * j0 : j0, ib = INTER ? 2 * j0 + 1 : half + j0;
+          const float u = x[ia], v = x[ib];
+          y[ia] = u * cs[0] - v * sn[0];
+          y[ib] = u * sn[0] + v * cs[0];
+        }
       }
     }
   }
@@ -115,8 +115,7 @@ extern "C" int rt_rotary(const float* q, int64_t ldq, float* q_out, int64_t ldq_
   if (T > 0x7FFFFFFF) return RT_ERR_INVALID_ARG;
   a.rows_per_wg = T <= 256 ? (int)(256 / T) : 1;
   const long long blocks = (M + a.rows_per_wg - 1) / a.rows_per_wg;
-  if (blocks > 0x7FFFFFFFLL) return RT_ERR_INVALID_ARG;
-  const unsigned n = (unsigned)blocks;
+  const unsigned n = (unsigned)(blocks < (1LL << 23) ? blocks : 1LL << 23);      // (a launch holds less than 2^32 threads; workgroups loop)
   if (vec) {
     if (interleaved) rotary_kernel<4, true><<<n, 256, 0, stream>>>(a);
     else rotary_kernel<4, false><<<n, 256, 0, stream>>>(a);

@@ -7,8 +7,11 @@
 // (sizes the kernels do not hold), HipLibraryError (not a float32 HIP tensor; a failed launch).
 #include <dlfcn.h>
 
+#include <cmath>
+
 #include <ATen/core/grad_mode.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/extension.h>
 
@@ -127,6 +130,9 @@ Tensor vec(const OptTensor& t, at::IntArrayRef want, const Tensor& first, const 
   check_device(*t, first, what);
   return t->contiguous();
 }
+void check_eps(double eps, const char* what) {      // (as the kernels see it: without it a row of zeros has no norm)
+  if (!((float)eps > 0.f)) bad(what, "eps is positive, got " + std::to_string(eps));
+}
 float* f(const Tensor& t) { return t.defined() ? static_cast<float*>(t.data_ptr()) : nullptr; }
 int64_t* i64(const Tensor& t) { return t.defined() ? static_cast<int64_t*>(t.data_ptr()) : nullptr; }
 rt_stream_t stream_of(const Tensor& t) { return reinterpret_cast<rt_stream_t>(c10::hip::getCurrentHIPStream(t.get_device()).stream()); }
@@ -144,6 +150,24 @@ void once(const char* what) {      // grad mode is on in a backward pass only un
   TORCH_CHECK(!at::GradMode::is_enabled(), what, " has no second derivative (create_graph=True)");
 }
 
+// Leaves whose gradient node was made on the default stream (by a graph that lives outside a capture, or by this call on that stream): the engine
+// hands their gradients over on that stream, which no capture can follow; the process would end there.  Noted in the forward pass, refused when
+// the backward pass runs under a capture.
+bool default_stream_leaves(std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts) {
+    if (!t->defined() || !t->is_leaf() || !t->requires_grad()) continue;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+    if (!node) continue;
+    const auto s = node->stream();
+    if (s.has_value() && s->id() == 0) return true;
+  }
+  return false;
+}
+void capturable(AutogradContext* ctx, const char* what) {
+  if (ctx->saved_data["leaves"].toBool() && c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None)
+    TORCH_CHECK(false, what, ": a backward pass cannot be captured while a graph made on the default stream holds the same leaf tensors; drop that graph first");
+}
+
 // ---- rotary -----------------------------------------------------------------------------------------------------------------------------
 struct RotaryMeta { int64_t n_heads, n_kv_heads, hd; bool interleaved; double gain; };
 void rotary_call(const Tensor& q, const Tensor& k, const Tensor& q2, const Tensor& k2, const Tensor& pos, const Tensor& freq, const RotaryMeta& m, bool backward) {
@@ -159,6 +183,7 @@ struct RotaryNode : torch::autograd::Function<RotaryNode> {
   static variable_list forward(AutogradContext* ctx, const Tensor& q, const OptTensor& k_opt, const Tensor& pos, const Tensor& freq, int64_t n_heads, int64_t n_kv_heads,
                                int64_t hd, bool interleaved, double gain) {
     const Tensor k = got(k_opt);
+    ctx->saved_data["leaves"] = default_stream_leaves({&q, &k});
     ctx->save_for_backward({pos, freq});
     ctx->saved_data["m"] = std::vector<int64_t>{n_heads, n_kv_heads, hd, interleaved};
     ctx->saved_data["g"] = gain;
@@ -170,6 +195,7 @@ struct RotaryNode : torch::autograd::Function<RotaryNode> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     once("rotary");
+    capturable(ctx, "rotary");
     variable_list out(9);
     Tensor gq = g[0].defined() ? dense_rows(g[0]) : Tensor(), gk = g.size() > 1 && g[1].defined() ? dense_rows(g[1]) : Tensor();
     if (!gq.defined() && !gk.defined()) return out;
@@ -220,11 +246,13 @@ Tensor lambda_call(const Tensor& q1, const Tensor& k1, const Tensor& q2, const T
 }
 struct LambdaNode : torch::autograd::Function<LambdaNode> {
   static Tensor forward(AutogradContext* ctx, const Tensor& q1, const Tensor& k1, const Tensor& q2, const Tensor& k2, double init) {
+    ctx->saved_data["leaves"] = default_stream_leaves({&q1, &k1, &q2, &k2});
     ctx->save_for_backward({q1, k1, q2, k2});
     return lambda_call(q1, k1, q2, k2, init);
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     once("diff_lambda");
+    capturable(ctx, "diff_lambda");
     const auto s = ctx->get_saved_variables();
     c10::DeviceGuard guard(s[0].device());
     variable_list out{like(s[0]), like(s[0]), like(s[0]), like(s[0]), Tensor()};
@@ -269,6 +297,7 @@ struct AttentionNode : torch::autograd::Function<AttentionNode> {
     const Tensor w = got(w_opt), cu_q = got(cu_q_opt), cu_k = got(cu_k_opt), ids = got(ids_opt);
     Tensor saved;
     const Tensor y = attention_call(q, k, v, lam, cu_q, cu_k, ids, w, m, &saved);
+    ctx->saved_data["leaves"] = default_stream_leaves({&q, &k, &v, &lam, &w});
     ctx->save_for_backward({lam, w, cu_q, cu_k, ids, saved});      // (not q, k, v: their planes are in `saved`)
     sizes.push_back(q.size(0));
     sizes.push_back(k.size(0));
@@ -278,6 +307,7 @@ struct AttentionNode : torch::autograd::Function<AttentionNode> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     once("diff_attention");
+    capturable(ctx, "diff_attention");
     const auto s = ctx->get_saved_variables();
     const Tensor &lam = s[0], &w = s[1], &saved = s[5];
     const auto z = ctx->saved_data["s"].toIntVector();
@@ -319,7 +349,8 @@ Tensor diff_attention(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in
   if (!cu_k_in.has_value() && k.size(0) != B * Lk) bad(what, std::to_string(k.size(0)) + " key rows for " + std::to_string(B) + " sessions of " + std::to_string(Lk));
   const Tensor cu_q = ints(cu_q_in, B + 1, q, "diff_attention cu_q"), cu_k = ints(cu_k_in, B + 1, q, "diff_attention cu_k"),
                ids = ints(ids_in, k.size(0), q, "diff_attention key_ids"), lam = vec(lam_in, {H}, q, "diff_attention lam"), w = vec(w_in, {2 * hd}, q, "diff_attention norm_w");
-  if (scale.has_value() && !(*scale > 0.0)) bad(what, "the logit scale is positive, got " + std::to_string(*scale));
+  if (scale.has_value() && !((float)*scale > 0.f && std::isfinite((float)*scale))) bad(what, "the logit scale is positive, got " + std::to_string(*scale));
+  if (w.defined()) check_eps(eps, what);
   const AttnMeta m{B, H, Hkv, hd, Lq, Lk, causal, scale.value_or(0.0), out_scale, eps};
   if (on_tape({&q, &k, &v, &lam, &w}))
     return AttentionNode::apply(q, k, v, lam, opt(w), opt(cu_q), opt(cu_k), opt(ids), std::vector<int64_t>{B, H, Hkv, hd, Lq, Lk, causal}, m.scale, out_scale, eps);
@@ -345,6 +376,7 @@ struct NormNode : torch::autograd::Function<NormNode> {
     const Tensor z = got(z_opt), sc = got(sc_opt), pw = got(pw_opt), pb = got(pb_opt), nw = got(nw_opt), nb = got(nb_opt);
     Tensor stat;
     variable_list out = norm_call(x, b, z, sc, pw, pb, nw, nb, {layer, alpha, eps, p, (uint64_t)seed, (uint64_t)sid}, &stat);
+    ctx->saved_data["leaves"] = default_stream_leaves({&x, &b, &z, &sc, &pw, &pb, &nw, &nb});
     ctx->save_for_backward({nw.defined() ? out[0] : Tensor(), b, z, sc, pw, pb, nw, stat});
     ctx->saved_data["i"] = std::vector<int64_t>{layer, seed, sid, nb.defined()};
     ctx->saved_data["f"] = std::vector<double>{alpha, p};
@@ -353,6 +385,7 @@ struct NormNode : torch::autograd::Function<NormNode> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     once("norm_gate_residual");
+    capturable(ctx, "norm_gate_residual");
     variable_list out(14);
     Tensor gy = g[0].defined() ? g[0].contiguous() : Tensor(), gh = g.size() > 1 && g[1].defined() ? g[1].contiguous() : Tensor();
     if (!gy.defined() && !gh.defined()) return out;
@@ -387,6 +420,7 @@ std::vector<Tensor> norm_gate(const Tensor& x_in, const Tensor& f_in, const OptT
   if (d > 8192) raise(PyExc_NotImplementedError, "norm_gate_residual: rows of at most 8,192 columns, got " + std::to_string(d));
   const Tensor x = x_in.contiguous(), b = vec(f_in, x_in.sizes(), x_in, what), z = vec(z_in, x_in.sizes(), x_in, what), sc = vec(sc_in, {d}, x_in, what),
                pw = vec(pw_in, {d}, x_in, what), pb = vec(pb_in, {d}, x_in, what), nw = vec(nw_in, {d}, x_in, what), nb = vec(nb_in, {d}, x_in, what);
+  check_eps(eps, what);
   if (on_tape({&x, &b, &z, &sc, &pw, &pb, &nw, &nb})) return NormNode::apply(x, b, opt(z), opt(sc), opt(pw), opt(pb), opt(nw), opt(nb), layer, alpha, eps, p, (int64_t)seed, (int64_t)sid);
   return norm_call(x, b, z, sc, pw, pb, nw, nb, {layer, alpha, eps, p, seed, sid}, nullptr);
 }

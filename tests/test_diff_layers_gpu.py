@@ -199,6 +199,31 @@ def test_operators_captured_and_replayed_beside_eager_work():
         assert torch.equal(one1, newest(*one)) and torch.equal(one2, newest(*other))
 
 
+def test_captured_backward_beside_an_eager_graph_of_the_same_leaves():
+    """That graph's gradient nodes belong to the default stream, which no capture can follow: refused; without it the capture works."""
+    from rectools_amd import ops
+
+    w = torch.rand(64, device="cuda").add_(0.5).requires_grad_()
+    x = torch.randn(8, 64, device="cuda")
+
+    def step():
+        return torch.autograd.grad(ops.norm_gate_residual(x, x, post=(w, None))[0], w, x)[0]
+
+    want = step()
+    alive = ops.norm_gate_residual(x, x, post=(w, None))[0]
+    with pytest.raises(RuntimeError, match="same leaf tensors"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            step()
+    assert torch.equal(torch.autograd.grad(alive, w, x)[0], want)
+    del alive
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step()
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+
+
 def test_operators_on_another_stream():
     from rectools_amd import ops
 

@@ -2,9 +2,11 @@
 (CPU), at the sizes, layouts and masks where they can go wrong.
 
 Tolerances.  u = 2^-24 is half a step of fp32.  A sum of n products carries at most (n + 1) u of the sum of its terms' magnitudes, whatever
-its order; the split products (six of nine terms) add at most 3 u of a product.  The references below return, next to every result, its
-MAGNITUDE: the same formula over absolute values.  A result may then be off by k * magnitude, with k counted from the lengths of the sums
-that lead to it (`_kappa`)."""
+its order.  A split product x y ~ h h' + h l' + l h' adds: x against h + l — h rounds x, at least 2^k, by 2^(k - 11) at most, l rounds that by 2^(k - 23)
+at most: 2 u of x; the same for y; the dropped l l': 2^-11 of x times 2^-11 of y: 4 u — 8 u of the product, and its sum has three terms
+for one.  (Values below 2^-17 of their row's largest carry 2^-38 of that instead: nothing here.)  The references below return, next to every
+result, its MAGNITUDE: the same formula over absolute values.  A result may then be off by k * magnitude, with k counted from the lengths of the
+sums that lead to it (`_kappa`)."""
 import math
 
 import pytest
@@ -192,11 +194,12 @@ def _attention_ref(q, k, v, lam, lens_q, lens_k, H, Hkv, causal, ids, w, c, eps,
 
 
 def _kappa(hd, n, top, rho):
-    """A logit of magnitude `top` is off by d = (hd + 6) u top (its sum, the split, the scale), a probability by 2 d + 8 u relative (the exponential, its
-    argument's rounding against the maximum, the row sum's n u counted below), products over n keys add (n + 8) u; a gradient passes the probability twice
-    and its own sums (2 hd + n); the statistics of the norm amplify what o is off by through rho (counted in the magnitudes of o, once more here)."""
-    d = (hd + 6) * U * top
-    return (2 * d + 8 * U) * 2 + (2 * n + 4 * hd + 32) * U * (1.0 + 0.25 * rho)
+    """A logit of magnitude `top` is off by d = (3 hd + 12) u top (its sum of 3 hd terms, the split, the scales), a probability by 2 d + 8 u relative (the
+    exponential, its argument's rounding against the maximum); products over n keys add (3 n + 9) u and the row sum n u; a gradient passes the
+    probability twice and its own sums (3 * 2 hd and 2 hd of delta); the statistics of the norm amplify what o is off by through rho (counted in the
+    magnitudes of o, once more here)."""
+    d = (3 * hd + 12) * U * top
+    return (2 * d + 8 * U) * 2 + (4 * n + 8 * hd + 32) * U * (1.0 + 0.25 * rho)
 
 
 def _cu(lens):
@@ -204,11 +207,13 @@ def _cu(lens):
 
 
 def _attention_case(lens_q, lens_k, H, Hkv, hd, causal, ids=None, w=True, packed_q=True, packed_k=True, train=True, seed=0, tail=0, spread=1.0, Lq=None,
-                    Lk=None, scale=None):
+                    Lk=None, scale=None, sizes=None):
     ops, dev = _ops(), _dev()
     g = torch.Generator().manual_seed(seed + hd * 7 + H)
     B, Nq, Nk = len(lens_q), sum(lens_q), sum(lens_k)
     q, k, v = (torch.randn(n, c * 2 * hd, generator=g) * s for n, c, s in ((Nq, H, spread), (Nk, Hkv, 1.0), (Nk, Hkv, 1.0)))
+    if sizes is not None:      # every row times a size of its own
+        q, k, v = (t * f[:, None].float() for t, f in zip((q, k, v), sizes(g, Nq, Nk)))
     lam, wt = torch.rand(H, generator=g) * 0.8 + 0.1, (1.0 + 0.1 * torch.randn(2 * hd, generator=g)) if w else None
     gy = torch.randn(Nq, H * 2 * hd, generator=g)
     c, eps = 0.64, 1e-5
@@ -335,6 +340,54 @@ def test_attention_flat_and_sharp_maps(spread):
     _attention_case([65, 130], [65, 130], 2, 2, 32, True, spread=spread)
 
 
+@pytest.mark.parametrize("lens_q,H,Hkv", [([9, 12], 1, 1), ([5, 3], 4, 2), ([4, 1], 3, 1), ([2, 2], 5, 1), ([2, 1], 6, 1), ([1, 1], 8, 1), ([1, 1], 9, 1), ([13], 1, 1)])
+@pytest.mark.parametrize("hd", [32, 50])
+def test_attention_few_queries_in_one_and_two_passes(lens_q, H, Hkv, hd):
+    lens_k = [900 + 70 * i for i in range(len(lens_q))]
+    _attention_case(lens_q, lens_k, H, Hkv, hd, True, train=False)
+    ids = torch.ones(sum(lens_k), dtype=torch.int64)
+    ids[5::3] = 0
+    ids[:880] = 0
+    _attention_case(lens_q, lens_k, H, Hkv, hd, True, train=False, ids=ids)
+
+
+@pytest.mark.parametrize("train", [True, False])
+@pytest.mark.parametrize("rows", [1, 80])
+def test_attention_rows_of_very_different_sizes(train, rows):
+    """Sessions of huge queries and tiny keys, and the other way round, values from 1e-10 to 1e10 next to each other: nothing leaves the range."""
+    def sizes(g, nq, nk):
+        a = torch.tensor([12.0, -12.0, 3.0]).double()
+        at_q, at_k = torch.arange(nq) * 3 // nq, torch.arange(nk) * 3 // nk
+        return (10.0 ** (a[at_q] - 4.0 * torch.rand(nq, generator=g)), 10.0 ** (-a[at_k] - 2.0 * torch.rand(nk, generator=g)), 10.0 ** (20.0 * torch.rand(nk, generator=g) - 10.0))
+    _attention_case([rows] * 3, [80] * 3, 2, 1, 32, True, w=False, train=train, sizes=sizes)
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_attention_sessions_do_not_see_their_neighbours(rows):
+    """A session of NaN between two others, in the same chunk of keys: their rows and gradients keep their bits."""
+    ops, dev = _ops(), _dev()
+    g = torch.Generator().manual_seed(21)
+    H, hd, lens = 2, 32, [45, 20, 50]
+    cu_q, cu_k = _cu([min(rows, n) for n in lens]).to(dev), _cu(lens).to(dev)
+    nq, a, b = int(cu_q[-1]), int(cu_q[1]), int(cu_q[2])
+    q, k, v, gy = (torch.randn(n, H * 2 * hd, generator=g).to(dev) for n in (nq, 115, 115, nq))
+    lam = torch.full((H,), 0.4, device=dev)
+    res = []
+    for bad in (False, True):
+        ts = [t.clone() for t in (q, k, v)]
+        if bad:
+            ts[0][a:b], ts[1][45:65], ts[2][45:65] = math.nan, math.inf, math.nan
+        with torch.no_grad():
+            y0 = ops.diff_attention(*ts, lam, cu_q, cu_k, 3, H, H, max(1, rows), 50, True)
+        for t in ts:
+            t.requires_grad_()
+        y = ops.diff_attention(*ts, lam, cu_q, cu_k, 3, H, H, rows, 50, True)
+        res.append([y0, y.detach(), *torch.autograd.grad(y, ts, gy)])
+    for i, (x, z) in enumerate(zip(*res)):
+        lo, hi = (a, b) if x.shape[0] == nq and i != 3 and i != 4 else (45, 65)
+        assert torch.equal(x[:lo], z[:lo]) and torch.equal(x[hi:], z[hi:]), i
+
+
 @pytest.mark.parametrize("train", [True, False])
 def test_attention_without_norm_and_own_scale(train):
     _attention_case([65, 13], [65, 13], 2, 1, 40, True, w=False, train=train)
@@ -361,6 +414,10 @@ def test_attention_column_blocks_and_empty_calls():
     e = torch.zeros(0, c, device=dev)
     z = torch.zeros(1, dtype=torch.int64, device=dev)
     assert ops.diff_attention(e, e, e, lam, z, z, 0, H, H, 0, 0, True).shape == (0, c)
+    for train in (False, True):      # no sessions: every row is behind the last one
+        r = torch.randn(5, c, generator=g).to(dev).requires_grad_(train)
+        y = ops.diff_attention(r, r, r, lam, z, z, 0, H, H, 0, 0, True)
+        assert not y.any() and (not train or not torch.autograd.grad(y.sum(), r)[0].any())
     e2 = torch.zeros(0, c, device=dev, requires_grad=True)
     y = ops.diff_attention(e2, e2, e2, lam, z, z, 0, H, H, 0, 0, True)
     (d,) = torch.autograd.grad(y.sum(), e2)
@@ -385,7 +442,10 @@ def test_attention_same_bits_twice_and_gradient_against_differences():
         return ops.diff_attention(*ts[:4], cu, cu, 2, H, Hkv, 90, 90, True, norm_w=ts[4], out_scale=0.5)
 
     first = torch.autograd.grad(run(*leaves), leaves, gy)
-    again = torch.autograd.grad(run(*leaves), leaves, gy)
+    y = run(*leaves)
+    again = torch.autograd.grad(y, leaves, gy, retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(first, again))
+    again = torch.autograd.grad(y, leaves, gy)      # the same graph's second pass
     assert all(torch.equal(a, b) for a, b in zip(first, again))
     for i, t in enumerate(leaves):      # a random direction: central differences of sum(gy * y); h^2 terms ~1e-4, rounding of y ~ 1e-6 / h
         d = torch.randn(t.shape, generator=g).to(dev)
@@ -430,7 +490,7 @@ def test_attention_refusals():
     ops.diff_attention(**ok)
     for bad in (dict(B=2), dict(H=3), dict(H_kv=1), dict(H=4, H_kv=3), dict(lam=lam[:1]), dict(cu_q=cu.int()), dict(cu_q=cu.cpu()), dict(cu_k=None, Lk=5),
                 dict(cu_q=None, Lq=7), dict(k=q[:5]), dict(v=q[:, :32]), dict(q=q[0]), dict(key_ids=cu), dict(norm_w=torch.ones(16, device=dev)),
-                dict(scale=0.0), dict(scale=-1.0), dict(Lq=-1)):
+                dict(scale=0.0), dict(scale=-1.0), dict(scale=1e-60), dict(scale=math.inf), dict(norm_w=torch.ones(32, device=dev), eps=0.0), dict(Lq=-1)):
         with pytest.raises(ValueError):
             ops.diff_attention(**{**ok, **bad})
     wide = torch.randn(6, 2 * 2 * 65, device=dev)
@@ -439,6 +499,76 @@ def test_attention_refusals():
     for bad in (dict(q=q.double()), dict(q=q.cpu()), dict(lam=lam.half())):
         with pytest.raises(HipLibraryError):
             ops.diff_attention(**{**ok, **bad})
+
+
+def _room(gib):
+    if torch.cuda.mem_get_info()[0] < gib * 2 ** 30:
+        pytest.skip(f"needs {gib} GiB")
+
+
+@pytest.mark.parametrize("rows", [1, 20])
+def test_offsets_beyond_32_bits(rows):
+    """Keys, values and rotated columns as blocks of rows 160 kB apart: more than 2^31 elements from the first to the last."""
+    _room(32)
+    ops, dev = _ops(), _dev()
+    n, ld, c = 60_001, 40_000, 64
+    wide = torch.empty(n, ld, device=dev)
+    blocks = [wide[:, i:i + c] for i in (0, 20_000, ld - c)]
+    dense = [torch.randn(n, c, device=dev) for _ in blocks]
+    for b, t in zip(blocks, dense):
+        b.copy_(t)
+    assert wide.stride(0) * (n - 1) > 2 ** 31
+    q, lam = torch.randn(rows, c, device=dev), torch.full((1,), 0.3, device=dev)
+    ask = lambda k, v: ops.diff_attention(q, k, v, lam, None, None, 1, 1, 1, rows, n, True)      # noqa: E731
+    assert torch.equal(ask(*blocks[:2]), ask(*dense[:2]))
+    freq, _ = ops.rotary_frequencies(32, device=dev)
+    pos = torch.arange(n, device=dev)
+    assert torch.equal(ops.rotary(blocks[2], pos, freq, 1), ops.rotary(dense[2], pos, freq, 1))
+
+
+def test_large_outputs():
+    """More than 2^31 elements in and out: the last rows are those of a small call."""
+    _room(80)
+    ops, dev = _ops(), _dev()
+    x = torch.zeros(270_000, 8192, device=dev)
+    x[-3:] = torch.randn(3, 8192, device=dev)
+    w = torch.rand(8192, device=dev)
+
+    def run(t):
+        t = t.detach().requires_grad_()
+        y, h = ops.norm_gate_residual(t, t, post=(w, None), pre=(w, None))
+        return (y[-3:].detach(), h[-3:].detach(), torch.autograd.grad(h, t, h.detach())[0][-3:])
+
+    assert all(torch.equal(a, b) for a, b in zip(run(x), run(x[-3:].clone())))
+    x = x.view(-1, 1280)
+    freq, _ = ops.rotary_frequencies(64, device=dev)
+    pos = torch.arange(x.shape[0], device=dev)
+    assert torch.equal(ops.rotary(x, pos, freq, 20)[-19:], ops.rotary(x[-19:].clone(), pos[-19:], freq, 20))
+
+
+def test_broadcast_inputs_and_their_gradients():
+    ops, dev = _ops(), _dev()
+    g = torch.Generator().manual_seed(8)
+    n, H, hd = 40, 2, 32
+    c = H * 2 * hd
+    row, lam1, gy = torch.randn(1, c, generator=g).to(dev), torch.tensor([0.4], device=dev), torch.randn(n, c, generator=g).to(dev)
+    k = torch.randn(n, c, generator=g).to(dev)
+    freq, _ = ops.rotary_frequencies(16, device=dev)
+    w = torch.rand(c, generator=g).to(dev) + 0.5
+    pos = torch.arange(n, device=dev)
+
+    def run(r, l1, wide):
+        x, lam = (r.expand(n, c), l1.expand(H)) if wide else (r, l1)
+        y = ops.diff_attention(ops.rotary(x, pos, freq, 2 * H), k, x, lam, None, None, 1, H, H, n, n, True)
+        z, h = ops.norm_gate_residual(x, y, gate=x, post=(w, None), pre=(w, None))
+        return (z.detach(), h.detach()) + torch.autograd.grad((z, h), (r, l1), (gy, gy[:1].expand(n, c)))
+
+    a = run(row.clone().requires_grad_(), lam1.clone().requires_grad_(), True)
+    b = run(row.repeat(n, 1).requires_grad_(), lam1.repeat(H).requires_grad_(), False)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    for got, each in zip(a[2:], b[2:]):      # the sum over the copies: n terms
+        each = each.cpu().double().reshape(-1, got.shape[-1])
+        _close(got.reshape(1, -1), each.sum(0, keepdim=True), each.abs().sum(0, keepdim=True), (each.shape[0] + 1) * U, "broadcast")
 
 
 # ---- norms, gate, residual scale ---------------------------------------------------------------------------------------------------------
@@ -562,6 +692,21 @@ def test_norm_constant_and_zero_rows():
     assert all(torch.isfinite(t).all() for t in grads)
     y, h = ops.norm_gate_residual(x, torch.zeros_like(f), post=(w, None), pre=(w, None), kind="rms")
     assert not y.any() and not h.any()
+
+
+def test_norm_gate_far_from_zero():
+    """The gate's slope sigmoid(z) sigmoid(-z) keeps its relative precision where 1 - sigmoid(z) would have none left, and is zero or finite behind that."""
+    ops, dev = _ops(), _dev()
+    z = torch.tensor([[0.0, 5.0, -5.0, 12.0, -12.0, 17.0, 40.0, -40.0, 80.0, -80.0, 200.0, -200.0]])
+    x = torch.ones_like(z)
+    zd = z.to(dev).requires_grad_()
+    y, _ = ops.norm_gate_residual(x.to(dev), x.to(dev), gate=zd)
+    (dz,) = torch.autograd.grad(y.sum(), zd)
+    want = torch.sigmoid(z.double()) * torch.sigmoid(-z.double())
+    # e^-|z|: its argument is exact, the function 2 u; the sum, the quotient, three products: u each
+    assert ((dz.cpu().double() - want).abs() <= 12 * U * want + 1e-37).all(), dz
+    want = 1.0 + torch.sigmoid(z.double())
+    assert ((y.detach().cpu().double() - want).abs() <= 8 * U * want).all()
 
 
 @pytest.mark.parametrize("d", [48, 50, 33])
