@@ -54,14 +54,13 @@ struct Args {
   unsigned char* qp; unsigned char* kp; unsigned char* vp; unsigned char* dp;
   float* qs; float* ks;                  // [H][2][Nq + PAD], [Hkv][2][Nk + PAD]
   float* vs; float* ivs; float* lvb;     // [Hkv][Nk + PAD]: 2^e, 2^-e, e (minus infinity: the key is masked)
-  float* ds;                             // [H][Nq + PAD]
   float* o12;                            // [Nq, H, 2, 2 hd] normalised outputs of the two maps (training)
   float* lse; float* lsf;                // [H][2][Nq + PAD] of the two maps (training): probability = exp2(s - lse) lsf, lse a whole number
   float* part; float* ml;                // split keys: [n_split, Nq, H, 2, 2 hd] and [n_split, Nq, H, 2, 2] (maximum, sum)
   int n_split;
   Grid own_q, own_k;                     // launches whose owner rows are queries / keys
   // backward
-  float* delta;                          // [H][2][Nq + PAD]
+  float* delta; float* dc;               // [H][2][Nq + PAD]: do . o_m 2^-e, e of dO's row; what turns exp2(s - lse) into the map's weight on dO's plane
   float* dq; float* dk; float* dv; long long lddq, lddk, lddv; int vec_q, vec_kv;
   int vec_y;
 };
@@ -185,6 +184,8 @@ __global__ __launch_bounds__(NT) void diff_planes_kernel(Args a, unsigned q_bloc
   if (c4 % (HD / 4) == 0) (what == 0 ? a.qs : a.ks)[(2 * h + mp) * (N + PAD) + row] = pow2(e);
 }
 
+__device__ __forceinline__ int wave_of(int tid) { return __builtin_amdgcn_readfirstlane(tid >> 6); }      // known to be the same in all lanes: scalar branches
+
 // ---- staging -----------------------------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ unsigned lds_addr(const void* p) { return (unsigned)(unsigned long long)(RT_LDS const void*)p; }
 __device__ __forceinline__ void dma16(const void* src, unsigned dst) {      // lane i: 16 bytes to dst + 16 i
@@ -292,20 +293,21 @@ __device__ __forceinline__ void cols_dot(const unsigned char* img, int c0, int p
   }
   __builtin_amdgcn_s_setprio(0);
 }
-__device__ __forceinline__ void split16(const float (&x)[16], P2 (&out)[2]) {
+// x factor as two halves; h and the rest of it leave one mixed-precision multiply-add each
+__device__ __forceinline__ void split16(const float (&x)[16], float factor, P2 (&out)[2]) {
 #pragma unroll
   for (int t = 0; t < 2; ++t)
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const float v = x[8 * t + j];
-      out[t].h[j] = (_Float16)v;
-      out[t].l[j] = (_Float16)(v - (float)out[t].h[j]);
+      out[t].h[j] = (_Float16)fmaf(v, factor, 0.f);
+      out[t].l[j] = (_Float16)fmaf(v, factor, -(float)out[t].h[j]);
     }
 }
 // The same for weights of unknown size (dS; the difference map times dO's scales): the lane's unit follows the largest magnitude it has met, as
 // the running maximum of a softmax does; when it grows, the lane's accumulators are rescaled (powers of two: exact).
 template <int NB>
-__device__ __forceinline__ void split16_scaled(float (&x)[16], float& inv, f32x16 (&acc)[NB], P2 (&out)[2]) {
+__device__ __forceinline__ void split16_scaled(const float (&x)[16], float& inv, f32x16 (&acc)[NB], P2 (&out)[2]) {
   float top = 0.f;
 #pragma unroll
   for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(x[r]));
@@ -318,9 +320,7 @@ __device__ __forceinline__ void split16_scaled(float (&x)[16], float& inv, f32x1
     for (int cb = 0; cb < NB; ++cb) acc[cb] *= ratio;
     inv = now;
   }
-#pragma unroll
-  for (int r = 0; r < 16; ++r) x[r] *= inv;
-  split16(x, out);
+  split16(x, inv, out);
 }
 constexpr float NO_UNIT = 0x1p126f;      // before the first weight
 
@@ -378,7 +378,7 @@ __global__ __launch_bounds__(NT, HD == 32 ? 3 : 2) void diff_fwd_kernel(Args a) 
   constexpr int DV = 2 * HD, NS = HD / 16, NB = DV / 32, STAGE = fwd_stage<HD>(), STAGES = fwd_stages<HD>();
   constexpr float UP = 14.f;      // weights come to 2^14 at most
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, mp = wave & 1, rg = wave >> 1, i = lane & 31, g = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, wave = wave_of(tid), mp = wave & 1, rg = wave >> 1, i = lane & 31, g = lane >> 5;
   const Work wk = work_of(a, a.own_q, blockIdx.x, a.H, a.causal != 0);
   if (!wk.any) return;
   const int h = wk.h, hk = h / (a.H / a.Hkv), dv = 2 * a.hd;
@@ -486,7 +486,9 @@ __global__ __launch_bounds__(NT, HD == 32 ? 3 : 2) void diff_fwd_kernel(Args a) 
       }
       lsum += ps;
       P2 Pp[2];
-      split16(x, Pp);
+      float one = 1.f;      // (opaque: or the multiply-adds become conversions and differences, four instructions for two)
+      asm("" : "+s"(one));
+      split16(x, one, Pp);
       cols_dot<HD, NB>(img + Row<HD>::CHUNK, 0, 4 * HD, Pp, lane, O);
     }
     const float l = lsum + __shfl_xor(lsum, 32, 64);
@@ -650,9 +652,11 @@ __global__ __launch_bounds__(NT) void diff_bwd_pre_kernel(Args a, const float* d
     const float s1 = group_sum<LANES>(d[0] * o1[0] + d[1] * o1[1] + d[2] * o1[2] + d[3] * o1[3]);
     const float s2 = group_sum<LANES>(d[0] * o2[0] + d[1] * o2[1] + d[2] * o2[2] + d[3] * o2[3]);
     if (c == 0) {
-      a.ds[h * NqP + row] = pow2(ex);
-      a.delta[2 * h * NqP + row] = s1;
-      a.delta[(2 * h + 1) * NqP + row] = s2;
+      const long long m1 = 2 * h * NqP + row, m2 = m1 + NqP;
+      a.delta[m1] = __builtin_amdgcn_ldexpf(s1, -ex);
+      a.delta[m2] = __builtin_amdgcn_ldexpf(s2, -ex);
+      a.dc[m1] = a.lsf[m1] * pow2(ex);
+      a.dc[m2] = a.lsf[m2] * -lam * pow2(ex);
     }
     dl -= (double)s2;
   }
@@ -688,14 +692,14 @@ __global__ __launch_bounds__(64) void diff_bwd_sums_kernel(const double* part, i
 // ---- backward, dQ: the owner is a query; both maps need G^T = V dO^T, each wave makes it over half of V's columns and they swap halves ------
 // STAGES: two where two workgroups with two chunk buffers fit a CU's LDS (HD 32), else one: the other workgroup's products run under the copy.
 template <int HD> constexpr int bwd_stages() { return HD == 32 ? 2 : 1; }
-template <int HD> constexpr int dkv_stage() { return 2 * Row<HD>::CHUNK + 1280; }
+template <int HD> constexpr int dkv_stage() { return 2 * Row<HD>::CHUNK + 1024; }
 template <int HD> constexpr int bwd_lds() { return bwd_stages<HD>() * dkv_stage<HD>() + 4 * 8 * 64 * 16; }      // (dQ needs less)
 
 template <int HD>
 __device__ __forceinline__ void bwd_dq(const Args& a, unsigned char* smem, int blk) {
   constexpr int NS = HD / 16, NB = HD / 32, STAGE = fwd_stage<HD>(), STAGES = bwd_stages<HD>();
   f32x4* swap = reinterpret_cast<f32x4*>(smem + STAGES * STAGE);      // [wave][4][64]
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, mp = wave & 1, rg = wave >> 1, i = lane & 31, g = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, wave = wave_of(tid), mp = wave & 1, rg = wave >> 1, i = lane & 31, g = lane >> 5;
   const Work wk = work_of(a, a.own_q, blk, a.H, a.causal != 0);
   if (!wk.any) return;
   const int h = wk.h, hk = h / (a.H / a.Hkv), hd = a.hd, dv = 2 * hd;
@@ -709,7 +713,6 @@ __device__ __forceinline__ void bwd_dq(const Args& a, unsigned char* smem, int b
   rows_of(a.cu_q, wk.b, a.Lq, a.Nq, qr0, nq);
   rows_of(a.cu_k, wk.b, a.Lk, a.Nk, kr0, nk);
   const int off = nk - nq;
-  const float sign = mp == 0 ? 1.f : -a.lam[h];
   const unsigned lds0 = lds_addr(smem);
   const long long krow = hk * NkP + kr0;
   auto issue = [&](int c, int st) {
@@ -729,8 +732,8 @@ __device__ __forceinline__ void bwd_dq(const Args& a, unsigned char* smem, int b
     P2 Qp[NS], Dp[NS];      // dO: columns mp * HD .. of the padded 2 HD
     load_own<NS>(a.qp + (h * NqP + qrow) * Row<HD>::BYTES + mp * 4 * HD, 0, 2 * HD, g, Qp);
     load_own<NS>(a.dp + (h * NqP + qrow) * Row<HD>::BYTES, mp * HD, 4 * HD, g, Dp);
-    const float qsc = a.qs[(2 * h + mp) * NqP + qrow] * (a.scale * LOG2E), dsc = a.ds[h * NqP + qrow];
-    const float lse = a.lse[(2 * h + mp) * NqP + qrow], lsf = a.lsf[(2 * h + mp) * NqP + qrow], dl = a.delta[(2 * h + mp) * NqP + qrow];
+    const long long at = (2 * h + mp) * NqP + qrow;
+    const float qsc = a.qs[at] * (a.scale * LOG2E), lse = a.lse[at], dl = a.delta[at], dc = a.dc[at];
     f32x16 dQ[NB];
 #pragma unroll
     for (int cb = 0; cb < NB; ++cb) dQ[cb] = zero16();
@@ -775,10 +778,12 @@ __device__ __forceinline__ void bwd_dq(const Args& a, unsigned char* smem, int b
         const f32x4 k4 = *reinterpret_cast<const f32x4*>(sc + 32 * mp + 8 * r + 4 * g), v4 = *reinterpret_cast<const f32x4*>(sc + 96 + 8 * r + 4 * g);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          float p = __builtin_amdgcn_exp2f(fmaf(S[4 * r + e] * k4[e], qsc, -lse));
-          if (edge) p = reg_row(4 * r + e, g) <= last ? p : 0.f;
-          x[4 * r + e] = p * fmaf((G[4 * r + e] + other[e]) * v4[e], dsc, -dl) * k4[e];
+          x[4 * r + e] = __builtin_amdgcn_exp2f(fmaf(S[4 * r + e] * k4[e], qsc, -lse)) * fmaf(G[4 * r + e] + other[e], v4[e], -dl) * k4[e];
         }
+      }
+      if (edge) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x[r] = reg_row(r, g) <= last ? x[r] : 0.f;
       }
       if (a.key_ids != nullptr) {
 #pragma unroll
@@ -795,7 +800,7 @@ __device__ __forceinline__ void bwd_dq(const Args& a, unsigned char* smem, int b
     if (qok) {
       const int n = fresh(hd), vec = fresh(a.vec_q);
       float* o = a.dq + (qr0 + qi) * a.lddq + (long long)(2 * h + mp) * n;
-      const float f = a.scale * sign * lsf / unit;      // (lsf belongs to the row: it waits until here)
+      const float f = a.scale * dc / unit;      // (the row's own factors wait until here)
 #pragma unroll
       for (int cb = 0; cb < NB; ++cb)
 #pragma unroll
@@ -811,7 +816,7 @@ template <int HD>
 __device__ __forceinline__ void bwd_dkv(const Args& a, unsigned char* smem, int blk) {
   constexpr int NS = HD / 16, NB = HD / 32, STAGE = dkv_stage<HD>(), STAGES = bwd_stages<HD>();
   f32x4* swap = reinterpret_cast<f32x4*>(smem + STAGES * STAGE);      // [wave][8][64]: G halves, probabilities
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, mp = wave & 1, rg = wave >> 1, i = lane & 31, g = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, wave = wave_of(tid), mp = wave & 1, rg = wave >> 1, i = lane & 31, g = lane >> 5;
   const Work wk = work_of(a, a.own_k, blk, a.Hkv, false);
   if (!wk.any) return;
   const int hk = wk.h, rep = a.H / a.Hkv, hd = a.hd, dv = 2 * hd;
@@ -830,16 +835,15 @@ __device__ __forceinline__ void bwd_dkv(const Args& a, unsigned char* smem, int 
   const int off = nk - nq;
   const unsigned lds0 = lds_addr(smem);
   const int c_all = (nq + CH - 1) / CH;
-  // row values behind the images: scales of the maps' queries | lse | delta | scale of dO | lsf, each [2][32]
+  // row values behind the images: scales of the maps' queries | lse | delta | dc, each [2][32]
   auto issue = [&](int h, int c, int st) {
     const unsigned dst = lds0 + st * STAGE;
     const long long r = h * NqP + qr0 + c * CH;
     copy_chunk<HD>(a.qp + r * Row<HD>::BYTES, dst, tid);
     copy_chunk<HD>(a.dp + r * Row<HD>::BYTES, dst + Row<HD>::CHUNK, tid);
     const long long at = (2 * h + g) * NqP + qr0 + c * CH + i;
-    const float* src = wave == 0 ? a.qs + at : wave == 1 ? a.lse + at : wave == 2 ? a.delta + at : a.ds + h * NqP + qr0 + c * CH + i;
-    dma4(src, dst + 2 * Row<HD>::CHUNK + __builtin_amdgcn_readfirstlane(wave) * 256);
-    if (wave == 0) dma4(a.lsf + at, dst + 2 * Row<HD>::CHUNK + 1024);
+    const float* src = wave == 0 ? a.qs + at : wave == 1 ? a.lse + at : wave == 2 ? a.delta + at : a.dc + at;
+    dma4(src, dst + 2 * Row<HD>::CHUNK + wave * 256);
   };
 
   for (int tile = wk.tile; tile * OWN < nk; tile += a.own_k.n_tiles) {
@@ -861,7 +865,6 @@ __device__ __forceinline__ void bwd_dkv(const Args& a, unsigned char* smem, int 
     int st = 0;
     for (int n = 0; n < n_all; ++n, st ^= STAGES - 1) {
       const int h = hk * rep + n / n_ch, c = c_lo + n % n_ch, t0 = c * CH, left = nq - t0;
-      const float lam = a.lam[h];
       unsigned char* img = smem + st * STAGE;
       float* sc = reinterpret_cast<float*>(img + 2 * Row<HD>::CHUNK);
       if (STAGES == 1) {
@@ -873,10 +876,7 @@ __device__ __forceinline__ void bwd_dkv(const Args& a, unsigned char* smem, int 
       if (STAGES == 2 && n + 1 < n_all) issue(hk * rep + (n + 1) / n_ch, c_lo + (n + 1) % n_ch, st ^ 1);
       if (left < CH) {      // rows behind the session's end have no probabilities
         clear_rows<HD>(img, left, tid);
-        if ((tid & 31) >= left) {
-          sc[tid] = 0.f;
-          if (tid < 64) sc[256 + tid] = 0.f;
-        }
+        if ((tid & 31) >= left) sc[tid] = 0.f;
         barrier();
       }
       const bool on = k0 < nk && !(a.causal && t0 + 31 + off < k0);
@@ -890,12 +890,9 @@ __device__ __forceinline__ void bwd_dkv(const Args& a, unsigned char* smem, int 
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const f32x4 q4 = *reinterpret_cast<const f32x4*>(sc + 32 * mp + 8 * r + 4 * g), l4 = *reinterpret_cast<const f32x4*>(sc + 64 + 32 * mp + 8 * r + 4 * g),
-                      f4 = *reinterpret_cast<const f32x4*>(sc + 256 + 32 * mp + 8 * r + 4 * g);
+                      c4 = *reinterpret_cast<const f32x4*>(sc + 192 + 32 * mp + 8 * r + 4 * g);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float x = __builtin_amdgcn_exp2f(fmaf(S[4 * r + e] * q4[e], ksc, -l4[e])) * f4[e];
-            p[4 * r + e] = x;
-          }
+          for (int e = 0; e < 4; ++e) p[4 * r + e] = __builtin_amdgcn_exp2f(fmaf(S[4 * r + e] * q4[e], ksc, -l4[e])) * c4[e];
         }
         if (edge) {
 #pragma unroll
@@ -909,24 +906,22 @@ __device__ __forceinline__ void bwd_dkv(const Args& a, unsigned char* smem, int 
       }
       barrier();
       if (!on) continue;
-      const float sign = mp == 0 ? 1.f : -lam;
       float x[16];
       P2 w[2];
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const f32x4 og = swap[((wave ^ 1) * 8 + r) * 64 + lane];
-        const f32x4 q4 = *reinterpret_cast<const f32x4*>(sc + 32 * mp + 8 * r + 4 * g), dl = *reinterpret_cast<const f32x4*>(sc + 128 + 32 * mp + 8 * r + 4 * g),
-                    d4 = *reinterpret_cast<const f32x4*>(sc + 192 + 8 * r + 4 * g);
+        const f32x4 q4 = *reinterpret_cast<const f32x4*>(sc + 32 * mp + 8 * r + 4 * g), dl = *reinterpret_cast<const f32x4*>(sc + 128 + 32 * mp + 8 * r + 4 * g);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[4 * r + e] = sign * p[4 * r + e] * fmaf((G[4 * r + e] + og[e]) * d4[e], vsc, -dl[e]) * q4[e];
+        for (int e = 0; e < 4; ++e) x[4 * r + e] = p[4 * r + e] * fmaf(G[4 * r + e] + og[e], vsc, -dl[e]) * q4[e];
       }
       split16_scaled<NB>(x, unit_k, dK, w);
       cols_dot<HD, NB>(img + mp * 4 * HD, 0, 2 * HD, w, lane, dK);
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const f32x4 op = swap[((wave ^ 1) * 8 + 4 + r) * 64 + lane], d4 = *reinterpret_cast<const f32x4*>(sc + 192 + 8 * r + 4 * g);
+        const f32x4 op = swap[((wave ^ 1) * 8 + 4 + r) * 64 + lane];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[4 * r + e] = (mp == 0 ? p[4 * r + e] - lam * op[e] : op[e] - lam * p[4 * r + e]) * d4[e];
+        for (int e = 0; e < 4; ++e) x[4 * r + e] = p[4 * r + e] + op[e];
       }
       split16_scaled<NB>(x, unit_v, dV, w);
       cols_dot<HD, NB>(img + Row<HD>::CHUNK, mp * HD, 4 * HD, w, lane, dV);
@@ -1242,8 +1237,8 @@ size_t carve_backward(Args& a, void* base, double*& part) {
   Carve c{static_cast<unsigned char*>(base)};
   const size_t row = 8 * (size_t)pad_hd(a.hd) + 48, nq = (size_t)a.Nq + PAD, H = a.H;
   c.take(a.dp, H * nq * row);
-  c.take(a.ds, H * nq);
   c.take(a.delta, 2 * H * nq);
+  c.take(a.dc, 2 * H * nq);
   c.take(part, (size_t)PRE_WG * (H + 2 * a.hd));
   return c.at;
 }
