@@ -678,14 +678,17 @@ __global__ __launch_bounds__(NT) void diff_bwd_pre_kernel(Args a, const float* d
   }
 }
 
-__global__ __launch_bounds__(64) void diff_bwd_sums_kernel(const double* part, int n, int H, int dv, float* dlam, float* dw) {
-  const int W = H + dv, c = blockIdx.x;
+struct Sums { const double* part; int n, blocks; float* dlam; float* dw; };      // of n workgroups of diff_bwd_pre_kernel
+// the partials' column sums: a wave per column (H of dlam, then 2 hd of dw)
+__device__ __forceinline__ void bwd_sums(const Args& a, const Sums& m, int blk) {
+  const int W = a.H + 2 * a.hd, c = blk * (NT / 64) + (int)(threadIdx.x >> 6);
+  if (c >= W) return;
   double s = 0.0;
-  for (int r = threadIdx.x; r < n; r += 64) s += part[(long long)r * W + c];
+  for (int r = threadIdx.x & 63; r < m.n; r += 64) s += m.part[(long long)r * W + c];
   s = wave_sum_d(s);
-  if (threadIdx.x == 0) {
-    if (c < H) dlam[c] = (float)s;
-    else if (dw != nullptr) dw[c - H] = (float)s;
+  if ((threadIdx.x & 63) == 0) {
+    if (c < a.H) m.dlam[c] = (float)s;
+    else if (m.dw != nullptr) m.dw[c - a.H] = (float)s;
   }
 }
 
@@ -949,10 +952,12 @@ __device__ __forceinline__ void bwd_dkv(const Args& a, unsigned char* smem, int 
 // Both passes in one launch, the dK/dV workgroups (one and a half times the work of the others) first: they share no data, and each alone ends with
 // a few of its longest workgroups on an empty machine.  One launch after the other took 309 + 445 us (two sessions of 4,096, 4 heads of hd 64, causal).
 template <int HD>
-__global__ __launch_bounds__(NT, 2) void diff_bwd_kernel(Args a) {
+__global__ __launch_bounds__(NT, 2) void diff_bwd_kernel(Args a, Sums m) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  if ((int)blockIdx.x < a.own_k.blocks) bwd_dkv<HD>(a, smem, blockIdx.x);
-  else bwd_dq<HD>(a, smem, (int)blockIdx.x - a.own_k.blocks);
+  const int blk = blockIdx.x;
+  if (blk < a.own_k.blocks) bwd_dkv<HD>(a, smem, blk);
+  else if (blk < a.own_k.blocks + m.blocks) bwd_sums(a, m, blk - a.own_k.blocks);
+  else bwd_dq<HD>(a, smem, blk - a.own_k.blocks - m.blocks);
 }
 
 // ---- few query rows: the products are matrix-vector products, the keys and values are read once and the loads are the work ---------------------
@@ -1248,10 +1253,10 @@ Args sizes(int H, int Hkv, int hd, long long Nq, long long Nk) {
   return a;
 }
 
-template <typename K>
-int start(K kernel, dim3 grid, size_t lds, hipStream_t stream, const Args& a) {
+template <typename K, typename... A>
+int start(K kernel, dim3 grid, size_t lds, hipStream_t stream, const A&... a) {
   if (lds > 65536) RT_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-  kernel<<<grid, NT, lds, stream>>>(a);
+  kernel<<<grid, NT, lds, stream>>>(a...);
   RT_CHECK_LAUNCH();
   return RT_OK;
 }
@@ -1398,15 +1403,12 @@ int rt_diffattn_bwd(const void* saved, size_t saved_bytes, const float* lam, con
   if (n_pre > PRE_WG) return RT_ERR_UNSUPPORTED;
   const int mode = mode_of(hd % 2 == 0 && vec_ok(dy, lddy) && (norm_w == nullptr || vec_ok(norm_w, 4)), hd);
   RT_TRY(HDP == 32 ? start_pre<32>(a, mode, (unsigned)n_pre, dy, lddy, part, stream) : start_pre<64>(a, mode, (unsigned)n_pre, dy, lddy, part, stream));
-  diff_bwd_sums_kernel<<<H + 2 * hd, 64, 0, stream>>>(part, (int)n_pre, H, 2 * hd, dlam, dw);
-  RT_CHECK_LAUNCH();
   if ((Nq > 0 && !plan_grid(a.own_q, B, H, Lq, cu_q != nullptr)) || (Nk > 0 && !plan_grid(a.own_k, B, Hkv, Lk, cu_k != nullptr))) return RT_ERR_UNSUPPORTED;
-  const long long blocks = (long long)a.own_q.blocks + a.own_k.blocks;
-  if (blocks > 0 && !grid_ok(blocks)) return RT_ERR_UNSUPPORTED;
-  if (blocks > 0) {
-    const dim3 grid((unsigned)blocks);
-    RT_TRY(HDP == 32 ? start(diff_bwd_kernel<32>, grid, bwd_lds<32>(), stream, a) : start(diff_bwd_kernel<64>, grid, bwd_lds<64>(), stream, a));
-  }
+  const Sums m{part, (int)n_pre, (H + 2 * hd + NT / 64 - 1) / (NT / 64), dlam, dw};
+  const long long blocks = (long long)a.own_q.blocks + a.own_k.blocks + m.blocks;
+  if (!grid_ok(blocks)) return RT_ERR_UNSUPPORTED;
+  const dim3 grid((unsigned)blocks);
+  RT_TRY(HDP == 32 ? start(diff_bwd_kernel<32>, grid, bwd_lds<32>(), stream, a, m) : start(diff_bwd_kernel<64>, grid, bwd_lds<64>(), stream, a, m));
   return RT_OK;
 }
 
