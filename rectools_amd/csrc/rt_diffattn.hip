@@ -39,7 +39,7 @@ constexpr int CH = 32;     // partner rows per staged chunk
 constexpr int PAD = 32;    // rows behind the last one that a chunk may copy (never used)
 
 // Work of a matrix launch: owner tiles per session (longer sessions loop), (session, head) pairs as they are counted, order (work_of)
-struct Grid { int n_tiles, bhs, paired, blocks; };
+struct Grid { int n_tiles, bhs, blocks; };
 
 struct Args {
   const float* q; const float* k; const float* v; long long ldq, ldk, ldv;
@@ -197,7 +197,6 @@ __device__ __forceinline__ void dma4(const void* src, unsigned dst) {       // l
   asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %1, off\n\ts_mov_b32 m0, %0" : "=&s"(keep) : "v"(src), "s"(dst) : "memory");
 }
 __device__ __forceinline__ void dma_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
-template <int N> __device__ __forceinline__ void dma_left() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void barrier() {      // LDS writes of this wave are visible behind it; LDS DMA is waited for by dma_done
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   __builtin_amdgcn_s_barrier();
@@ -208,17 +207,6 @@ template <int HD> __device__ __forceinline__ void copy_chunk(const unsigned char
 #pragma unroll
   for (int i = 0; i < (Row<HD>::UNITS + NT - 1) / NT; ++i)
     if (tid + i * NT < Row<HD>::UNITS) dma16(src + (size_t)(tid + i * NT) * 16, dst + (wave0 + i * NT) * 16);
-}
-// Copies of a chunk pair a wave issues (two images; row values by waves 0 and 1), and the wait that leaves `later` chunk pairs in flight: copies
-// land in the order of their issue
-template <int HD> constexpr int copies(bool first_waves) {
-  return 2 * (Row<HD>::UNITS / NT + (first_waves && Row<HD>::UNITS % NT > 0 ? 1 : 0)) + (first_waves ? 1 : 0);
-}
-template <int HD> __device__ __forceinline__ void dma_left_chunks(int later, bool first_waves) {
-  static_assert(Row<HD>::UNITS % NT <= 128, "the tail of an image is copied by waves 0 and 1");
-  if (later <= 0) dma_left<0>();
-  else if (later == 1) { if (first_waves) dma_left<copies<HD>(true)>(); else dma_left<copies<HD>(false)>(); }
-  else { if (first_waves) dma_left<2 * copies<HD>(true)>(); else dma_left<2 * copies<HD>(false)>(); }
 }
 // rows [left, CH) of two staged images: zeros (they belong to the next session, or to nobody)
 template <int HD> __device__ __forceinline__ void clear_rows(unsigned char* img, int left, int tid) {
@@ -336,13 +324,12 @@ __device__ __forceinline__ void row_norm(float base, float total, float& n, floa
 
 // blockIdx -> (owner tile, session, head, split): the tiles of the real sessions, then (b == B) the rows behind the last one.
 // Heavy tiles first (causal: a session's last queries, its first keys): where the launch is many times the machine, the light ones fill the gaps
-// at its end.  Where all workgroups are resident at once (two per CU), each CU keeps the two it is given: then (`paired`) the second half of the
-// tiles comes in the opposite order, a light one to every heavy one.
+// at its end.
 // Workgroups go to the eight dies in turn and each die has its own 4 MB of L2: with the (session, head) pairs counted in a multiple of eight (`bhs`:
 // rounded up where there are many), all tiles of a pair, which stream the same chunks, meet on one die.
 struct Work { int tile, b, h, split; bool any; };
 __device__ __forceinline__ Work work_of(const Args& a, const Grid& n, int blk, int H, bool last_first) {
-  const int real = n.bhs * n.n_tiles, half = n.n_tiles / 2, bh = blk % n.bhs;
+  const int real = n.bhs * n.n_tiles, bh = blk % n.bhs, o = blk / n.bhs;
   Work w;
   w.split = blockIdx.y;
   if (blk >= real) {
@@ -352,8 +339,6 @@ __device__ __forceinline__ Work work_of(const Args& a, const Grid& n, int blk, i
     w.any = true;
     return w;
   }
-  int o = blk / n.bhs;
-  if (n.paired && o >= n.n_tiles - half) o = n.n_tiles - 1 - (o - (n.n_tiles - half));
   w.tile = last_first ? n.n_tiles - 1 - o : o;
   w.b = bh / H;
   w.h = bh % H;
@@ -370,15 +355,14 @@ __device__ __forceinline__ int fresh(int x) {
 // ---- forward ----------------------------------------------------------------------------------------------------------------------------
 // Values carry their row's scale 2^e: the running maximum is that of s + e, so the weights exp2(s + e - m) stay below one whatever the scales
 // are, and the row sum takes them back by 2^-e.
-template <int HD> constexpr int fwd_stages() { return 2; }
 template <int HD> constexpr int fwd_stage() { return 2 * Row<HD>::CHUNK + 512; }      // K | V | key scales of the maps | e, 2^-e
 
-template <int HD>
-__global__ __launch_bounds__(NT, HD == 32 ? 3 : 2) void diff_fwd_kernel(Args a) {
-  constexpr int DV = 2 * HD, NS = HD / 16, NB = DV / 32, STAGE = fwd_stage<HD>(), STAGES = fwd_stages<HD>();
+template <int HD, int KH>
+__global__ __launch_bounds__(KH * NT, HD == 32 && KH == 1 ? 3 : 2) void diff_fwd_kernel(Args a) {
+  constexpr int DV = 2 * HD, NS = HD / 16, NB = DV / 32, STAGE = KH * fwd_stage<HD>();
   constexpr float UP = 14.f;      // weights come to 2^14 at most
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  const int tid = threadIdx.x, lane = tid & 63, wave = wave_of(tid), mp = wave & 1, rg = wave >> 1, i = lane & 31, g = lane >> 5;
+  const int tid = threadIdx.x % NT, kh = KH == 1 ? 0 : wave_of(threadIdx.x) / 4, lane = tid & 63, wave = wave_of(tid), mp = wave & 1, rg = wave >> 1, i = lane & 31, g = lane >> 5;
   const Work wk = work_of(a, a.own_q, blockIdx.x, a.H, a.causal != 0);
   if (!wk.any) return;
   const int h = wk.h, hk = h / (a.H / a.Hkv), dv = 2 * a.hd;
@@ -387,7 +371,7 @@ __global__ __launch_bounds__(NT, HD == 32 ? 3 : 2) void diff_fwd_kernel(Args a) 
   if (wk.b == a.B) {      // rows behind the last session: zeros
     if (wk.split != 0) return;
     const long long r0 = rows_used(a.cu_q, a.B, a.Nq);
-    for (long long r = r0 + wk.tile; r < a.Nq; r += a.own_q.n_tiles) {
+    for (long long r = r0 + wk.tile; r < a.Nq && kh == 0; r += a.own_q.n_tiles) {
       for (int c = tid; c < dv; c += NT) a.y[r * a.ldy + (long long)h * dv + c] = 0.f;
       if (a.o12 != nullptr) for (int c = tid; c < 2 * dv; c += NT) a.o12[(r * a.H + h) * 2 * dv + c] = 0.f;
     }
@@ -398,7 +382,7 @@ __global__ __launch_bounds__(NT, HD == 32 ? 3 : 2) void diff_fwd_kernel(Args a) 
   rows_of(a.cu_k, wk.b, a.Lk, a.Nk, kr0, nk);
   const int off = nk - nq;
   const float lam = a.lam[h];
-  const unsigned lds0 = lds_addr(smem);
+  const unsigned lds0 = lds_addr(smem) + kh * fwd_stage<HD>();
   const long long krow = hk * NkP + kr0;
   auto issue = [&](int c, int st) {
     const unsigned dst = lds0 + st * STAGE;
@@ -430,24 +414,24 @@ __global__ __launch_bounds__(NT, HD == 32 ? 3 : 2) void diff_fwd_kernel(Args a) 
       c_hi = min(c_hi, c_lo + each);
     }
     barrier();      // (the previous tile's readers are done)
-#pragma unroll
-    for (int k = 0; k < STAGES - 1; ++k)
-      if (c_lo + k < c_hi) issue(c_lo + k, k);
+    if (c_lo + kh < c_hi) issue(c_lo + kh, 0);
     int st = 0;
-    for (int c = c_lo; c < c_hi; ++c) {
+    for (int c0 = c_lo; c0 < c_hi; c0 += KH, st ^= 1) {
+      const int c = c0 + kh;
       const int t0 = c * CH, left = nk - t0;
-      unsigned char* img = smem + st * STAGE;
+      unsigned char* img = smem + st * STAGE + kh * fwd_stage<HD>();
       float* sc = reinterpret_cast<float*>(img + 2 * Row<HD>::CHUNK);
-      dma_left_chunks<HD>(min(STAGES - 2, c_hi - 1 - c), wave < 2);
+      dma_done();
       barrier();                                    // chunk c is here, chunk c - 1 has been read
-      if (c + STAGES - 1 < c_hi) issue(c + STAGES - 1, st == 0 ? STAGES - 1 : st - 1);
-      st = st == STAGES - 1 ? 0 : st + 1;
-      if (left < CH) {
-        clear_rows<HD>(img, left, tid);
-        if (tid < 128 && (tid & 31) >= left) sc[tid] = 0.f;
+      if (c + KH < c_hi) issue(c + KH, st ^ 1);
+      if (nk - (c0 + KH - 1) * CH < CH) {      // (the same in all waves)
+        if (left < CH && c < c_hi) {
+          clear_rows<HD>(img, left, tid);
+          if (tid < 128 && (tid & 31) >= left) sc[tid] = 0.f;
+        }
         barrier();
       }
-      if (q0 >= nq || (a.causal && t0 > q0 + 31 + off)) continue;      // (wave-uniform) nothing of the chunk is visible to the row group
+      if (c >= c_hi || q0 >= nq || (a.causal && t0 > q0 + 31 + off)) continue;      // (wave-uniform) nothing of the chunk is visible to the row group
       f32x16 S = zero16();
       rows_dot<HD, NS>(img + mp * 4 * HD, 0, 2 * HD, Qp, i, g, S);
       float x[16];
@@ -491,9 +475,35 @@ __global__ __launch_bounds__(NT, HD == 32 ? 3 : 2) void diff_fwd_kernel(Args a) 
       split16(x, one, Pp);
       cols_dot<HD, NB>(img + Row<HD>::CHUNK, 0, 4 * HD, Pp, lane, O);
     }
-    const float l = lsum + __shfl_xor(lsum, 32, 64);
+    float l = lsum + __shfl_xor(lsum, 32, 64);
+    if (KH == 2) {      // the second half's maximum, sum and outputs join the first's
+      f32x4* xh = reinterpret_cast<f32x4*>(smem) + wave * (NB * 4 + 1) * 64;
+      barrier();
+      if (kh == 1) {
+#pragma unroll
+        for (int cb = 0; cb < NB; ++cb)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) xh[(cb * 4 + r) * 64 + lane] = f32x4{O[cb][4 * r], O[cb][4 * r + 1], O[cb][4 * r + 2], O[cb][4 * r + 3]};
+        xh[NB * 4 * 64 + lane] = f32x4{m, l, 0.f, 0.f};
+      }
+      barrier();
+      if (kh == 0) {
+        const f32x4 ml = xh[NB * 4 * 64 + lane];
+        const float mx = fmaxf(m, ml[0]), base = mx == -INFINITY ? 0.f : mx, e0 = __builtin_amdgcn_exp2f(m - base), e1 = __builtin_amdgcn_exp2f(ml[0] - base);
+        m = mx;
+        l = l * e0 + ml[1] * e1;
+#pragma unroll
+        for (int cb = 0; cb < NB; ++cb)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const f32x4 o = xh[(cb * 4 + r) * 64 + lane];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) O[cb][4 * r + e] = fmaf(o[e], e1, O[cb][4 * r + e] * e0);
+          }
+      }
+    }
     if (a.n_split > 1) {      // partial sums as they are; diff_combine_kernel joins the splits
-      if (qok) {
+      if (kh == 0 && qok) {
         const int n = fresh(dv);
         const long long at = (((long long)wk.split * a.Nq + qr0 + qi) * a.H + h) * 2 + mp;
         if (g == 0) { a.ml[2 * at] = m; a.ml[2 * at + 1] = l * 0x1p-14f; }
@@ -509,8 +519,8 @@ __global__ __launch_bounds__(NT, HD == 32 ? 3 : 2) void diff_fwd_kernel(Args a) 
     const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);      // (a NaN sum stays one)
 #pragma unroll
     for (int cb = 0; cb < NB; ++cb) O[cb] *= inv;
-    if (qok && a.lse != nullptr && g == 0) row_norm(m - UP, l, a.lse[(2 * h + mp) * NqP + qr0 + qi], a.lsf[(2 * h + mp) * NqP + qr0 + qi]);
-    if (qok && a.o12 != nullptr) {
+    if (kh == 0 && qok && a.lse != nullptr && g == 0) row_norm(m - UP, l, a.lse[(2 * h + mp) * NqP + qr0 + qi], a.lsf[(2 * h + mp) * NqP + qr0 + qi]);
+    if (kh == 0 && qok && a.o12 != nullptr) {
       const int n = fresh(dv);
       float* o = a.o12 + (((qr0 + qi) * a.H + h) * 2 + mp) * (long long)n;
 #pragma unroll
@@ -521,14 +531,14 @@ __global__ __launch_bounds__(NT, HD == 32 ? 3 : 2) void diff_fwd_kernel(Args a) 
     // the second map's wave hands its output over; the first one's subtracts, normalises and writes
     barrier();
     f32x4* xo = reinterpret_cast<f32x4*>(smem) + rg * (NB * 4 * 64);
-    if (mp == 1) {
+    if (kh == 0 && mp == 1) {
 #pragma unroll
       for (int cb = 0; cb < NB; ++cb)
 #pragma unroll
         for (int r = 0; r < 4; ++r) xo[(cb * 4 + r) * 64 + lane] = f32x4{O[cb][4 * r], O[cb][4 * r + 1], O[cb][4 * r + 2], O[cb][4 * r + 3]};
     }
     barrier();
-    if (mp == 0) {
+    if (kh == 0 && mp == 0) {
       float ss = 0.f;
 #pragma unroll
       for (int cb = 0; cb < NB; ++cb)
@@ -1207,7 +1217,7 @@ bool grid_ok(long long blocks) { return blocks > 0 && blocks <= 0xFFFFFFFFLL / N
 bool plan_grid(Grid& g, int B, int H, int L, bool tail) {
   const long long bhs = (long long)B * H, counted = bhs >= 64 ? (bhs + 7) / 8 * 8 : (bhs > 0 ? bhs : 1), tiles = L > 0 ? (L + OWN - 1) / OWN : 1;
   const long long blocks = (counted + (tail ? H : 0)) * tiles;
-  g = Grid{(int)tiles, (int)counted, 0, (int)blocks};
+  g = Grid{(int)tiles, (int)counted, (int)blocks};
   return grid_ok(blocks);
 }
 
@@ -1254,9 +1264,9 @@ Args sizes(int H, int Hkv, int hd, long long Nq, long long Nk) {
 }
 
 template <typename K, typename... A>
-int start(K kernel, dim3 grid, size_t lds, hipStream_t stream, const A&... a) {
+int start(K kernel, dim3 grid, int threads, size_t lds, hipStream_t stream, const A&... a) {
   if (lds > 65536) RT_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-  kernel<<<grid, NT, lds, stream>>>(a...);
+  kernel<<<grid, threads, lds, stream>>>(a...);
   RT_CHECK_LAUNCH();
   return RT_OK;
 }
@@ -1265,8 +1275,8 @@ int mode_of(bool vec, int hd) { return !vec ? 2 : (hd == pad_hd(hd) ? 0 : 1); }
 
 template <int HD, int R>
 int start_decode(int mode, dim3 grid, hipStream_t stream, const Args& a) {
-  return mode == 0 ? start(diff_decode_kernel<HD, 0, R>, grid, 0, stream, a) : mode == 1 ? start(diff_decode_kernel<HD, 1, R>, grid, 0, stream, a)
-                                                                                         : start(diff_decode_kernel<HD, 2, R>, grid, 0, stream, a);
+  return mode == 0 ? start(diff_decode_kernel<HD, 0, R>, grid, NT, 0, stream, a) : mode == 1 ? start(diff_decode_kernel<HD, 1, R>, grid, NT, 0, stream, a)
+                                                                                         : start(diff_decode_kernel<HD, 2, R>, grid, NT, 0, stream, a);
 }
 template <int HD>
 int start_decode(long long queries, int mode, dim3 grid, hipStream_t stream, const Args& a) {
@@ -1351,11 +1361,18 @@ int rt_diffattn_fwd(const float* q, int64_t ldq, const float* k, int64_t ldk, co
     RT_TRY(HDP == 32 ? start_decode<32>(queries, mode, grid, stream, a) : start_decode<64>(queries, mode, grid, stream, a));
   } else {
     if (!plan_grid(a.own_q, B, H, Lq, cu_q != nullptr)) return RT_ERR_UNSUPPORTED;
-    a.own_q.paired = causal && (long long)B * H * a.own_q.n_tiles * p.n_split <= 2LL * rt_num_cus();
+    // One workgroup of eight waves per CU, two chunks at a time, where all the workgroups of four would be resident at once: a CU keeps the two it is given
+    // then, and a causal session's heavy one ends alone; as one workgroup the tiles are dealt out one after the other, the light ones behind the
+    // heavy ones.  4 heads, planes included: 2 x 4,096 rows, hd 64 267 -> 219 us, hd 32 174 -> 134; 1 x 4,096 (keys in two splits) 197 -> 148.  Short shares of
+    // the keys lose by the join of the two halves (1 x 1,024, eight splits: 36 -> 42 us; 100 x 128, hd 32: 22.5 -> 25.8), and where there are more tiles
+    // than that, two independent workgroups overlap better (64 x 512, hd 64: 205 -> 248).
+    const bool wide = causal && Lk / p.n_split > 256 && (long long)B * H * a.own_q.n_tiles * p.n_split <= 2LL * rt_num_cus();
     carve_planes(a, saved != nullptr ? saved : (unsigned char*)ws + ((part_bytes + 255) & ~(size_t)255), saved != nullptr);
     RT_TRY(HDP == 32 ? start_planes<32>(a, mode, stream) : start_planes<64>(a, mode, stream));
     const dim3 grid((unsigned)a.own_q.blocks, p.n_split);
-    RT_TRY(HDP == 32 ? start(diff_fwd_kernel<32>, grid, fwd_stages<32>() * fwd_stage<32>(), stream, a) : start(diff_fwd_kernel<64>, grid, fwd_stages<64>() * fwd_stage<64>(), stream, a));
+    const int lds = HDP == 32 ? 2 * fwd_stage<32>() : 2 * fwd_stage<64>();
+    if (wide) RT_TRY(HDP == 32 ? start(diff_fwd_kernel<32, 2>, grid, 2 * NT, 2 * lds, stream, a) : start(diff_fwd_kernel<64, 2>, grid, 2 * NT, 2 * lds, stream, a));
+    else RT_TRY(HDP == 32 ? start(diff_fwd_kernel<32, 1>, grid, NT, lds, stream, a) : start(diff_fwd_kernel<64, 1>, grid, NT, lds, stream, a));
   }
   if (p.n_split > 1) {
     if (!grid_ok(Nq * H)) return RT_ERR_UNSUPPORTED;
@@ -1408,7 +1425,7 @@ int rt_diffattn_bwd(const void* saved, size_t saved_bytes, const float* lam, con
   const long long blocks = (long long)a.own_q.blocks + a.own_k.blocks + m.blocks;
   if (!grid_ok(blocks)) return RT_ERR_UNSUPPORTED;
   const dim3 grid((unsigned)blocks);
-  RT_TRY(HDP == 32 ? start(diff_bwd_kernel<32>, grid, bwd_lds<32>(), stream, a, m) : start(diff_bwd_kernel<64>, grid, bwd_lds<64>(), stream, a, m));
+  RT_TRY(HDP == 32 ? start(diff_bwd_kernel<32>, grid, NT, bwd_lds<32>(), stream, a, m) : start(diff_bwd_kernel<64>, grid, NT, bwd_lds<64>(), stream, a, m));
   return RT_OK;
 }
 

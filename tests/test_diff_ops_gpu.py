@@ -331,6 +331,20 @@ def test_attention_split_keys(rows, keys, hd):
     _attention_case([rows, 1], [keys, 3], 2, 1, hd, False, train=False)
 
 
+@pytest.mark.parametrize("hd", [32, 50, 64])
+def test_attention_long_causal_sessions(hd):
+    """Few long sessions: two halves of the keys per workgroup; odd counts of chunks, a session without rows, one of a single chunk."""
+    _attention_case([600, 289, 0, 33], [600, 289, 0, 33], 2, 1, hd, True, train=True)
+    ids = torch.ones(935, dtype=torch.int64)
+    ids[::7] = 0
+    ids[600:640] = 0
+    _attention_case([610, 325], [610, 325], 2, 2, hd, True, ids=ids, train=False)
+
+
+def test_attention_long_causal_session_in_halves_and_splits():
+    _attention_case([2_500], [2_500], 4, 2, 32, True, train=True)
+
+
 def test_attention_split_keys_training():
     _attention_case([20], [3_000], 2, 1, 32, True, train=True)
 
