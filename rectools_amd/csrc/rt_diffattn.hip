@@ -236,10 +236,10 @@ template <int NS> __device__ __forceinline__ void load_own(const unsigned char* 
     out[s].l = *reinterpret_cast<const h8*>(row + (c0 + 16 * s + 8 * g) * 2 + plane);
   }
 }
-// acc[r] += sum_c img[row(r)][c0 + c] * own[c], row(r) = 8 (r / 4) + 4 g + r % 4: the partner rows are the registers, the owner the lane
+// acc[r] = sum_c img[row(r)][c0 + c] * own[c], row(r) = 8 (r / 4) + 4 g + r % 4: the partner rows are the registers, the owner the lane
 // All fragments are read in front of the products (the compiler reads each in front of the instruction that needs it: an LDS latency per step).
 template <int HD, int NS>
-__device__ __forceinline__ void rows_dot(const unsigned char* img, int c0, int plane, const P2 (&own)[NS], int i, int g, f32x16& acc) {
+__device__ __forceinline__ void rows_dot(const unsigned char* img, int c0, int plane, const P2 (&own)[NS], int i, int g, f32x16& out) {
   const unsigned char* p = img + i * Row<HD>::BYTES + c0 * 2 + 16 * g;
   P2 A[NS];
 #pragma unroll
@@ -247,11 +247,13 @@ __device__ __forceinline__ void rows_dot(const unsigned char* img, int c0, int p
     A[s].h = *reinterpret_cast<const h8*>(p + 32 * s);
     A[s].l = *reinterpret_cast<const h8*>(p + 32 * s + plane);
   }
+  f32x16 acc = zero16();      // (the first product's constant operand)
   __builtin_amdgcn_sched_barrier(0);
   __builtin_amdgcn_s_setprio(1);
 #pragma unroll
   for (int s = 0; s < NS; ++s) acc = mfma3(A[s], own[s], acc);
   __builtin_amdgcn_s_setprio(0);
+  out = acc;
 }
 // acc[cb][r] += sum over the 32 partner rows of img[row][c0 + 32 cb + col(r)] * w[row], the lane's weights in the accumulator order of rows_dot
 // (slot j of step t = register 8 t + j = row 16 t + 8 (j / 4) + 4 g + j % 4): the partner rows are the reduction index, read transposed
@@ -432,7 +434,7 @@ __global__ __launch_bounds__(KH * NT, HD == 32 && KH == 1 ? 3 : 2) void diff_fwd
         barrier();
       }
       if (c >= c_hi || q0 >= nq || (a.causal && t0 > q0 + 31 + off)) continue;      // (wave-uniform) nothing of the chunk is visible to the row group
-      f32x16 S = zero16();
+      f32x16 S;
       rows_dot<HD, NS>(img + mp * 4 * HD, 0, 2 * HD, Qp, i, g, S);
       float x[16];
 #pragma unroll
@@ -773,7 +775,7 @@ __device__ __forceinline__ void bwd_dq(const Args& a, unsigned char* smem, int b
         barrier();
       }
       const bool on = q0 < nq && !(a.causal && t0 > q0 + 31 + off);      // (the same for the two waves of a row group)
-      f32x16 S = zero16(), G = zero16();
+      f32x16 S, G;
       if (on) {
         rows_dot<HD, NS>(img + Row<HD>::CHUNK, mp * HD, 4 * HD, Dp, i, g, G);
 #pragma unroll
@@ -893,7 +895,7 @@ __device__ __forceinline__ void bwd_dkv(const Args& a, unsigned char* smem, int 
         barrier();
       }
       const bool on = k0 < nk && !(a.causal && t0 + 31 + off < k0);
-      f32x16 S = zero16(), G = zero16();
+      f32x16 S, G;
       float p[16];
       if (on) {
         rows_dot<HD, NS>(img + mp * 4 * HD, 0, 2 * HD, Kp, i, g, S);
