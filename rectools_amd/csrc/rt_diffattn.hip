@@ -356,13 +356,15 @@ __device__ __forceinline__ int fresh(int x) {
 
 // ---- forward ----------------------------------------------------------------------------------------------------------------------------
 // Values carry their row's scale 2^e: the running maximum is that of s + e, so the weights exp2(s + e - m) stay below one whatever the scales
-// are, and the row sum takes them back by 2^-e.
+// are, and the row sum takes them back by 2^-e.  m is a whole number, taken up only when a logit passes it (by the next whole number above it): e - m is
+// exact then and the weight's argument has one rounding, at its own size — s + e, 10 and more in magnitude, would carry 5e-7 into every
+// weight (outputs were off by 3.2e-7 for it, where the plain form is by 1.5e-7).
 template <int HD> constexpr int fwd_stage() { return 2 * Row<HD>::CHUNK + 512; }      // K | V | key scales of the maps | e, 2^-e
 
 template <int HD, int KH>
 __global__ __launch_bounds__(KH * NT, HD == 32 && KH == 1 ? 3 : 2) void diff_fwd_kernel(Args a) {
   constexpr int DV = 2 * HD, NS = HD / 16, NB = DV / 32, STAGE = KH * fwd_stage<HD>();
-  constexpr float UP = 14.f;      // weights come to 2^14 at most
+  constexpr float UP = 0x1p14f;      // weights of at most 1 come to the fp16 planes as 2^14
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const int tid = threadIdx.x % NT, kh = KH == 1 ? 0 : wave_of(threadIdx.x) / 4, lane = tid & 63, wave = wave_of(tid), mp = wave & 1, rg = wave >> 1, i = lane & 31, g = lane >> 5;
   const Work wk = work_of(a, a.own_q, blockIdx.x, a.H, a.causal != 0);
@@ -437,44 +439,50 @@ __global__ __launch_bounds__(KH * NT, HD == 32 && KH == 1 ? 3 : 2) void diff_fwd
       f32x16 S;
       rows_dot<HD, NS>(img + mp * 4 * HD, 0, 2 * HD, Qp, i, g, S);
       float x[16];
+      const bool edge = left < CH || (a.causal && t0 + 31 > q0 + off);
+      const int last = a.causal ? min(qi + off - t0, left - 1) : left - 1;
+      auto logits = [&](float from) {      // s + e - from, one rounding: e and `from` are whole numbers
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const f32x4 k4 = *reinterpret_cast<const f32x4*>(sc + 32 * mp + 8 * r + 4 * g), e4 = *reinterpret_cast<const f32x4*>(sc + 64 + 8 * r + 4 * g);
+        for (int r = 0; r < 4; ++r) {
+          const f32x4 k4 = *reinterpret_cast<const f32x4*>(sc + 32 * mp + 8 * r + 4 * g), e4 = *reinterpret_cast<const f32x4*>(sc + 64 + 8 * r + 4 * g);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[4 * r + e] = fmaf(S[4 * r + e] * k4[e], qsc, e4[e]);
-      }
-      if (left < CH || (a.causal && t0 + 31 > q0 + off)) {
-        const int last = a.causal ? min(qi + off - t0, left - 1) : left - 1;
+          for (int e = 0; e < 4; ++e) x[4 * r + e] = fmaf(S[4 * r + e] * k4[e], qsc, e4[e] - from);
+        }
+        if (edge) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) x[r] = reg_row(r, g) <= last ? x[r] : -INFINITY;
-      }
-      float mx = x[0];
+          for (int r = 0; r < 16; ++r) x[r] = reg_row(r, g) <= last ? x[r] : -INFINITY;
+        }
+      };
+      const float was = m == -INFINITY ? 0.f : m;      // a row that has seen no key yet
+      logits(was);
+      float top = x[0];
 #pragma unroll
-      for (int r = 1; r < 16; ++r) mx = fmaxf(mx, x[r]);
-      mx = fmaxf(m, fmaxf(mx, __shfl_xor(mx, 32, 64)));
-      const float base = mx == -INFINITY ? 0.f : mx;      // a row that has seen no key yet
-      const float alpha = __builtin_amdgcn_exp2f(m - base);
-      if (__any(mx != m)) {
+      for (int r = 1; r < 16; ++r) top = fmaxf(top, x[r]);
+      top = fmaxf(top, __shfl_xor(top, 32, 64));
+      const bool grows = top > 0.f || (m == -INFINITY && top > -INFINITY);
+      if (__any(grows)) {
+        const float now = grows ? was + ceilf(top) : was, alpha = __builtin_amdgcn_exp2f(m - now);
+        m = grows ? now : m;
         lsum *= alpha;
 #pragma unroll
         for (int cb = 0; cb < NB; ++cb) O[cb] *= alpha;
+        logits(now);
       }
-      m = mx;
       float ps = 0.f;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const f32x4 i4 = *reinterpret_cast<const f32x4*>(sc + 96 + 8 * r + 4 * g);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          x[4 * r + e] = __builtin_amdgcn_exp2f(x[4 * r + e] - (base - UP));
+          x[4 * r + e] = __builtin_amdgcn_exp2f(x[4 * r + e]);
           ps = fmaf(x[4 * r + e], i4[e], ps);
         }
       }
       lsum += ps;
       P2 Pp[2];
-      float one = 1.f;      // (opaque: or the multiply-adds become conversions and differences, four instructions for two)
-      asm("" : "+s"(one));
-      split16(x, one, Pp);
+      float up = UP;      // (opaque: or the multiply-adds become conversions and differences, four instructions for two)
+      asm("" : "+s"(up));
+      split16(x, up, Pp);
       cols_dot<HD, NB>(img + Row<HD>::CHUNK, 0, 4 * HD, Pp, lane, O);
     }
     float l = lsum + __shfl_xor(lsum, 32, 64);
@@ -508,7 +516,7 @@ __global__ __launch_bounds__(KH * NT, HD == 32 && KH == 1 ? 3 : 2) void diff_fwd
       if (kh == 0 && qok) {
         const int n = fresh(dv);
         const long long at = (((long long)wk.split * a.Nq + qr0 + qi) * a.H + h) * 2 + mp;
-        if (g == 0) { a.ml[2 * at] = m; a.ml[2 * at + 1] = l * 0x1p-14f; }
+        if (g == 0) { a.ml[2 * at] = m; a.ml[2 * at + 1] = l; }
         float* o = a.part + at * dv;
 #pragma unroll
         for (int cb = 0; cb < NB; ++cb)
@@ -520,8 +528,8 @@ __global__ __launch_bounds__(KH * NT, HD == 32 && KH == 1 ? 3 : 2) void diff_fwd
     }
     const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);      // (a NaN sum stays one)
 #pragma unroll
-    for (int cb = 0; cb < NB; ++cb) O[cb] *= inv;
-    if (kh == 0 && qok && a.lse != nullptr && g == 0) row_norm(m - UP, l, a.lse[(2 * h + mp) * NqP + qr0 + qi], a.lsf[(2 * h + mp) * NqP + qr0 + qi]);
+    for (int cb = 0; cb < NB; ++cb) O[cb] *= inv * (1.f / UP);
+    if (kh == 0 && qok && a.lse != nullptr && g == 0) row_norm(m, l, a.lse[(2 * h + mp) * NqP + qr0 + qi], a.lsf[(2 * h + mp) * NqP + qr0 + qi]);
     if (kh == 0 && qok && a.o12 != nullptr) {
       const int n = fresh(dv);
       float* o = a.o12 + (((qr0 + qi) * a.H + h) * 2 + mp) * (long long)n;
