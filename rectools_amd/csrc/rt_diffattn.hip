@@ -95,6 +95,19 @@ template <int LANES> __device__ __forceinline__ float group_sum(float v) {      
   if (LANES > 16) v += lane_xor16(v);
   return v;
 }
+template <int CTRL> __device__ __forceinline__ double dpp_d(double v) {
+  const long long b = __builtin_bit_cast(long long, v);
+  const unsigned lo = __builtin_amdgcn_update_dpp(0, (int)b, CTRL, 0xF, 0xF, true), hi = __builtin_amdgcn_update_dpp(0, (int)(b >> 32), CTRL, 0xF, 0xF, true);
+  return __builtin_bit_cast(double, (unsigned long long)lo | (unsigned long long)hi << 32);
+}
+template <int LANES> __device__ __forceinline__ double group_sum(double v) {
+  v += dpp_d<0xB1>(v);
+  v += dpp_d<0x4E>(v);
+  v += dpp_d<0x141>(v);
+  if (LANES > 8) v += dpp_d<0x140>(v);
+  if (LANES > 16) v += __shfl_xor(v, 16, 64);
+  return v;
+}
 template <int LANES> __device__ __forceinline__ float group_max(float v) {
   v = fmaxf(v, dpp<0xB1>(v));
   v = fmaxf(v, dpp<0x4E>(v));
@@ -651,34 +664,42 @@ __global__ __launch_bounds__(NT) void diff_bwd_pre_kernel(Args a, const float* d
     const long long at = row * H + h;
     const f32x4 o1 = get4<MODE>(a.o12 + at * 2 * dv, c, dv), o2 = get4<MODE>(a.o12 + (at * 2 + 1) * dv, c, dv);
     const f32x4 g = get4<MODE>(dy + row * lddy + (long long)h * dv, c, dv), e = g * w;
-    f32x4 d = e;
+    double t[4] = {e[0], e[1], e[2], e[3]};
     if (a.norm_w != nullptr) {
-      const f32x4 x = o1 - o2 * lam;
-      const float r = 1.f / sqrtf(group_sum<LANES>(x[0] * x[0] + x[1] * x[1] + x[2] * x[2] + x[3] * x[3]) * inv + a.eps);
-      const f32x4 u = x * r;
-      const float mean = group_sum<LANES>(e[0] * u[0] + e[1] * u[1] + e[2] * u[2] + e[3] * u[3]) * inv;
+      double x[4], xx = 0.0, ex = 0.0;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        d[k] = r * (e[k] - u[k] * mean);
-        dw[k] += (double)(a.out_scale * g[k] * u[k]);
+        x[k] = (double)o1[k] - (double)lam * (double)o2[k];
+        xx += x[k] * x[k];
+        ex += t[k] * x[k];
+      }
+      xx = group_sum<LANES>(xx) + (double)dv * (double)a.eps;
+      const float r = 1.f / sqrtf((float)xx * inv);
+      const double part_x = group_sum<LANES>(ex) / xx;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        t[k] = (double)r * (t[k] - part_x * x[k]);
+        dw[k] += (double)(a.out_scale * g[k] * r) * x[k];
       }
     }
-    if (MODE != 0) {
+    f32x4 d;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) d[k] = c + k < dv ? d[k] : 0.f;
+    for (int k = 0; k < 4; ++k) {
+      if (MODE != 0) t[k] = c + k < dv ? t[k] : 0.0;
+      d[k] = (float)t[k];
     }
     const int ex = row_exp(group_max<LANES>(top4(d)), -126);
     put_planes(a.dp + (h * NqP + row) * Row<HD>::BYTES + 2 * c, 4 * HD, d, ex);
-    const float s1 = group_sum<LANES>(d[0] * o1[0] + d[1] * o1[1] + d[2] * o1[2] + d[3] * o1[3]);
-    const float s2 = group_sum<LANES>(d[0] * o2[0] + d[1] * o2[1] + d[2] * o2[2] + d[3] * o2[3]);
+    const double s1 = group_sum<LANES>(t[0] * o1[0] + t[1] * o1[1] + t[2] * o1[2] + t[3] * o1[3]);
+    const double s2 = group_sum<LANES>(t[0] * o2[0] + t[1] * o2[1] + t[2] * o2[2] + t[3] * o2[3]);
     if (c == 0) {
       const long long m1 = 2 * h * NqP + row, m2 = m1 + NqP;
-      a.delta[m1] = __builtin_amdgcn_ldexpf(s1, -ex);
-      a.delta[m2] = __builtin_amdgcn_ldexpf(s2, -ex);
+      a.delta[m1] = __builtin_amdgcn_ldexpf((float)s1, -ex);
+      a.delta[m2] = __builtin_amdgcn_ldexpf((float)s2, -ex);
       a.dc[m1] = a.lsf[m1] * pow2(ex);
       a.dc[m2] = a.lsf[m2] * -lam * pow2(ex);
     }
-    dl -= (double)s2;
+    dl -= s2;
   }
 #pragma unroll
   for (int k = 0; k < 4; ++k) sw[gid][c + k] = dw[k];
@@ -712,6 +733,9 @@ __device__ __forceinline__ void bwd_sums(const Args& a, const Sums& m, int blk) 
   }
 }
 
+// dS = p (G - delta), delta the row's mean of G under p.  delta comes from the outputs (do . o: rows as long as one likes, one number), which is off by
+// the rounding of o; where one key holds nearly all of the weight G - delta cancels down to that.  Rows that see 32 keys at most — a session's
+// first rows, short sessions — take the mean of the very G that it is taken from: a row with one key has a gradient of exactly zero.
 // ---- backward, dQ: the owner is a query; both maps need G^T = V dO^T, each wave makes it over half of V's columns and they swap halves ------
 // STAGES: two where two workgroups with two chunk buffers fit a CU's LDS (HD 32), else one: the other workgroup's products run under the copy.
 template <int HD> constexpr int bwd_stages() { return HD == 32 ? 2 : 1; }
@@ -795,14 +819,31 @@ __device__ __forceinline__ void bwd_dq(const Args& a, unsigned char* smem, int b
       float x[16];
       const bool edge = left < CH || (a.causal && t0 + 31 > q0 + off);
       const int last = a.causal ? min(qi + off - t0, left - 1) : left - 1;
+      float mean = dl;
+      if ((a.causal ? min(nk, q0 + 32 + off) : nk) <= CH) {      // the only chunk that these rows see
+        float sum = 0.f, d = 0.f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const bool ok = reg_row(r, g) <= last && sc[64 + reg_row(r, g)] != -INFINITY;
+          x[r] = ok ? __builtin_amdgcn_exp2f(fmaf(S[r] * sc[32 * mp + reg_row(r, g)], qsc, -lse)) : 0.f;
+          sum += x[r];
+        }
+        sum += __shfl_xor(sum, 32, 64);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          if (x[r] > 0.f) d = fmaf(x[r] / sum, (G[r] + swap[((wave ^ 1) * 4 + (r >> 2)) * 64 + lane][r & 3]) * sc[96 + reg_row(r, g)], d);
+          __builtin_amdgcn_sched_barrier(0);      // (one key after the other: few registers)
+        }
+        d += __shfl_xor(d, 32, 64);
+        mean = sum > 0.f ? d : dl;
+      }
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const f32x4 other = swap[((wave ^ 1) * 4 + r) * 64 + lane];
         const f32x4 k4 = *reinterpret_cast<const f32x4*>(sc + 32 * mp + 8 * r + 4 * g), v4 = *reinterpret_cast<const f32x4*>(sc + 96 + 8 * r + 4 * g);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          x[4 * r + e] = __builtin_amdgcn_exp2f(fmaf(S[4 * r + e] * k4[e], qsc, -lse)) * fmaf(G[4 * r + e] + other[e], v4[e], -dl) * k4[e];
-        }
+        for (int e = 0; e < 4; ++e)
+          x[4 * r + e] = __builtin_amdgcn_exp2f(fmaf(S[4 * r + e] * k4[e], qsc, -lse)) * fmaf(G[4 * r + e] + other[e], v4[e], -mean) * k4[e];
       }
       if (edge) {
 #pragma unroll
@@ -931,12 +972,22 @@ __device__ __forceinline__ void bwd_dkv(const Args& a, unsigned char* smem, int 
       if (!on) continue;
       float x[16];
       P2 w[2];
+      if ((a.causal ? min(nk, t0 + 32 + off) : nk) <= CH) {      // rows that see no other keys than the wave's
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const f32x4 og = swap[((wave ^ 1) * 8 + r) * 64 + lane];
-        const f32x4 q4 = *reinterpret_cast<const f32x4*>(sc + 32 * mp + 8 * r + 4 * g), dl = *reinterpret_cast<const f32x4*>(sc + 128 + 32 * mp + 8 * r + 4 * g);
+        for (int r = 0; r < 16; ++r) {
+          const bool ok = kok && (!a.causal || t0 + reg_row(r, g) + off >= ki);
+          const float sum = group_sum<32>(ok ? p[r] : 0.f), gr = (G[r] + swap[((wave ^ 1) * 8 + (r >> 2)) * 64 + lane][r & 3]) * vsc;
+          x[r] = p[r] * (gr - group_sum<32>(ok && sum != 0.f ? p[r] / sum * gr : 0.f)) * sc[32 * mp + reg_row(r, g)];
+          __builtin_amdgcn_sched_barrier(0);      // (one row after the other: few registers)
+        }
+      } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[4 * r + e] = p[4 * r + e] * fmaf(G[4 * r + e] + og[e], vsc, -dl[e]) * q4[e];
+        for (int r = 0; r < 4; ++r) {
+          const f32x4 og = swap[((wave ^ 1) * 8 + r) * 64 + lane];
+          const f32x4 q4 = *reinterpret_cast<const f32x4*>(sc + 32 * mp + 8 * r + 4 * g), dl = *reinterpret_cast<const f32x4*>(sc + 128 + 32 * mp + 8 * r + 4 * g);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[4 * r + e] = p[4 * r + e] * fmaf(G[4 * r + e] + og[e], vsc, -dl[e]) * q4[e];
+        }
       }
       split16_scaled<NB>(x, unit_k, dK, w);
       cols_dot<HD, NB>(img + mp * 4 * HD, 0, 2 * HD, w, lane, dK);
