@@ -735,7 +735,7 @@ __device__ __forceinline__ void bwd_sums(const Args& a, const Sums& m, int blk) 
 
 // dS = p (G - delta), delta the row's mean of G under p.  delta comes from the outputs (do . o: rows as long as one likes, one number), which is off by
 // the rounding of o; where one key holds nearly all of the weight G - delta cancels down to that.  Rows that see 32 keys at most — a session's
-// first rows, short sessions — take the mean of the very G that it is taken from: a row with one key has a gradient of exactly zero.
+// first rows, short sessions — take the mean of the very G - delta in a second step: a row with one key has a gradient of exactly zero.
 // ---- backward, dQ: the owner is a query; both maps need G^T = V dO^T, each wave makes it over half of V's columns and they swap halves ------
 // STAGES: two where two workgroups with two chunk buffers fit a CU's LDS (HD 32), else one: the other workgroup's products run under the copy.
 template <int HD> constexpr int bwd_stages() { return HD == 32 ? 2 : 1; }
@@ -819,31 +819,33 @@ __device__ __forceinline__ void bwd_dq(const Args& a, unsigned char* smem, int b
       float x[16];
       const bool edge = left < CH || (a.causal && t0 + 31 > q0 + off);
       const int last = a.causal ? min(qi + off - t0, left - 1) : left - 1;
-      float mean = dl;
       if ((a.causal ? min(nk, q0 + 32 + off) : nk) <= CH) {      // the only chunk that these rows see
-        float sum = 0.f, d = 0.f;
+        float sum = 0.f, mean = 0.f;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const bool ok = reg_row(r, g) <= last && sc[64 + reg_row(r, g)] != -INFINITY;
           x[r] = ok ? __builtin_amdgcn_exp2f(fmaf(S[r] * sc[32 * mp + reg_row(r, g)], qsc, -lse)) : 0.f;
+          G[r] = fmaf(G[r] + swap[((wave ^ 1) * 4 + (r >> 2)) * 64 + lane][r & 3], sc[96 + reg_row(r, g)], -dl);
           sum += x[r];
         }
         sum += __shfl_xor(sum, 32, 64);
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          if (x[r] > 0.f) d = fmaf(x[r] / sum, (G[r] + swap[((wave ^ 1) * 4 + (r >> 2)) * 64 + lane][r & 3]) * sc[96 + reg_row(r, g)], d);
+          if (x[r] > 0.f) mean = fmaf(x[r] / sum, G[r], mean);
           __builtin_amdgcn_sched_barrier(0);      // (one key after the other: few registers)
         }
-        d += __shfl_xor(d, 32, 64);
-        mean = sum > 0.f ? d : dl;
-      }
+        mean += __shfl_xor(mean, 32, 64);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const f32x4 other = swap[((wave ^ 1) * 4 + r) * 64 + lane];
-        const f32x4 k4 = *reinterpret_cast<const f32x4*>(sc + 32 * mp + 8 * r + 4 * g), v4 = *reinterpret_cast<const f32x4*>(sc + 96 + 8 * r + 4 * g);
+        for (int r = 0; r < 16; ++r) x[r] *= (G[r] - mean) * sc[32 * mp + reg_row(r, g)];
+      } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          x[4 * r + e] = __builtin_amdgcn_exp2f(fmaf(S[4 * r + e] * k4[e], qsc, -lse)) * fmaf(G[4 * r + e] + other[e], v4[e], -mean) * k4[e];
+        for (int r = 0; r < 4; ++r) {
+          const f32x4 other = swap[((wave ^ 1) * 4 + r) * 64 + lane];
+          const f32x4 k4 = *reinterpret_cast<const f32x4*>(sc + 32 * mp + 8 * r + 4 * g), v4 = *reinterpret_cast<const f32x4*>(sc + 96 + 8 * r + 4 * g);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            x[4 * r + e] = __builtin_amdgcn_exp2f(fmaf(S[4 * r + e] * k4[e], qsc, -lse)) * fmaf(G[4 * r + e] + other[e], v4[e], -dl) * k4[e];
+        }
       }
       if (edge) {
 #pragma unroll
@@ -976,7 +978,7 @@ __device__ __forceinline__ void bwd_dkv(const Args& a, unsigned char* smem, int 
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const bool ok = kok && (!a.causal || t0 + reg_row(r, g) + off >= ki);
-          const float sum = group_sum<32>(ok ? p[r] : 0.f), gr = (G[r] + swap[((wave ^ 1) * 8 + (r >> 2)) * 64 + lane][r & 3]) * vsc;
+          const float sum = group_sum<32>(ok ? p[r] : 0.f), gr = fmaf(G[r] + swap[((wave ^ 1) * 8 + (r >> 2)) * 64 + lane][r & 3], vsc, -sc[128 + 32 * mp + reg_row(r, g)]);
           x[r] = p[r] * (gr - group_sum<32>(ok && sum != 0.f ? p[r] / sum * gr : 0.f)) * sc[32 * mp + reg_row(r, g)];
           __builtin_amdgcn_sched_barrier(0);      // (one row after the other: few registers)
         }
@@ -1208,21 +1210,22 @@ __global__ __launch_bounds__(NT, R > 4 ? 1 : 2) void diff_decode_kernel(Args a) 
 }
 
 // ---- lam = exp(q1 . k1) - exp(q2 . k2) + init, one wave per head ----------------------------------------------------------------------------
-__device__ __forceinline__ float wave_dot(const float* x, const float* y, int n, int lane) {
-  float s = 0.f;
-  for (int c = lane; c < n; c += 64) s = fmaf(x[c], y[c], s);
-  return wave_sum(s);
+// In 64 bits: the difference of the two exponentials is all that is left of them (a head of few columns lost 2e-7 of lam; the time is the launch)
+__device__ __forceinline__ double wave_dot(const float* x, const float* y, int n, int lane) {
+  double s = 0.0;
+  for (int c = lane; c < n; c += 64) s += (double)x[c] * (double)y[c];
+  return wave_sum_d(s);
 }
 __global__ __launch_bounds__(64) void diff_lambda_fwd_kernel(const float* q1, const float* k1, const float* q2, const float* k2, float init, int hd, float* lam) {
   const long long o = (long long)blockIdx.x * hd;
-  const float e1 = expf(wave_dot(q1 + o, k1 + o, hd, threadIdx.x)), e2 = expf(wave_dot(q2 + o, k2 + o, hd, threadIdx.x));
-  if (threadIdx.x == 0) lam[blockIdx.x] = e1 - e2 + init;
+  const double e1 = exp(wave_dot(q1 + o, k1 + o, hd, threadIdx.x)), e2 = exp(wave_dot(q2 + o, k2 + o, hd, threadIdx.x));
+  if (threadIdx.x == 0) lam[blockIdx.x] = (float)(e1 - e2 + (double)init);
 }
 __global__ __launch_bounds__(64) void diff_lambda_bwd_kernel(const float* dlam, const float* q1, const float* k1, const float* q2, const float* k2, int hd,
                                                              float* dq1, float* dk1, float* dq2, float* dk2) {
   const long long o = (long long)blockIdx.x * hd;
   const float g = dlam[blockIdx.x];
-  const float e1 = g * expf(wave_dot(q1 + o, k1 + o, hd, threadIdx.x)), e2 = -g * expf(wave_dot(q2 + o, k2 + o, hd, threadIdx.x));
+  const float e1 = (float)(g * exp(wave_dot(q1 + o, k1 + o, hd, threadIdx.x))), e2 = (float)(-g * exp(wave_dot(q2 + o, k2 + o, hd, threadIdx.x)));
   for (int c = threadIdx.x; c < hd; c += 64) {
     dq1[o + c] = e1 * k1[o + c];
     dk1[o + c] = e1 * q1[o + c];

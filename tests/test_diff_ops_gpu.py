@@ -331,6 +331,67 @@ def test_attention_split_keys(rows, keys, hd):
     _attention_case([rows, 1], [keys, 3], 2, 1, hd, False, train=False)
 
 
+@pytest.mark.parametrize("hd", [4, 32, 64])
+@pytest.mark.parametrize("H,Hkv", [(2, 2), (4, 2)])
+def test_attention_rows_of_one_key_have_no_gradient(hd, H, Hkv):
+    """One visible key: its weight is 1 whatever the logits are, dS is exactly zero.  First rows of causal sessions, sessions of one row, one key left
+    by the mask."""
+    ops, dev = _ops(), _dev()
+    g = torch.Generator().manual_seed(hd)
+    lens = [1, 5, 40, 1]
+    cu = _cu(lens).to(dev)
+    q, k, v = (torch.randn(47, n * 2 * hd, generator=g).to(dev).requires_grad_() for n in (H, Hkv, Hkv))
+    lam, w = torch.full((H,), 0.4, device=dev), torch.rand(2 * hd, generator=g).to(dev) + 0.5
+    gy = torch.randn(47, H * 2 * hd, generator=g).to(dev)
+    y = ops.diff_attention(q, k, v, lam, cu, cu, 4, H, Hkv, 40, 40, True, norm_w=w)
+    dq, dk, _ = torch.autograd.grad(y, (q, k, v), gy)
+    assert not dq[[0, 1, 6, 46]].any() and dq[[2, 7, 45]].any(1).all() and not dk[[0, 46]].any()
+    ids = torch.zeros(47, dtype=torch.int64)
+    ids[[9, 46]] = 1
+    y = ops.diff_attention(q, k, v, lam, cu, cu, 4, H, Hkv, 40, 40, False, key_ids=ids.to(dev), norm_w=w)
+    dq, dk, _ = torch.autograd.grad(y, (q, k, v), gy)
+    assert not dq[46].any() and not dk[46].any() and not dq[:6].any()      # (the 40 rows' session is longer than a chunk: rounding)
+
+
+@pytest.mark.parametrize("H,Hkv", [(1, 1), (4, 2)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_attention_short_sessions_with_one_heavy_key(H, Hkv, causal):
+    """Nearly all of the weight on one key h: dS_j = p_j (G_j - sum p G) cancels there to sum over the others of p_j (G_h - G_j), and the gradient of
+    q is held to the size of that."""
+    ops, dev = _ops(), _dev()
+    g = torch.Generator().manual_seed(5)
+    hd, lens = 32, [2, 3, 9, 30]
+    n, sc = sum(lens), 1.0 / math.sqrt(hd)
+    q, k, v = (torch.randn(n, c * 2 * hd, generator=g) for c in (H, Hkv, Hkv))
+    k = k * 0.02
+    k[[0, 2, 5, 14]] = 1.0                 # the first key of every session, seen by all of its rows
+    q = q * 0.1 + 1.5                      # logits of about 1.5 * 32 / sqrt(32) = 8.5 there, 0 at the others: weights e^-8.5
+    lam = torch.full((H,), 0.4)
+    gy = torch.randn(n, H * 2 * hd, generator=g)
+    want, top, _ = _attention_ref(q, k, v, lam, lens, lens, H, Hkv, causal, None, None, 1.0, 1e-5, gy)
+    qd, kd, vd = (t.to(dev).requires_grad_() for t in (q, k, v))
+    cu = _cu(lens).to(dev)
+    y = ops.diff_attention(qd, kd, vd, lam.to(dev), cu, cu, 4, H, Hkv, 30, 30, causal)
+    dq = torch.autograd.grad(y, qd, gy.to(dev))[0].cpu().double()
+    # a weight is off by 2 d + 8 u relative (d: its logit), G by (3 * 2 hd + 12) u of |dO| |v| (no norm: dO = dy), the mean over the keys and the product
+    # with k by (4 * 32 + 16) u: all of them of terms p_j (|G_j| + |G_h|) (|k_j| + |k_h|), j not h
+    k_ = 2 * (2 * (3 * hd + 12) * U * top + 8 * U) + (6 * hd + 12 + 4 * 32 + 16) * U
+    at = 0
+    for m in lens:
+        see = torch.ones(m, m, dtype=torch.bool).tril() if causal else torch.ones(m, m, dtype=torch.bool)
+        for h in range(H):
+            hk = h // (H // Hkv)
+            G = gy[at:at + m, h * 2 * hd:(h + 1) * 2 * hd].double().abs() @ v[at:at + m, hk * 2 * hd:(hk + 1) * 2 * hd].double().abs().T
+            for mp in (0, 1):
+                c, ck = (slice((2 * x + mp) * hd, (2 * x + mp + 1) * hd) for x in (h, hk))
+                K = k[at:at + m, ck].double()
+                p = torch.softmax((q[at:at + m, c].double() @ K.T * sc).masked_fill(~see, -math.inf), 1)
+                allowed = ((p[:, 1:] * (G[:, 1:] + G[:, :1]))[..., None] * (K[1:].abs() + K[:1].abs())).sum(1) * sc * (1.0 if mp == 0 else 0.4)
+                err = (dq[at:at + m, c] - want["dq"][0][at:at + m, c]).abs()
+                assert (err <= k_ * allowed).all(), (m, h, mp, float((err / (k_ * allowed + 1e-300)).max()))
+        at += m
+
+
 @pytest.mark.parametrize("hd", [32, 50, 64])
 def test_attention_long_causal_sessions(hd):
     """Few long sessions: two halves of the keys per workgroup; odd counts of chunks, a session without rows, one of a single chunk."""
