@@ -8,7 +8,8 @@
 //
 // Memory bound: every column is read and written once.  The sine and cosine of a (row, pair) are shared by all heads of q AND k: a thread
 // keeps them for up to 4 heads of its pairs (64-bit product, reduction and sincos are about 50 operations a pair; at one head per thread
-// they would cost as much issue time as the memory traffic).  With few rows the heads go to threads of their own instead: latency counts there.
+// they cost as much issue time as the memory traffic).  65,536 rows, 16 + 4 heads of 64 columns, 32 of them turned, interleaved: 135 us = 5.0 TB/s
+// (one head per thread: 201 us).  With few rows the heads go to threads of their own instead: latency counts there.
 #include "rt_common.h"
 
 namespace {
@@ -109,8 +110,9 @@ extern "C" int rt_rotary(const float* q, int64_t ldq, float* q_out, int64_t ldq_
     if (s.heads > 0) vec = vec && (((uintptr_t)s.x | (uintptr_t)s.y) & 15u) == 0 && s.ldx % 4 == 0 && s.ldy % 4 == 0;
   const int V = vec ? 4 : 1;
   a.units = rot / 2 / V + (hd - rot) / V;
-  // up to 4 heads per thread once the rows alone fill the machine (256 CUs x 2,048 threads), else one
-  a.groups = (M * a.units * heads > 4LL * 256 * 2048) ? (heads + 3) / 4 : heads;
+  // up to 4 heads per thread where one per thread would be more threads than the machine holds (2,048 per CU): 17,920 rows of 8 + 8 heads of 32 14.4 us
+  // (one: 15.4), 64 such rows 4.2 us (one: 3.6)
+  a.groups = M * a.units * heads > 2048LL * rt_num_cus() ? (heads + 3) / 4 : heads;
   const long long T = (long long)a.groups * a.units;
   if (T > 0x7FFFFFFF) return RT_ERR_INVALID_ARG;
   a.rows_per_wg = T <= 256 ? (int)(256 / T) : 1;
