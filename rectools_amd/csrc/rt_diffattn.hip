@@ -9,9 +9,10 @@
 //
 // Arithmetic: fp32 in, fp32 out.  A product runs on the fp16 matrix instruction as three terms of a two-way split: x = 2^e (h + l), e from the
 // largest magnitude of the row, h = fp16(x 2^-e), l = fp16 of the rest; x y ~ h h' + h l' + l h'.  h and l hold 11 bits each and a sign, so x
-// is held to 2^-22 of its row's largest value and the dropped l l' is below 2^-22 of the product: rounding of the size fp32 sums of
-// this length carry themselves (measured against 64 bits: DESIGN of the tests).  Three bf16 planes, the exact split, need six terms: twice the matrix work, 1.5 x the
-// LDS traffic and the registers (the dK/dV kernel spilled 263 registers at hd 64), and were measured 1.9 - 2.6 x slower.
+// is held to 2^-23 of itself (values below 2^-17 of their row's largest: to 2^-38 of that) and the dropped l l' is below 2^-22 of the product: roundings
+// of the size that fp32 sums of this length carry themselves — over 150 drawn training calls the error against 64 bits is 0.9 x that of the same
+// formulas in fp32 tensors (median; outputs, dq, dk, dv).  Three bf16 planes, the exact split, take six terms: two sessions of 4,096 rows, 4 heads of hd 64,
+// forward and backward 1,840 us with them, 1,100 with these.
 // The split is made ONCE per call by diff_planes_kernel (one pass over q, k, v: memory bound), not at every staging: a 4,096-row session
 // stages each of its rows 64 times.  Softmax statistics, sums and accumulators are fp32; scores live in the base-2 domain.
 //
@@ -22,6 +23,10 @@
 // lie by LDS DMA (global_load_lds: no registers, no address arithmetic): the planes are stored head-major with 48 bytes behind every row, so
 // rows lie 3 sixteen-byte units apart modulo the 256 bytes of the banks: 32 rows of 16 bytes without a conflict, 4-row transpose blocks two-way (with 16
 // bytes behind them: four-way, 192 conflict cycles per wave and chunk of the forward pass).
+//
+// What bounds it (two sessions of 4,096, 4 heads of hd 64, causal): forward 215 us, backward 510 us.  Least matrix work, three terms each, at the rate a large
+// 16-bit matrix product reaches on this card (1,385 TFLOP/s): 112 and 260 us.  Counters: the matrix pipe is busy 36 - 38 % of the time, the vector
+// pipe 43 % (exponentials, scales, splits), and the two waves of a SIMD overlap them little; two waves are what 256 registers each leave.
 #include "rt_attn_planes.h"
 
 namespace {
@@ -165,7 +170,8 @@ __device__ __forceinline__ void put_planes(unsigned char* p, int plane, f32x4 x,
 }
 __device__ __forceinline__ float top4(f32x4 x) { return fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))); }
 
-// q, k and v -> planes and scales: HD / 2 lanes per (row, head), four columns each; blocks [0, q_blocks) q, then k, then v
+// q, k and v -> planes and scales: HD / 2 lanes per (row, head), four columns each; blocks [0, q_blocks) q, then k, then v.  Memory bound: 8,192 rows of 4
+// heads of hd 64, 50 MB in and 55 MB out, 19.5 us = 5.4 TB/s; 14,381 rows of 4 heads of hd 32 19 us = 5.1 TB/s.
 template <int HD, int MODE>
 __global__ __launch_bounds__(NT) void diff_planes_kernel(Args a, unsigned q_blocks, unsigned kv_blocks) {
   constexpr int LANES = HD / 2, GROUPS = NT / LANES;
@@ -341,7 +347,8 @@ __device__ __forceinline__ void row_norm(float base, float total, float& n, floa
 // Heavy tiles first (causal: a session's last queries, its first keys): where the launch is many times the machine, the light ones fill the gaps
 // at its end.
 // Workgroups go to the eight dies in turn and each die has its own 4 MB of L2: with the (session, head) pairs counted in a multiple of eight (`bhs`:
-// rounded up where there are many), all tiles of a pair, which stream the same chunks, meet on one die.
+// rounded up where there are many), all tiles of a pair, which stream the same chunks, meet on one die (forward, 33 sessions of 1,000, 3 heads of hd 64: 384 ->
+// 365 us; 7 of 2,000, 11 heads: 974 -> 911).
 struct Work { int tile, b, h, split; bool any; };
 __device__ __forceinline__ Work work_of(const Args& a, const Grid& n, int blk, int H, bool last_first) {
   const int real = n.bhs * n.n_tiles, bh = blk % n.bhs, o = blk / n.bhs;
@@ -595,7 +602,7 @@ __global__ __launch_bounds__(KH * NT, HD == 32 && KH == 1 ? 3 : 2) void diff_fwd
 }
 
 // join of the key splits: one workgroup per (row, head); a lane holds the statistics of a split (n_split <= 64), then a thread sums one value
-// column over its share of the splits
+// column over its share of the splits.  8 rows of 8 heads, 32 splits: 8 us, two dependent reads of memory
 __global__ __launch_bounds__(NT) void diff_combine_kernel(Args a) {
   __shared__ float wgt[2][64], sums[NT], res[2][128], ssq[2];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, dv = 2 * a.hd;
@@ -645,7 +652,9 @@ __global__ __launch_bounds__(NT) void diff_combine_kernel(Args a) {
 
 // ---- backward, in front: gradient of o (as planes), delta_m = do . o_m, and the sums behind dlam and dw --------------------------------------
 // HD / 2 lanes per (row, head), four columns each; a lane group keeps its head, so dlam and dw stay in registers over all of its rows.  They
-// are summed in 64 bits, per workgroup, in a fixed order.
+// are summed in 64 bits, per workgroup, in a fixed order.  do stands at right angles to o (but for eps) and do . o_m is what is left of that: formed in
+// 64 bits, from the outputs as they are (in 32 the gradient of lam was 2 - 5 x further off; 15.5 -> 17 us).  Memory bound: 8,192 rows of 4 heads of hd 64,
+// 70 MB, 18 us = 3.9 TB/s.
 constexpr int PRE_WG = 1024;      // workgroups at most: the partials are [PRE_WG][H + 2 hd] doubles
 
 template <int HD, int MODE>
@@ -737,7 +746,8 @@ __device__ __forceinline__ void bwd_sums(const Args& a, const Sums& m, int blk) 
 // the rounding of o; where one key holds nearly all of the weight G - delta cancels down to that.  Rows that see 32 keys at most — a session's
 // first rows, short sessions — take the mean of the very G - delta in a second step: a row with one key has a gradient of exactly zero.
 // ---- backward, dQ: the owner is a query; both maps need G^T = V dO^T, each wave makes it over half of V's columns and they swap halves ------
-// STAGES: two where two workgroups with two chunk buffers fit a CU's LDS (HD 32), else one: the other workgroup's products run under the copy.
+// STAGES: two where two workgroups with two chunk buffers fit a CU's LDS (HD 32; training passes with two | with one: 128 sessions of 200 285 | 290 us,
+// 16 of 2,048 1,021 | 1,028), else one: the other workgroup's products run under the copy.
 template <int HD> constexpr int bwd_stages() { return HD == 32 ? 2 : 1; }
 template <int HD> constexpr int dkv_stage() { return 2 * Row<HD>::CHUNK + 1024; }
 template <int HD> constexpr int bwd_lds() { return bwd_stages<HD>() * dkv_stage<HD>() + 4 * 8 * 64 * 16; }      // (dQ needs less)
@@ -1023,7 +1033,8 @@ __device__ __forceinline__ void bwd_dkv(const Args& a, unsigned char* smem, int 
 }
 
 // Both passes in one launch, the dK/dV workgroups (one and a half times the work of the others) first: they share no data, and each alone ends with
-// a few of its longest workgroups on an empty machine.  One launch after the other took 309 + 445 us (two sessions of 4,096, 4 heads of hd 64, causal).
+// a few of its longest workgroups on an empty machine.  Two sessions of 4,096, 4 heads of hd 64, causal: 510 us = 3.6e11 flops (three terms a product) at
+// 710 TFLOP/s; one launch after the other 309 + 445 us before the later steps, together 562.  The column sums of dlam and dw ride along between the two.
 template <int HD>
 __global__ __launch_bounds__(NT, 2) void diff_bwd_kernel(Args a, Sums m) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
@@ -1038,7 +1049,9 @@ __global__ __launch_bounds__(NT, 2) void diff_bwd_kernel(Args a, Sums m) {
 // into registers: a key's two maps (and its value row) lie across 2 HD / 4 lanes, four columns each, so every load is whole cache lines; a
 // dot product is four multiply-adds and a sum over the lanes of its map (cross-lane adds, no LDS), the two maps' lanes swap their probabilities, the value
 // sums stay with the lanes' columns.  Every lane group keeps its own running maximum and sum until the end; no barrier in the loop, and the
-// next TK keys are read while these are taken.
+// next TK keys are read while these are taken.  1,024 sessions of up to 200 keys, 4 heads of hd 32, one query each: 43 us = 6.1 TB/s (memory bound);
+// 8 sessions of up to 65,536, 4 queries to each of 2 key heads of hd 64: 166 us = 3.9 TB/s, the vector pipe (a key costs a query 4 multiply-adds, 5
+// cross-lane adds and 2 exponentials).  R is the next power of two: instances for 1, 2, 4, 8, so that one query pays for one.
 constexpr int MAXR = 8;
 
 template <int HD> __device__ __forceinline__ float other_map(float v) {
