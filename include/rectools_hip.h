@@ -759,7 +759,7 @@ int rt_diff_lambda_bwd(const float* dlam, const float* q1, const float* k1, cons
 
 /* Differential attention: o = (softmax(scale q1 k1^T) - lam_h softmax(scale q2 k2^T)) v, y = out_scale * norm_w * o / sqrt(mean(o^2) + eps)
  * (norm_w null: y = out_scale * o).  q [Nq, H][2][hd], k [Nk, Hkv][2][hd], v [Nk, Hkv][2 hd], y [Nq, H][2 hd] (row strides ld*); query head h
- * reads key head h / (H / Hkv); hd <= 64.  cu_q / cu_k [B+1] (first 0, ascending): first row of every session, or null: B sessions of Lq / Lk
+ * reads key head h / (H / Hkv); hd <= 64, Nq, Nk < 2^30, eps > 0 with norm_w.  cu_q / cu_k [B+1] (first 0, ascending): first row of every session, or null: B sessions of Lq / Lk
  * rows (then Nq == B * Lq, Nk == B * Lk).  With cu, Lq / Lk are the expected longest sessions (longer ones are served all the same).  The last
  * query of a session is aligned with its last key: causal = key j is seen by query i iff j <= i + nk - nq.  key_ids (null or [Nk]): keys with id 0
  * are masked.  A query that sees no key gives 0.  scale <= 0: 1 / sqrt(hd).  Rows behind the last session of cu_q are written as zeros.
@@ -780,7 +780,7 @@ int rt_diffattn_bwd(const void* saved, size_t saved_bytes, const float* lam, con
                     float* dlam, float* dw, void* ws, size_t ws_bytes, rt_stream_t stream);
 
 /* The norm behind a block, its gate, its residual scale and the norm in front of the next block: n = N_post(f), y = alpha x + scale * sigmoid(z) *
- * drop(n), h = N_pre(y) over contiguous [M, d] rows, d <= 8192.  layer = 1: LayerNorm, 0: root mean square.  post_w / pre_w null: that norm is left
+ * drop(n), h = N_pre(y) over contiguous [M, d] rows, d <= 8192, eps > 0.  layer = 1: LayerNorm, 0: root mean square.  post_w / pre_w null: that norm is left
  * out (h null iff pre_w null); post_b, pre_b, z, scale null: left out.  p, seed, stream_id: the dropout mask of rt_act_dropout_*.  stat [M, 4]
  * (16-byte aligned, null without a backward pass): the norms' statistics.  Backward: gy / gh may be null (no gradient); dscale .. dpre_b: the ones that
  * are asked for. */

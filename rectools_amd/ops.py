@@ -2605,7 +2605,9 @@ def diff_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam: torch
     cu_q / cu_k [B + 1] int64: first row of every session (first 0, ascending), with Lq / Lk the longest sessions expected (plans the
     launch; longer ones are served).  None: B sessions of exactly Lq / Lk rows.  The last query of a session meets its last key: with
     causal, key j is seen by query i iff j <= i + nk - nq — so Lq = 1 is the newest row of a stored session.  key_ids [Nk] int64: keys with
-    id 0 are masked, whatever their rows hold.  A query that sees no key gives zeros; so do rows behind the last session of cu_q."""
+    id 0 are masked, whatever their rows hold.  A query that sees no key gives zeros; so do rows behind the last session of cu_q.  eps and
+    scale (None: 1 / sqrt(hd)) are positive.  No second derivative; a backward pass is not captured into a graph while a graph made on the
+    default stream holds the same leaf tensors (refused)."""
     return _native_op("diff_attention", q, k, v, lam, cu_q, cu_k, B, H, H_kv, Lq, Lk, causal, key_ids, norm_w, out_scale, eps, scale)
 
 
@@ -2618,7 +2620,7 @@ def norm_gate_residual(x: torch.Tensor, f: torch.Tensor, gate: tp.Optional[torch
     """One pass over the rows between two blocks: y = alpha x + scale * sigmoid(gate) * dropout(N_post(f)), h = N_pre(y) -> (y, h).
     x (residual stream), f (the block's output), gate (logits) [M, d]; scale [d] (a learned residual scale); post / pre = (weight [d], bias
     [d] or None) of the norm behind this block and the one in front of the next; kind "rms" (root mean square) or "layer" (LayerNorm).  Any of
-    gate, post, scale, pre may be None (h is None without pre).  d <= 8192."""
+    gate, post, scale, pre may be None (h is None without pre).  d <= 8192, eps > 0."""
     if kind not in ("rms", "layer"):
         raise ValueError(f"norm_gate_residual: kind is 'rms' or 'layer', got {kind!r}")
     if not 0.0 <= p < 1.0:
