@@ -239,6 +239,50 @@ def test_operators_on_another_stream():
     assert torch.equal(got, want)
 
 
+def test_operators_from_two_threads_on_two_streams():
+    """Passes of different shapes at the same time, each with its own buffers: the same bits as alone."""
+    import threading
+
+    from rectools_amd import ops
+
+    freq, _ = ops.rotary_frequencies(16, device="cuda")
+
+    def make(seed, n, L, H):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        q, k, v, up = (torch.randn(n * L, H * 64, generator=g, device="cuda") for _ in range(4))
+        lam, w = torch.full((H,), 0.3, device="cuda"), torch.rand(H * 64, generator=g, device="cuda")
+        pos = torch.arange(L, device="cuda").repeat(n)
+
+        def step():
+            ts = [t.detach().requires_grad_() for t in (q, k, v)]
+            a, b = ops.rotary_qk(ts[0], ts[1], pos, freq, 2 * H, 2 * H)
+            o = ops.diff_attention(a, b, ts[2], lam, None, None, n, H, H, L, L, True)
+            y, h = ops.norm_gate_residual(o, ts[2], gate=ts[0], post=(w, None), pre=(w, None))
+            return (y.detach(), h.detach()) + torch.autograd.grad((y, h), ts, (up, up))
+
+        return step
+
+    steps = [make(1, 3, 700, 2), make(2, 40, 90, 1)]
+    want = [s() for s in steps]
+    torch.cuda.synchronize()
+    got = [[], []]
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(6):
+                got[i].append(steps[i]())
+        stream.synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for g, w in zip(got, want):
+        assert len(g) == 6 and all(torch.equal(a, b) for out in g for a, b in zip(out, w))
+
+
 def test_no_second_derivative():
     from rectools_amd import ops
 
