@@ -984,22 +984,32 @@ __device__ __forceinline__ void bwd_dkv(const Args& a, unsigned char* smem, int 
       if (!on) continue;
       float x[16];
       P2 w[2];
-      if ((a.causal ? min(nk, t0 + 32 + off) : nk) <= CH) {      // rows that see no other keys than the wave's
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
+      const bool few = (a.causal ? min(nk, t0 + 32 + off) : nk) <= CH;      // rows that see no other keys than the wave's
+      if (few) {
+        const float* own = reinterpret_cast<const float*>(swap + wave * 8 * 64 + lane);
+        const float* other = reinterpret_cast<const float*>(swap + (wave ^ 1) * 8 * 64 + lane);
+#pragma unroll 1
+        for (int r = 0; r < 16; ++r) {      // (a loop: unrolled it costs the kernel registers that it has not got)
+          const int at = (r >> 2) * 256 + (r & 3), row = 32 * mp + reg_row(r, g);
           const bool ok = kok && (!a.causal || t0 + reg_row(r, g) + off >= ki);
-          const float sum = group_sum<32>(ok ? p[r] : 0.f), gr = fmaf(G[r] + swap[((wave ^ 1) * 8 + (r >> 2)) * 64 + lane][r & 3], vsc, -sc[128 + 32 * mp + reg_row(r, g)]);
-          x[r] = p[r] * (gr - group_sum<32>(ok && sum != 0.f ? p[r] / sum * gr : 0.f)) * sc[32 * mp + reg_row(r, g)];
-          __builtin_amdgcn_sched_barrier(0);      // (one row after the other: few registers)
+          const float pr = ok ? own[1024 + at] : 0.f, sum = group_sum<32>(pr), gr = fmaf(own[at] + other[at], vsc, -sc[128 + row]);
+          const float mean = group_sum<32>(ok && sum != 0.f ? pr / sum * gr : 0.f);
+          if (i == 0) sc[64 + row] = mean;      // (where the exponents were: read above, by this wave alone)
         }
-      } else {
+      }
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const f32x4 og = swap[((wave ^ 1) * 8 + r) * 64 + lane];
-          const f32x4 q4 = *reinterpret_cast<const f32x4*>(sc + 32 * mp + 8 * r + 4 * g), dl = *reinterpret_cast<const f32x4*>(sc + 128 + 32 * mp + 8 * r + 4 * g);
+      for (int r = 0; r < 4; ++r) {
+        const f32x4 og = swap[((wave ^ 1) * 8 + r) * 64 + lane];
+        const f32x4 q4 = *reinterpret_cast<const f32x4*>(sc + 32 * mp + 8 * r + 4 * g), dl = *reinterpret_cast<const f32x4*>(sc + 128 + 32 * mp + 8 * r + 4 * g);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) x[4 * r + e] = p[4 * r + e] * fmaf(G[4 * r + e] + og[e], vsc, -dl[e]) * q4[e];
+        for (int e = 0; e < 4; ++e) G[4 * r + e] = fmaf(G[4 * r + e] + og[e], vsc, -dl[e]);
+        if (few) {
+          const f32x4 m4 = *reinterpret_cast<const f32x4*>(sc + 64 + 32 * mp + 8 * r + 4 * g);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) G[4 * r + e] -= m4[e];
         }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[4 * r + e] = p[4 * r + e] * G[4 * r + e] * q4[e];
       }
       split16_scaled<NB>(x, unit_k, dK, w);
       cols_dot<HD, NB>(img + mp * 4 * HD, 0, 2 * HD, w, lane, dK);
