@@ -1233,7 +1233,7 @@ __global__ __launch_bounds__(NT, R > 4 ? 1 : 2) void diff_decode_kernel(Args a) 
 }
 
 // ---- lam = exp(q1 . k1) - exp(q2 . k2) + init, one wave per head ----------------------------------------------------------------------------
-// In 64 bits: the difference of the two exponentials is all that is left of them (a head of few columns lost 2e-7 of lam; the time is the launch)
+// In 64 bits: the difference of the two exponentials is all that is left of them (a head of few columns lost 2e-7 of lam).  1.8 us, 4.6 behind a kernel that has emptied the caches
 __device__ __forceinline__ double wave_dot(const float* x, const float* y, int n, int lane) {
   double s = 0.0;
   for (int c = lane; c < n; c += 64) s += (double)x[c] * (double)y[c];

@@ -536,7 +536,7 @@ def test_attention_same_bits_twice_and_gradient_against_differences():
 def test_diff_lambda():
     ops, dev = _ops(), _dev()
     g = torch.Generator().manual_seed(2)
-    for H, hd in ((1, 1), (4, 32), (3, 65), (8, 200)):
+    for H, hd in ((1, 1), (4, 32), (3, 65), (8, 200), (37, 16)):
         vs = [(torch.randn(H, hd, generator=g) * 0.2) for _ in range(4)]
         ds = [t.to(dev).requires_grad_() for t in vs]
         lam = ops.diff_lambda(*ds, 0.35)
