@@ -62,7 +62,7 @@ struct Args {
   float* o12;                            // [Nq, H, 2, 2 hd] normalised outputs of the two maps (training)
   float* lse; float* lsf;                // [H][2][Nq + PAD] of the two maps (training): probability = exp2(s - lse) lsf, lse a whole number
   float* part; float* ml;                // split keys: [n_split, Nq, H, 2, 2 hd] and [n_split, Nq, H, 2, 2] (maximum, sum)
-  int n_split;
+  int n_split, share;                    // share (diff_decode_kernel): TK-key tiles of a split at least; 0: sessions of one length
   Grid own_q, own_k;                     // launches whose owner rows are queries / keys
   // backward
   float* delta; float* dc;               // [H][2][Nq + PAD]: do . o_m 2^-e, e of dO's row; what turns exp2(s - lse) into the map's weight on dO's plane
@@ -630,7 +630,11 @@ __global__ __launch_bounds__(NT) void diff_combine_kernel(Args a) {
           v[k] = s < a.n_split ? a.part[(((long long)s * plane + at) * 2 + mp) * dv + c] : 0.f;
         }
 #pragma unroll
-        for (int k = 0; k < 8; ++k) x = fmaf(v[k], wgt[mp][min(s0 + k * slots, 63)], x);
+        for (int k = 0; k < 8; ++k) {
+          const float w = wgt[mp][min(s0 + k * slots, 63)];
+          if (a.share > 0) v[k] = w != 0.f ? v[k] : 0.f;      // (an empty share's sums were not written)
+          x = fmaf(v[k], w, x);
+        }
       }
     sums[tid] = x;
     __syncthreads();
@@ -1083,9 +1087,9 @@ __global__ __launch_bounds__(NT, R > 4 ? 1 : 2) void diff_decode_kernel(Args a) 
   constexpr int DV = 2 * HD, LPK = HD / 2, KPL = 64 / LPK, NL = 4, TK = KPL * NL;
   __shared__ float wstat[4][R][2][2], wacc[4][R][2][DV];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, kk = lane / LPK, c4 = lane % LPK, mp = c4 / (HD / 4), cm = c4 % (HD / 4), col = cm * 4;
-  const int b = blockIdx.x / a.Hkv, hk = blockIdx.x % a.Hkv, rep = a.H / a.Hkv, hd = a.hd, dv = 2 * hd;
+  const int id = blockIdx.x, nbh = gridDim.x / a.n_split, split = a.share > 0 ? id % a.n_split : id / nbh, bh = a.share > 0 ? id / a.n_split : id % nbh, b = bh / a.Hkv, hk = bh % a.Hkv, rep = a.H / a.Hkv, hd = a.hd, dv = 2 * hd;
   if (b == a.B) {      // rows behind the last session: zeros
-    if (blockIdx.y != 0) return;
+    if (split != 0) return;
     const long long r0 = rows_used(a.cu_q, a.B, a.Nq), cols = (long long)rep * dv;
     for (long long x = tid; x < (a.Nq - r0) * cols; x += NT) a.y[(r0 + x / cols) * a.ldy + (long long)hk * rep * dv + x % cols] = 0.f;
     return;
@@ -1113,7 +1117,16 @@ __global__ __launch_bounds__(NT, R > 4 ? 1 : 2) void diff_decode_kernel(Args a) 
       l[w] = 0.f;
     }
     const int k_end = a.causal ? max(0, min(nk, first + rows + off)) : nk;
-    const int n_t = (k_end + TK - 1) / TK, each = (n_t + a.n_split - 1) / a.n_split, t_lo = min(n_t, (int)blockIdx.y * each), t_hi = min(n_t, t_lo + each);
+    const int n_t = (k_end + TK - 1) / TK, each = max(a.share, (n_t + a.n_split - 1) / a.n_split), t_lo = min(n_t, split * each), t_hi = min(n_t, t_lo + each);
+    if (a.share > 0 && split > 0 && t_lo >= n_t) {      // nothing left: an empty share (diff_combine_kernel does not read its sums)
+      for (int u = tid; u < 2 * rows * rep; u += NT) {
+        const int w = u >> 1;
+        const long long at = (((long long)split * a.Nq + qr0 + first + w / rep) * a.H + hk * rep + w % rep) * 2 + (u & 1);
+        a.ml[2 * at] = -INFINITY;
+        a.ml[2 * at + 1] = 0.f;
+      }
+      continue;
+    }
     const float* kbase = a.k + kr0 * a.ldk + (long long)(2 * hk + mp) * hd;
     const float* vbase = a.v + kr0 * a.ldv + (long long)hk * dv;
     struct Tile { f32x4 k[NL], v[NL]; unsigned live; };
@@ -1211,7 +1224,7 @@ __global__ __launch_bounds__(NT, R > 4 ? 1 : 2) void diff_decode_kernel(Args a) 
           if (DV > 64) s1 = fmaf(wacc[k][u][q][(lane + 64) % DV], e, s1);
         }
         if (a.n_split > 1) {
-          const long long at = (((long long)blockIdx.y * a.Nq + row) * a.H + h) * 2 + q;
+          const long long at = (((long long)split * a.Nq + row) * a.H + h) * 2 + q;
           if (lane == 0) { a.ml[2 * at] = mx; a.ml[2 * at + 1] = lt; }
           if (lane < dv) a.part[at * dv + lane] = s0;
           if (lane + 64 < dv) a.part[at * dv + lane + 64] = s1;
@@ -1261,7 +1274,7 @@ __global__ __launch_bounds__(64) void diff_lambda_bwd_kernel(const float* dlam, 
 bool vec_ok(const void* p, long long ld) { return ((uintptr_t)p & 15u) == 0 && ld % 4 == 0; }
 int pad_hd(int hd) { return hd <= 32 ? 32 : 64; }
 
-struct Plan { bool decode; int n_split; };
+struct Plan { bool decode; int n_split, share; };
 // Training keeps the outputs of both maps and always takes the matrix kernels.  Otherwise few queries to a key head (rows x heads of its group) go
 // through diff_decode_kernel, up to twelve of them, in two passes over the keys behind eight.  Decode against matrix, causal, hd 64, 2 key heads:
 //   1 query   8 x 65,536 keys 185 | 763 us   256 x 200 19 | 62     1 x 8,192 17 | 29
@@ -1271,19 +1284,26 @@ struct Plan { bool decode; int n_split; };
 // Keys are split over workgroups until the launch has what the machine holds at once, two per CU (decode of more than four queries: its registers
 // leave one), with 2 (decode) or 4 chunks each at least.  Decode, 64 sessions of 2,048 keys: 4 queries 52 us (1 per CU: 68, 4 per CU: 58), 8 queries
 // 105 (2: 114, 4: 133); matrix, 8 x 1,024 rows of 4 heads: 82 (1: 84, 4: 134).
-Plan plan_of(int B, int H, int Hkv, int hd, int Lq, int Lk, bool train) {
+// Decode over sessions of different lengths (their keys are below nine tenths of B x Lk): shares of one size instead of one number, so that a long session
+// has more workgroups and not longer ones, an eighth fewer than fit (a session's last share counts as one), a session's shares on different
+// dies.  Lengths of a long tail, one size | one number: 8 of up to 65,536 keys, 8 heads on 2 of hd 64 155 | 183 us; 300 of up to 1,000, one head of
+// hd 50 86 | 105; 100 of up to 2,000, 8 heads on 2 of hd 32 40 | 45; 32 of up to 8,192, 4 heads of hd 64 154 | 142.  Sessions of one length keep the order that
+// leaves a session's shares on one die (8 of 65,536: 194 us, spread out 204).
+Plan plan_of(int B, int H, int Hkv, int hd, int Lq, int Lk, long long Nk, bool train) {
   Plan p;
   const int rep = H / Hkv;
   const long long queries = (long long)rep * Lq;
   p.decode = !train && rep <= MAXR && queries <= MAXR + MAXR / 2;
   const long long wgs = p.decode ? (long long)B * Hkv : (long long)B * H * ((Lq + OWN - 1) / OWN);
-  const int chunk = p.decode ? 4 * decode_keys(pad_hd(hd)) : CH;      // keys a workgroup takes at once
+  const int tile = decode_keys(pad_hd(hd)), chunk = p.decode ? 4 * tile : CH;      // keys a workgroup takes at once
   const long long want = (long long)rt_num_cus() * (p.decode && queries > 4 ? 1 : 2);
-  long long s = wgs > 0 ? want / wgs : 1;
+  const bool ragged = p.decode && 10 * Nk < 9 * (long long)B * Lk && Nk > 0;
+  long long s = ragged ? want * 7 / 8 * Lk / (Nk * Hkv) : (wgs > 0 ? want / wgs : 1);
   const long long most = Lk / (p.decode ? 2 * chunk : 4 * chunk);
   if (s > most) s = most;
   if (s > 64) s = 64;
   p.n_split = s > 1 ? (int)s : 1;
+  p.share = ragged && p.n_split > 1 ? ((Lk + tile - 1) / tile + p.n_split - 1) / p.n_split : 0;
   return p;
 }
 size_t part_floats(const Plan& p, long long Nq, int H, int hd) {
@@ -1407,7 +1427,7 @@ size_t rt_diffattn_saved_bytes(int32_t H, int32_t Hkv, int32_t hd, int64_t Nq, i
 
 size_t rt_diffattn_fwd_workspace_bytes(int32_t B, int32_t H, int32_t Hkv, int32_t hd, int32_t Lq, int32_t Lk, int64_t Nq, int64_t Nk, int32_t train) {
   if (B < 0 || H <= 0 || Hkv <= 0 || hd <= 0 || hd > 64 || Lq < 0 || Lk < 0 || Nq <= 0 || Nk < 0 || H % Hkv != 0) return 0;
-  const Plan p = plan_of(B > 0 ? B : 1, H, Hkv, hd, Lq, Lk, train != 0);
+  const Plan p = plan_of(B > 0 ? B : 1, H, Hkv, hd, Lq, Lk, Nk, train != 0);
   Args a = sizes(H, Hkv, hd, Nq, Nk);
   return part_floats(p, Nq, H, hd) * sizeof(float) + (train == 0 && !p.decode ? carve_planes(a, nullptr, false) + 256 : 0);
 }
@@ -1428,8 +1448,8 @@ int rt_diffattn_fwd(const float* q, int64_t ldq, const float* k, int64_t ldk, co
   a.B = B; a.Lq = Lq; a.Lk = Lk;
   a.scale = scale > 0.f ? scale : 1.f / sqrtf((float)hd); a.causal = causal;
   a.norm_w = norm_w; a.out_scale = out_scale; a.eps = eps; a.y = y; a.ldy = ldy;
-  const Plan p = plan_of(B > 0 ? B : 1, H, Hkv, hd, Lq, Lk, saved != nullptr);
-  a.n_split = p.n_split;
+  const Plan p = plan_of(B > 0 ? B : 1, H, Hkv, hd, Lq, Lk, Nk, saved != nullptr);
+  a.n_split = p.n_split; a.share = p.share;
   const size_t part_bytes = part_floats(p, Nq, H, hd) * sizeof(float);
   const size_t need = part_bytes + (saved == nullptr && !p.decode ? carve_planes(a, nullptr, false) + 256 : 0);
   if (need > 0 && (ws == nullptr || ws_bytes < need || ((uintptr_t)ws & 15u) != 0)) return RT_ERR_WORKSPACE;
@@ -1442,9 +1462,9 @@ int rt_diffattn_fwd(const float* q, int64_t ldq, const float* k, int64_t ldk, co
   a.vec_y = hd % 2 == 0 && vec_ok(y, ldy);
   const long long B1 = B + (cu_q != nullptr ? 1 : 0);
   if (p.decode) {
-    if (!grid_ok(B1 * Hkv)) return RT_ERR_UNSUPPORTED;
+    if (!grid_ok(B1 * Hkv * p.n_split)) return RT_ERR_UNSUPPORTED;
     const long long queries = (long long)(H / Hkv) * (Lq > 0 ? Lq : 1);
-    const dim3 grid((unsigned)(B1 * Hkv), p.n_split);
+    const dim3 grid((unsigned)(B1 * Hkv * p.n_split));
     RT_TRY(HDP == 32 ? start_decode<32>(queries, mode, grid, stream, a) : start_decode<64>(queries, mode, grid, stream, a));
   } else {
     if (!plan_grid(a.own_q, B, H, Lq, cu_q != nullptr)) return RT_ERR_UNSUPPORTED;

@@ -406,6 +406,20 @@ def test_attention_long_causal_session_in_halves_and_splits():
     _attention_case([2_500], [2_500], 4, 2, 32, True, train=True)
 
 
+@pytest.mark.parametrize("hd", [32, 50])
+@pytest.mark.parametrize("rows", [1, 3, 10])
+def test_attention_few_queries_of_sessions_of_different_lengths(hd, rows):
+    """Shares of one size: long sessions fill many, short ones one, the rest are empty; sessions without keys and longer than expected among them."""
+    lens_k = [9_000, 3, 700, 0, 65, 4_321]
+    lens_q = [rows] * 6
+    _attention_case(lens_q, lens_k, 2, 2, hd, True, train=False)
+    _attention_case(lens_q, lens_k, 2, 1 if rows < 6 else 2, hd, False, train=False, Lk=6_000)
+    ids = torch.ones(sum(lens_k), dtype=torch.int64)
+    ids[:5_000] = 0
+    ids[9_000:9_003] = 0
+    _attention_case(lens_q, lens_k, 1, 1, hd, True, train=False, ids=ids)
+
+
 def test_attention_split_keys_training():
     _attention_case([20], [3_000], 2, 1, 32, True, train=True)
 
