@@ -8,8 +8,8 @@
 //
 // Memory bound: every column is read and written once.  The sine and cosine of a (row, pair) are shared by all heads of q AND k: a thread
 // keeps them for up to 4 heads of its pairs (64-bit product, reduction and sincos are about 50 operations a pair; at one head per thread
-// they cost as much issue time as the memory traffic).  65,536 rows, 16 + 4 heads of 64 columns, 32 of them turned, interleaved: 135 us = 5.0 TB/s
-// (one head per thread: 201 us).  With few rows the heads go to threads of their own instead: latency counts there.
+// they cost as much issue time as the memory traffic: half as long again).  65,536 rows, 16 + 4 heads of 64 columns, 32 of them turned, interleaved: 122 us
+// = 5.5 TB/s; heads of 63 columns, which no wide load divides: 164 us = 4.0 TB/s, all of them turned 135.  With few rows the heads go to threads of their own instead: latency counts there.
 #include "rt_common.h"
 
 namespace {
@@ -46,43 +46,57 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotArgs a) {
           sn[e] = s * a.gain * a.sign;
         }
       }
+      auto in = [&](int h) { return h < a.s[0].heads ? a.s[0].x + row * a.s[0].ldx + (long long)h * a.hd : a.s[1].x + row * a.s[1].ldx + (long long)(h - a.s[0].heads) * a.hd; };
+      auto out = [&](int h) { return h < a.s[0].heads ? a.s[0].y + row * a.s[0].ldy + (long long)h * a.hd : a.s[1].y + row * a.s[1].ldy + (long long)(h - a.s[0].heads) * a.hd; };
+      if (V == 1) {      // single columns: a thread's heads are read in front of the first one's store (one after the other: two
+        // 4-byte loads in flight, 65,536 rows of 20 heads of 63 columns 294 us instead of 164)
+        const int ia = turns ? (INTER ? 2 * j0 : j0) : a.rot + unit - turn_units, ib = INTER ? 2 * j0 + 1 : half + j0;
+        for (int h0 = hg; h0 < heads; h0 += 4 * a.groups) {
+          float u[4], v[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int h = h0 + j * a.groups;
+            if (h < heads) {
+              u[j] = in(h)[ia];
+              v[j] = turns ? in(h)[ib] : 0.f;
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int h = h0 + j * a.groups;
+            if (h < heads) {
+              float* y = out(h);
+              y[ia] = turns ? u[j] * cs[0] - v[j] * sn[0] : u[j];
+              if (turns) y[ib] = u[j] * sn[0] + v[j] * cs[0];
+            }
+          }
+        }
+        continue;
+      }
       for (int h = hg; h < heads; h += a.groups) {
-        const Seg& s = a.s[h < a.s[0].heads ? 0 : 1];
-        const int hh = h < a.s[0].heads ? h : h - a.s[0].heads;
-        const float* x = s.x + row * s.ldx + (long long)hh * a.hd;
-        float* y = s.y + row * s.ldy + (long long)hh * a.hd;
+        const float* x = in(h);
+        float* y = out(h);
         if (!turns) {
           const int c0 = a.rot + (unit - turn_units) * V;
-          if (V == 4) {
-            *reinterpret_cast<f32x4*>(y + c0) = *reinterpret_cast<const f32x4*>(x + c0);
-          } else {
-            y[c0] = x[c0];
-          }
+          *reinterpret_cast<f32x4*>(y + c0) = *reinterpret_cast<const f32x4*>(x + c0);
           continue;
         }
-        if (V == 4) {
-          if (INTER) {
-            f32x4 u = *reinterpret_cast<const f32x4*>(x + 2 * j0), v = *reinterpret_cast<const f32x4*>(x + 2 * j0 + 4);
-            *reinterpret_cast<f32x4*>(y + 2 * j0) = f32x4{u[0] * cs[0] - u[1] * sn[0], u[0] * sn[0] + u[1] * cs[0],
-                                                          u[2] * cs[1 % V] - u[3] * sn[1 % V], u[2] * sn[1 % V] + u[3] * cs[1 % V]};
-            *reinterpret_cast<f32x4*>(y + 2 * j0 + 4) = f32x4{v[0] * cs[2 % V] - v[1] * sn[2 % V], v[0] * sn[2 % V] + v[1] * cs[2 % V],
-                                                              v[2] * cs[3 % V] - v[3] * sn[3 % V], v[2] * sn[3 % V] + v[3] * cs[3 % V]};
-          } else {
-            const f32x4 u = *reinterpret_cast<const f32x4*>(x + j0), v = *reinterpret_cast<const f32x4*>(x + half + j0);
-            f32x4 p, q;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              p[e] = u[e] * cs[e % V] - v[e] * sn[e % V];
-              q[e] = u[e] * sn[e % V] + v[e] * cs[e % V];
-            }
-            *reinterpret_cast<f32x4*>(y + j0) = p;
-            *reinterpret_cast<f32x4*>(y + half + j0) = q;
-          }
+        if (INTER) {
+          const f32x4 u = *reinterpret_cast<const f32x4*>(x + 2 * j0), v = *reinterpret_cast<const f32x4*>(x + 2 * j0 + 4);
+          *reinterpret_cast<f32x4*>(y + 2 * j0) = f32x4{u[0] * cs[0] - u[1] * sn[0], u[0] * sn[0] + u[1] * cs[0],
+                                                        u[2] * cs[1 % V] - u[3] * sn[1 % V], u[2] * sn[1 % V] + u[3] * cs[1 % V]};
+          *reinterpret_cast<f32x4*>(y + 2 * j0 + 4) = f32x4{v[0] * cs[2 % V] - v[1] * sn[2 % V], v[0] * sn[2 % V] + v[1] * cs[2 % V],
+                                                            v[2] * cs[3 % V] - v[3] * sn[3 % V], v[2] * sn[3 % V] + v[3] * cs[3 % V]};
         } else {
-          const int ia = INTER ? 2 * j0 : j0, ib = INTER ? 2 * j0 + 1 : half + j0;
-          const float u = x[ia], v = x[ib];
-          y[ia] = u * cs[0] - v * sn[0];
-          y[ib] = u * sn[0] + v * cs[0];
+          const f32x4 u = *reinterpret_cast<const f32x4*>(x + j0), v = *reinterpret_cast<const f32x4*>(x + half + j0);
+          f32x4 p, q;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            p[e] = u[e] * cs[e % V] - v[e] * sn[e % V];
+            q[e] = u[e] * sn[e % V] + v[e] * cs[e % V];
+          }
+          *reinterpret_cast<f32x4*>(y + j0) = p;
+          *reinterpret_cast<f32x4*>(y + half + j0) = q;
         }
       }
     }
