@@ -1064,7 +1064,8 @@ __global__ __launch_bounds__(NT, 2) void diff_bwd_kernel(Args a, Sums m) {
 // dot product is four multiply-adds and a sum over the lanes of its map (cross-lane adds, no LDS), the two maps' lanes swap their probabilities, the value
 // sums stay with the lanes' columns.  Every lane group keeps its own running maximum and sum until the end; no barrier in the loop, and the
 // next TK keys are read while these are taken.  1,024 sessions of up to 200 keys, 4 heads of hd 32, one query each: 43 us = 6.1 TB/s (memory bound);
-// 8 sessions of up to 65,536, 4 queries to each of 2 key heads of hd 64: 130 us = 5.0 TB/s; 8 of 65,536 each 186 us = 5.8 TB/s with one query, 194 with four.  R is the next power of two: instances for 1, 2, 4, 8, so that one query pays for one.
+// 8 sessions of up to 65,536, 4 queries to each of 2 key heads of hd 64: 130 us = 5.0 TB/s; 8 of 65,536 each 186 us = 5.8 TB/s with one query, 194 with
+// four.  R is the next power of two: instances for 1, 2, 4, 8, so that one query pays for one.
 constexpr int MAXR = 8;
 
 template <int HD> __device__ __forceinline__ float other_map(float v) {
