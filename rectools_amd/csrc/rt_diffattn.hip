@@ -150,8 +150,13 @@ template <int HD> struct Row {
 // exponent of the row's scale: its largest magnitude comes to 2^13 .. 2^14 (2 x below the fp16 range; what is 2^-18 of it keeps all 22 bits)
 // `least`: values below 2^(least + 14) lose bits.  -126 keeps 2^e a normal number; v takes -80, so that a row sum of weights that carry 2^-e
 // stays finite over any number of keys.
-__device__ __forceinline__ int row_exp(float top, int least) {
-  if (!(top > 0.f) || top > 3.0e38f) return 0;      // a zero row; infinities and NaN stay what they are
+// `zero`: of a row of zeros.  It adds nothing to a product, but its weights, which carry its 2^e, stand beside the other rows' where those are split into
+// halves with one unit: with exponent 0 they drove the bits of rows of ordinary size out of the fp16 range (dV beside queries without a gradient, |dO| = 1e-6:
+// 3 % off).  q, k and dO take the least there is.
+constexpr int LEAST = -126, LEAST_V = -80;
+__device__ __forceinline__ int row_exp(float top, int least, int zero) {
+  if (top == 0.f) return zero;
+  if (!(top <= 3.0e38f)) return 0;      // infinities and NaN stay what they are
   const int e = __builtin_amdgcn_frexp_expf(top) - 14;
   return e < least ? least : e;
 }
@@ -186,7 +191,7 @@ __global__ __launch_bounds__(NT) void diff_planes_kernel(Args a, unsigned q_bloc
   const long long slot = h * (N + PAD) + row;
   if (what == 2) {
     const f32x4 x = live ? get4<MODE>(a.v + row * a.ldv + (long long)h * 2 * hd, 4 * c4, 2 * hd) : f32x4{0.f, 0.f, 0.f, 0.f};
-    const int e = row_exp(group_max<LANES>(top4(x)), -80);
+    const int e = row_exp(group_max<LANES>(top4(x)), LEAST_V, 0);
     put_planes(a.vp + slot * Row<HD>::BYTES + 8 * c4, 4 * HD, x, e);
     if (c4 == 0) {
       a.vs[slot] = pow2(e);
@@ -198,7 +203,7 @@ __global__ __launch_bounds__(NT) void diff_planes_kernel(Args a, unsigned q_bloc
   const int mp = c4 / (HD / 4), col = (c4 % (HD / 4)) * 4;
   const float* src = what == 0 ? a.q + row * a.ldq + (long long)(2 * h + mp) * hd : a.k + row * a.ldk + (long long)(2 * h + mp) * hd;
   const f32x4 x = live ? get4<MODE>(src, col, hd) : f32x4{0.f, 0.f, 0.f, 0.f};
-  const int e = row_exp(group_max<LANES / 2>(top4(x)), -126);
+  const int e = row_exp(group_max<LANES / 2>(top4(x)), LEAST, LEAST);
   put_planes((what == 0 ? a.qp : a.kp) + slot * Row<HD>::BYTES + mp * 4 * HD + 2 * col, 2 * HD, x, e);
   if (c4 % (HD / 4) == 0) (what == 0 ? a.qs : a.ks)[(2 * h + mp) * (N + PAD) + row] = pow2(e);
 }
@@ -314,7 +319,8 @@ __device__ __forceinline__ void split16(const float (&x)[16], float factor, P2 (
     }
 }
 // The same for weights of unknown size (dS; the difference map times dO's scales): the lane's unit follows the largest magnitude it has met, as
-// the running maximum of a softmax does; when it grows, the lane's accumulators are rescaled (powers of two: exact).
+// the running maximum of a softmax does; when it grows, the lane's accumulators are rescaled (powers of two: exact).  That keeps the result's bits if a
+// large weight meets a row of large plane values: every row's planes are scaled to one size, and a zero row's weight is the least there is (row_exp).
 template <int NB>
 __device__ __forceinline__ void split16_scaled(const float (&x)[16], float& inv, f32x16 (&acc)[NB], P2 (&out)[2]) {
   float top = 0.f;
@@ -701,7 +707,7 @@ __global__ __launch_bounds__(NT) void diff_bwd_pre_kernel(Args a, const float* d
       if (MODE != 0) t[k] = c + k < dv ? t[k] : 0.0;
       d[k] = (float)t[k];
     }
-    const int ex = row_exp(group_max<LANES>(top4(d)), -126);
+    const int ex = row_exp(group_max<LANES>(top4(d)), LEAST, LEAST);
     put_planes(a.dp + (h * NqP + row) * Row<HD>::BYTES + 2 * c, 4 * HD, d, ex);
     const double s1 = group_sum<LANES>(t[0] * o1[0] + t[1] * o1[1] + t[2] * o1[2] + t[3] * o1[3]);
     const double s2 = group_sum<LANES>(t[0] * o2[0] + t[1] * o2[1] + t[2] * o2[2] + t[3] * o2[3]);
