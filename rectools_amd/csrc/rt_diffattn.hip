@@ -152,8 +152,9 @@ template <int HD> struct Row {
 // stays finite over any number of keys.
 // `zero`: of a row of zeros.  It adds nothing to a product, but its weights, which carry its 2^e, stand beside the other rows' where those are split into
 // halves with one unit: with exponent 0 they drove the bits of rows of ordinary size out of the fp16 range (dV beside queries without a gradient, |dO| = 1e-6:
-// 3 % off).  q, k and dO take the least there is.
-constexpr int LEAST = -126, LEAST_V = -80;
+// 3 % off; outputs beside one zero value row, |v| = 1e-6: 1 %).  q, k and dO take the least there is.  A zero value row's weight is counted in the row sum
+// through s + e - m, rounded at its size: -40 keeps that at 7e-7 of it beside values of size one (-80: 3e-6) and all bits of values down to 1e-12.
+constexpr int LEAST = -126, LEAST_V = -80, ZERO_V = -40;
 __device__ __forceinline__ int row_exp(float top, int least, int zero) {
   if (top == 0.f) return zero;
   if (!(top <= 3.0e38f)) return 0;      // infinities and NaN stay what they are
@@ -191,7 +192,7 @@ __global__ __launch_bounds__(NT) void diff_planes_kernel(Args a, unsigned q_bloc
   const long long slot = h * (N + PAD) + row;
   if (what == 2) {
     const f32x4 x = live ? get4<MODE>(a.v + row * a.ldv + (long long)h * 2 * hd, 4 * c4, 2 * hd) : f32x4{0.f, 0.f, 0.f, 0.f};
-    const int e = row_exp(group_max<LANES>(top4(x)), LEAST_V, 0);
+    const int e = row_exp(group_max<LANES>(top4(x)), LEAST_V, ZERO_V);
     put_planes(a.vp + slot * Row<HD>::BYTES + 8 * c4, 4 * HD, x, e);
     if (c4 == 0) {
       a.vs[slot] = pow2(e);

@@ -1,5 +1,5 @@
-"""Differential attention where rows are exactly zero: queries without a gradient (rows without a target, padded rows), zero queries and keys, next
-to rows of ordinary and of very small size.  A zero row has no size that its neighbours could be measured against.
+"""Differential attention where rows are exactly zero: queries without a gradient (rows without a target, padded rows), zero values, queries and keys,
+next to rows of ordinary and of very small size.  A zero row has no size that its neighbours could be measured against.
 
 Tolerance, per tensor, in the 2-norm.  An operand held as two halves is off by 2 u (u = 2^-24), the term that a product of them drops by 4 u more: a
 product's factors and the term, 8 u.  What such roundings can do to a result depends on the inputs (a row whose two maps nearly cancel is divided by
@@ -94,6 +94,21 @@ def test_queries_without_a_gradient(H, Hkv, hd, norm, causal, size):
     assert not got["dq"][none.cuda()].any()
 
 
+@pytest.mark.parametrize("size", [1e4, 1.0, 1e-3, 1e-6, 1e-9])
+@pytest.mark.parametrize("train", [True, False])
+@pytest.mark.parametrize("H,Hkv,hd,norm", [(2, 2, 32, True), (2, 1, 64, False)])
+@pytest.mark.parametrize("share", [0.05, 0.5, 0.95])
+def test_zero_values(share, H, Hkv, hd, norm, train, size):
+    n = sum(LENS)
+    ins, gy, g = _inputs(n, n, H, Hkv, hd, norm, seed=1)
+    none = torch.rand(n, generator=g) < share
+    none[[10, 71, 104, 130]] = True
+    none[[0, 70, 103, 108]] = False
+    ins[2] = torch.where(none[:, None], 0.0, ins[2] * size)
+    _check(ins, gy if train else None, LENS, LENS, H, Hkv, True)
+    _check(ins, gy if train else None, LENS, LENS, H, Hkv, False)
+
+
 @pytest.mark.parametrize("size", [1.0, 1e-3, 1e-6])
 @pytest.mark.parametrize("which", [0, 1])
 @pytest.mark.parametrize("causal", [True, False])
@@ -105,6 +120,17 @@ def test_zero_queries_and_keys(causal, which, size):
     ins[which] = torch.where(none[:, None], 0.0, ins[which] * size)
     ins[1 - which] = ins[1 - which] / size
     _check(ins, gy, LENS, LENS, 2, 1, causal)
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_zero_values_of_split_keys(rows):
+    """Few queries and few matrix tiles against long keys."""
+    for size in (1.0, 1e-6):
+        ins, _, g = _inputs(rows, 3_000, 2, 1, 32, False, seed=3)
+        none = torch.rand(3_000, generator=g) < 0.3
+        none[1_000:2_000] = True
+        ins[2] = torch.where(none[:, None], 0.0, ins[2] * size)
+        _check(ins, None, [rows], [3_000], 2, 1, True)
 
 
 @pytest.mark.parametrize("size", [1.0, 1e-6])
