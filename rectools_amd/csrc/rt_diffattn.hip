@@ -666,7 +666,37 @@ __global__ __launch_bounds__(NT) void diff_combine_kernel(Args a) {
 // are summed in 64 bits, per workgroup, in a fixed order.  do stands at right angles to o (but for eps) and do . o_m is what is left of that: formed in
 // 64 bits, from the outputs as they are (in 32 the gradient of lam was 2 - 5 x further off; 15.5 -> 17 us).  Memory bound: 8,192 rows of 4 heads of hd 64,
 // 70 MB, 18 us = 3.9 TB/s.
+//
+// A row that sees ONE key has that key's values for both maps' outputs, whatever the logits are: dO stands at right angles to them but for eps, and the
+// row's share of dlam, 1e-5 of its terms, would be the two outputs' own roundings (sessions of one row: 0.3 to 3 % off).  o_2 is o_1 there.  Which rows
+// those are is looked up where the saved outputs nearly agree (128 packed sessions of up to 200, 4 heads of hd 32: 16.5 -> 18.9 us; two of 4,096: 17.0 -> 17.6).
 constexpr int PRE_WG = 1024;      // workgroups at most: the partials are [PRE_WG][H + 2 hd] doubles
+
+// whether query row `row` sees one key: its session by bisection, its keys by the lane group, which stops at the second one
+template <int LANES>
+__device__ __forceinline__ bool sees_one_key(const Args& a, long long row, int lane) {
+  int b = 0;
+  if (a.cu_q != nullptr) {
+    for (int e = a.B; e - b > 1;) {
+      const int mid = b + (e - b) / 2;
+      if (a.cu_q[mid] <= row) b = mid;
+      else e = mid;
+    }
+  } else {
+    b = (int)(row / a.Lq);
+  }
+  long long qr0, kr0; int nq, nk;
+  rows_of(a.cu_q, b, a.Lq, a.Nq, qr0, nq);
+  rows_of(a.cu_k, b, a.Lk, a.Nk, kr0, nk);
+  const long long at = row - qr0;
+  if (at < 0 || at >= nq) return false;
+  const int end = a.causal ? min(nk, (int)at + nk - nq + 1) : nk;
+  if (a.key_ids == nullptr) return end == 1;
+  float seen = 0.f;
+  for (int j0 = 0; j0 < end && seen < 2.f; j0 += LANES)
+    seen += group_sum<LANES>(j0 + lane < end && a.key_ids[kr0 + j0 + lane] != 0 ? 1.f : 0.f);
+  return seen == 1.f;
+}
 
 template <int HD, int MODE>
 __global__ __launch_bounds__(NT) void diff_bwd_pre_kernel(Args a, const float* dy, long long lddy, double* part) {
@@ -682,10 +712,17 @@ __global__ __launch_bounds__(NT) void diff_bwd_pre_kernel(Args a, const float* d
   double dw[4] = {0.0, 0.0, 0.0, 0.0}, dl = 0.0;
   for (long long row = gg < step * H ? gg / H : used; row < used; row += step) {
     const long long at = row * H + h;
-    const f32x4 o1 = get4<MODE>(a.o12 + at * 2 * dv, c, dv), o2 = get4<MODE>(a.o12 + (at * 2 + 1) * dv, c, dv);
+    const f32x4 o1 = get4<MODE>(a.o12 + at * 2 * dv, c, dv);
+    f32x4 o2 = get4<MODE>(a.o12 + (at * 2 + 1) * dv, c, dv);
     const f32x4 g = get4<MODE>(dy + row * lddy + (long long)h * dv, c, dv), e = g * w;
     double t[4] = {e[0], e[1], e[2], e[3]};
     if (a.norm_w != nullptr) {
+      // (outputs of one key's values: each off by 2 u for the values' halves, 8 u for the product, 4 u for the row sum's reciprocal and the products with it, u = 2^-24)
+      const float top = group_max<LANES>(top4(o1)), apart = group_max<LANES>(top4(o1 - o2));
+      const bool near = apart <= 0x1p-19f * top;
+      if (__builtin_expect(__any(near), 0)) {
+        if (near && apart > 0.f && sees_one_key<LANES>(a, row, c / 4)) o2 = o1;
+      }
       double x[4], xx = 0.0, ex = 0.0;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
