@@ -146,6 +146,12 @@ bool on_tape(std::initializer_list<const Tensor*> ts) {
     if (t->defined() && t->requires_grad()) return true;
   return false;
 }
+// Forward-mode derivatives are refused, as second ones are: a tensor with a tangent need not require a gradient, and without a node its tangent would be
+// dropped in silence (a zero derivative).
+void no_tangent(const char* what, std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts)
+    if (t->defined() && t->_fw_grad(0).defined()) raise(PyExc_NotImplementedError, std::string(what) + " has no forward-mode derivative");
+}
 void once(const char* what) {      // grad mode is on in a backward pass only under create_graph
   TORCH_CHECK(!at::GradMode::is_enabled(), what, " has no second derivative (create_graph=True)");
 }
@@ -210,6 +216,8 @@ struct RotaryNode : torch::autograd::Function<RotaryNode> {
 
 std::vector<Tensor> rotary(const Tensor& q_in, const OptTensor& k_in, const Tensor& pos_in, const Tensor& freq_in, int64_t n_heads, int64_t n_kv_heads, bool interleaved,
                            double gain) {
+  const Tensor k_any = got(k_in);
+  no_tangent("rotary", {&q_in, &k_any, &freq_in});
   if (n_heads <= 0 || (k_in.has_value() && n_kv_heads <= 0)) bad("rotary", "head counts must be positive, got " + std::to_string(n_heads) + " and " + std::to_string(n_kv_heads));
   const Tensor q = rows(q_in, -1, "rotary");
   const int64_t M = q.size(0), cols = q.size(1);
@@ -263,6 +271,7 @@ struct LambdaNode : torch::autograd::Function<LambdaNode> {
   }
 };
 Tensor diff_lambda(const Tensor& q1_in, const Tensor& k1_in, const Tensor& q2_in, const Tensor& k2_in, double init) {
+  no_tangent("diff_lambda", {&q1_in, &k1_in, &q2_in, &k2_in});
   check_f32(q1_in, "diff_lambda");
   if (q1_in.dim() != 2 || q1_in.size(1) == 0) bad("diff_lambda", "expected [heads, columns], got " + shape(q1_in));
   const Tensor q1 = q1_in.contiguous(), k1 = vec(k1_in, q1_in.sizes(), q1_in, "diff_lambda"), q2 = vec(q2_in, q1_in.sizes(), q1_in, "diff_lambda"),
@@ -334,6 +343,8 @@ struct AttentionNode : torch::autograd::Function<AttentionNode> {
 Tensor diff_attention(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, const Tensor& lam_in, const OptTensor& cu_q_in, const OptTensor& cu_k_in, int64_t B, int64_t H,
                       int64_t Hkv, int64_t Lq, int64_t Lk, bool causal, const OptTensor& ids_in, const OptTensor& w_in, double out_scale, double eps, c10::optional<double> scale) {
   const char* what = "diff_attention";
+  const Tensor w_any = got(w_in);
+  no_tangent(what, {&q_in, &k_in, &v_in, &lam_in, &w_any});
   constexpr int64_t most = 0x7FFFFFFF;
   if (B < 0 || H <= 0 || Hkv <= 0 || H % Hkv != 0 || Lq < 0 || Lk < 0 || B > most || H > most || Lq > most || Lk > most)
     bad(what, "B=" + std::to_string(B) + ", H=" + std::to_string(H) + ", H_kv=" + std::to_string(Hkv) + ", Lq=" + std::to_string(Lq) + ", Lk=" + std::to_string(Lk));
@@ -414,6 +425,11 @@ struct NormNode : torch::autograd::Function<NormNode> {
 std::vector<Tensor> norm_gate(const Tensor& x_in, const Tensor& f_in, const OptTensor& z_in, const OptTensor& sc_in, const OptTensor& pw_in, const OptTensor& pb_in,
                               const OptTensor& nw_in, const OptTensor& nb_in, bool layer, double alpha, double eps, double p, uint64_t seed, uint64_t sid) {
   const char* what = "norm_gate_residual";
+  for (const OptTensor* t : {&z_in, &sc_in, &pw_in, &pb_in, &nw_in, &nb_in}) {
+    const Tensor any = got(*t);
+    no_tangent(what, {&any});
+  }
+  no_tangent(what, {&x_in, &f_in});
   check_f32(x_in, what);
   if (x_in.dim() != 2 || x_in.size(1) == 0) bad(what, "expected [rows, columns], got " + shape(x_in));
   const int64_t d = x_in.size(1);

@@ -2537,7 +2537,8 @@ def softmax_loss(sess: torch.Tensor, table: torch.Tensor, act_idx: torch.Tensor,
 # --------------------------------------------------------------------------------------------------
 # Argument checks, buffers and autograd nodes are compiled (csrc/rt_torch.cpp: the host set the pace of these small launches when they were
 # written here); the kernels are the C entries rt_rotary, rt_diff_lambda_*, rt_diffattn_*, rt_norm_gate_*.  Work is issued on the current
-# stream of the tensors' device; a backward pass of any of them has no second derivative.
+# stream of the tensors' device; a backward pass of any of them has no second derivative, and none has a forward-mode derivative (refused, with tensors
+# that carry a tangent).
 def _native_op(name: str, *args: tp.Any) -> tp.Any:
     fn = getattr(_lib.torch_ops(), name)
     if _TIMING is None:
