@@ -218,6 +218,7 @@ std::vector<Tensor> rotary(const Tensor& q_in, const OptTensor& k_in, const Tens
                            double gain) {
   const Tensor k_any = got(k_in);
   no_tangent("rotary", {&q_in, &k_any, &freq_in});
+  if (at::GradMode::is_enabled() && freq_in.requires_grad()) raise(PyExc_NotImplementedError, "rotary has no gradient of the frequencies: detach them");
   if (n_heads <= 0 || (k_in.has_value() && n_kv_heads <= 0)) bad("rotary", "head counts must be positive, got " + std::to_string(n_heads) + " and " + std::to_string(n_kv_heads));
   const Tensor q = rows(q_in, -1, "rotary");
   const int64_t M = q.size(0), cols = q.size(1);

@@ -2579,7 +2579,8 @@ def rotary_frequencies(rot: int, base: float = 10_000.0, scaling: str = "none", 
 
 def rotary(x: torch.Tensor, positions: torch.Tensor, freq: torch.Tensor, n_heads: int, interleaved: bool = False, gain: float = 1.0) -> torch.Tensor:
     """Rotary positions on x [M, n_heads * hd] (a column block of a wider matrix is read in place): the first 2 * len(freq) columns of every
-    head turn by positions[row] * freq; interleaved pairs (2 j, 2 j + 1) or halves (j, j + rot / 2).  positions [M] int64."""
+    head turn by positions[row] * freq; interleaved pairs (2 j, 2 j + 1) or halves (j, j + rot / 2).  positions [M] int64.  The frequencies have no
+    gradient (refused where they require one)."""
     return _native_op("rotary", x, None, positions, freq, n_heads, 0, interleaved, gain)[0]
 
 

@@ -47,3 +47,15 @@ def test_forward_mode_is_refused_on_the_device():
         call(*tensors)      # (and nothing else is)
         with pytest.raises((NotImplementedError, RuntimeError)):
             torch.func.jvp(lambda *t: call(*t), tuple(tensors), tuple(torch.ones_like(t) for t in tensors))
+
+
+@pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_frequencies_that_require_a_gradient_are_refused(dev):
+    x, pos = torch.randn(6, 64, device=dev), torch.arange(6, device=dev)
+    freq = ops.rotary_frequencies(16, device=dev)[0].requires_grad_()
+    for call in (lambda: ops.rotary(x, pos, freq, 4), lambda: ops.rotary_qk(x, x, pos, freq, 4, 4)):
+        with pytest.raises(NotImplementedError, match="frequencies"):
+            call()
+    if dev == "cuda":
+        with torch.no_grad():
+            assert torch.equal(ops.rotary(x, pos, freq, 4), ops.rotary(x, pos, freq.detach(), 4))
