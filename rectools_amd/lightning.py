@@ -35,8 +35,11 @@ def requires_negatives(loss: str) -> tp.Optional[bool]:
 
 
 def xavier_normal_init(model: nn.Module) -> None:
+    """Every parameter of two and more dimensions, but those that a module names in `own_init`: rows of vectors, not matrices, which start as their
+    constructor made them."""
+    kept = {id(getattr(module, name)) for module in model.modules() for name in getattr(module, "own_init", ())}
     for _, param in model.named_parameters():
-        if param.data.dim() > 1:
+        if param.data.dim() > 1 and id(param) not in kept:
             torch.nn.init.xavier_normal_(param.data)
 
 

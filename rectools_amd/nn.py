@@ -800,6 +800,8 @@ class DifferentialTransformerLayer(nn.Module):
     """One block of `DifferentialTransformerLayers`: differential attention over rotary positions, then a feed-forward, each between a
     norm in front and a norm behind, the latter with a gate on the residual stream and a learned residual scale."""
 
+    own_init = ("lambda_q1", "lambda_k1", "lambda_q2", "lambda_k2")      # a vector per head, deviation 0.1: lam starts near lambda_init
+
     def __init__(self, n_factors: int, n_heads: int, n_kv_heads: int, dropout_rate: float, ff_factors_multiplier: int, ff_activation: str,
                  bias_in_ff: bool, lambda_init: float) -> None:
         super().__init__()
@@ -808,7 +810,7 @@ class DifferentialTransformerLayer(nn.Module):
         self.widths = [n_factors, 2 * n_kv_heads * hd, 2 * n_kv_heads * hd]
         self.in_proj = LinearParams(n_factors, sum(self.widths), bias=False)
         self.out_proj = LinearParams(n_factors, n_factors, bias=False)
-        for name in ("lambda_q1", "lambda_k1", "lambda_q2", "lambda_k2"):
+        for name in self.own_init:
             setattr(self, name, nn.Parameter(torch.randn(n_heads, hd) * 0.1))
         self.head_norm = nn.Parameter(torch.ones(2 * hd))
         self.feed_forward = init_feed_forward(n_factors, ff_factors_multiplier, dropout_rate, ff_activation, bias_in_ff)
