@@ -130,6 +130,7 @@ Tensor vec(const OptTensor& t, at::IntArrayRef want, const Tensor& first, const 
   check_device(*t, first, what);
   return t->contiguous();
 }
+constexpr int64_t MOST = 0x7FFFFFFF;      // the C entries count heads and columns in 32 bits
 void check_eps(double eps, const char* what) {      // (as the kernels see it: without it a row of zeros has no norm)
   if (!((float)eps > 0.f)) bad(what, "eps is positive, got " + std::to_string(eps));
 }
@@ -219,14 +220,16 @@ std::vector<Tensor> rotary(const Tensor& q_in, const OptTensor& k_in, const Tens
   const Tensor k_any = got(k_in);
   no_tangent("rotary", {&q_in, &k_any, &freq_in});
   if (at::GradMode::is_enabled() && freq_in.requires_grad()) raise(PyExc_NotImplementedError, "rotary has no gradient of the frequencies: detach them");
-  if (n_heads <= 0 || (k_in.has_value() && n_kv_heads <= 0)) bad("rotary", "head counts must be positive, got " + std::to_string(n_heads) + " and " + std::to_string(n_kv_heads));
+  if (n_heads <= 0 || (k_in.has_value() && (n_kv_heads <= 0 || n_kv_heads > MOST))) bad("rotary", "head counts must be positive, got " + std::to_string(n_heads) + " and " + std::to_string(n_kv_heads));
   const Tensor q = rows(q_in, -1, "rotary");
   const int64_t M = q.size(0), cols = q.size(1);
+  if (cols > MOST) raise(PyExc_NotImplementedError, "rotary: at most 2^31 - 1 columns, got " + std::to_string(cols));
   if (cols == 0 || cols % n_heads != 0) bad("rotary", std::to_string(cols) + " columns do not split into " + std::to_string(n_heads) + " heads");
   const int64_t hd = cols / n_heads;
   Tensor k;
   if (k_in.has_value()) {
     k = rows(*k_in, n_kv_heads * hd, "rotary");
+    if (k.size(1) > MOST) raise(PyExc_NotImplementedError, "rotary: at most 2^31 - 1 columns, got " + std::to_string(k.size(1)));
     if (k.size(0) != M) bad("rotary", std::to_string(M) + " query rows and " + std::to_string(k.size(0)) + " key rows");
     check_device(k, q, "rotary");
   }
@@ -275,6 +278,7 @@ Tensor diff_lambda(const Tensor& q1_in, const Tensor& k1_in, const Tensor& q2_in
   no_tangent("diff_lambda", {&q1_in, &k1_in, &q2_in, &k2_in});
   check_f32(q1_in, "diff_lambda");
   if (q1_in.dim() != 2 || q1_in.size(1) == 0) bad("diff_lambda", "expected [heads, columns], got " + shape(q1_in));
+  if (q1_in.size(0) > MOST || q1_in.size(1) > MOST) raise(PyExc_NotImplementedError, "diff_lambda: at most 2^31 - 1 heads and columns, got " + shape(q1_in));
   const Tensor q1 = q1_in.contiguous(), k1 = vec(k1_in, q1_in.sizes(), q1_in, "diff_lambda"), q2 = vec(q2_in, q1_in.sizes(), q1_in, "diff_lambda"),
                k2 = vec(k2_in, q1_in.sizes(), q1_in, "diff_lambda");
   return on_tape({&q1, &k1, &q2, &k2}) ? LambdaNode::apply(q1, k1, q2, k2, init) : lambda_call(q1, k1, q2, k2, init);
@@ -346,8 +350,7 @@ Tensor diff_attention(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in
   const char* what = "diff_attention";
   const Tensor w_any = got(w_in);
   no_tangent(what, {&q_in, &k_in, &v_in, &lam_in, &w_any});
-  constexpr int64_t most = 0x7FFFFFFF;
-  if (B < 0 || H <= 0 || Hkv <= 0 || H % Hkv != 0 || Lq < 0 || Lk < 0 || B > most || H > most || Lq > most || Lk > most)
+  if (B < 0 || H <= 0 || Hkv <= 0 || H % Hkv != 0 || Lq < 0 || Lk < 0 || B > MOST || H > MOST || Lq > MOST || Lk > MOST)
     bad(what, "B=" + std::to_string(B) + ", H=" + std::to_string(H) + ", H_kv=" + std::to_string(Hkv) + ", Lq=" + std::to_string(Lq) + ", Lk=" + std::to_string(Lk));
   const Tensor q = rows(q_in, -1, "diff_attention q");
   if (q.size(1) == 0 || q.size(1) % (2 * H) != 0) bad(what, std::to_string(q.size(1)) + " query columns do not split into " + std::to_string(H) + " heads of two maps");
