@@ -886,8 +886,8 @@ class DifferentialTransformerLayers(TransformerLayersBase):
                  rotary_trained_len: int = 4096, **kwargs: tp.Any) -> None:
         super().__init__()
         n_kv_heads = n_heads if n_kv_heads is None else n_kv_heads
-        if n_factors % (2 * n_heads) != 0 or n_heads % n_kv_heads != 0:
-            raise ValueError(f"DifferentialTransformerLayers: n_factors must be divisible by 2 * n_heads and n_heads by n_kv_heads, got n_factors={n_factors}, "
+        if n_heads < 1 or n_kv_heads < 1 or n_factors < 1 or n_factors % (2 * n_heads) != 0 or n_heads % n_kv_heads != 0:
+            raise ValueError(f"DifferentialTransformerLayers: head counts are positive, n_factors must be divisible by 2 * n_heads and n_heads by n_kv_heads, got n_factors={n_factors}, "
                              f"n_heads={n_heads}, n_kv_heads={n_kv_heads}")
         hd = n_factors // (2 * n_heads)
         if hd > 64:

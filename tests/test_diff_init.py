@@ -56,3 +56,9 @@ def test_a_fitted_model_started_there(family):
     m = cls(n_factors=256, n_blocks=2, n_heads=4, session_max_len=24, lr=1e-12, batch_size=48, dropout_rate=0.1, loss="softmax", epochs=1, seed=1, deterministic=True,
             use_key_padding_mask=True, transformer_layers_type=hnn.DifferentialTransformerLayers).fit(_dataset())
     _starts(m.torch_model.transformer_layers)
+
+
+@pytest.mark.parametrize("H,kv,d", [(4, 0, 64), (4, -1, 64), (4, -4, 64), (0, None, 64), (-2, -1, 64), (4, 2, 0), (2, 1, -64)])
+def test_counts_that_are_not_positive_are_refused(H, kv, d):
+    with pytest.raises(ValueError):
+        hnn.DifferentialTransformerLayers(1, d, H, 0.0, n_kv_heads=kv)
