@@ -159,7 +159,7 @@ void once(const char* what) {      // grad mode is on in a backward pass only un
 
 // Leaves whose gradient node was made on the default stream (by a graph that lives outside a capture, or by this call on that stream): the engine
 // hands their gradients over on that stream, which no capture can follow; the process would end there.  Noted in the forward pass, refused when
-// the backward pass runs under a capture.
+// the backward pass runs under a capture.  `held`: the same of the caller's own tensors, where the node is given a dense copy of one (rows(), contiguous()).
 bool default_stream_leaves(std::initializer_list<const Tensor*> ts) {
   for (const Tensor* t : ts) {
     if (!t->defined() || !t->is_leaf() || !t->requires_grad()) continue;
@@ -188,9 +188,9 @@ Tensor like(const Tensor& t) { return t.defined() ? at::empty(t.sizes(), t.optio
 
 struct RotaryNode : torch::autograd::Function<RotaryNode> {
   static variable_list forward(AutogradContext* ctx, const Tensor& q, const OptTensor& k_opt, const Tensor& pos, const Tensor& freq, int64_t n_heads, int64_t n_kv_heads,
-                               int64_t hd, bool interleaved, double gain) {
+                               int64_t hd, bool interleaved, double gain, bool held) {
     const Tensor k = got(k_opt);
-    ctx->saved_data["leaves"] = default_stream_leaves({&q, &k});
+    ctx->saved_data["leaves"] = held || default_stream_leaves({&q, &k});
     ctx->save_for_backward({pos, freq});
     ctx->saved_data["m"] = std::vector<int64_t>{n_heads, n_kv_heads, hd, interleaved};
     ctx->saved_data["g"] = gain;
@@ -203,7 +203,7 @@ struct RotaryNode : torch::autograd::Function<RotaryNode> {
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     once("rotary");
     capturable(ctx, "rotary");
-    variable_list out(9);
+    variable_list out(10);
     Tensor gq = g[0].defined() ? dense_rows(g[0]) : Tensor(), gk = g.size() > 1 && g[1].defined() ? dense_rows(g[1]) : Tensor();
     if (!gq.defined() && !gk.defined()) return out;
     const auto saved = ctx->get_saved_variables();
@@ -242,7 +242,7 @@ std::vector<Tensor> rotary(const Tensor& q_in, const OptTensor& k_in, const Tens
   }
   check_device(freq_in, q, "rotary");
   const Tensor freq = freq_in.contiguous();
-  if (on_tape({&q, &k})) return RotaryNode::apply(q, opt(k), pos, freq, n_heads, n_kv_heads, hd, interleaved, gain);
+  if (on_tape({&q, &k})) return RotaryNode::apply(q, opt(k), pos, freq, n_heads, n_kv_heads, hd, interleaved, gain, default_stream_leaves({&q_in, &k_any}));
   variable_list out{like(q)};
   if (k.defined()) out.push_back(like(k));
   rotary_call(q, k, out[0], k.defined() ? out[1] : Tensor(), pos, freq, {n_heads, n_kv_heads, hd, interleaved, gain}, false);
@@ -257,8 +257,8 @@ Tensor lambda_call(const Tensor& q1, const Tensor& k1, const Tensor& q2, const T
   return lam;
 }
 struct LambdaNode : torch::autograd::Function<LambdaNode> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& q1, const Tensor& k1, const Tensor& q2, const Tensor& k2, double init) {
-    ctx->saved_data["leaves"] = default_stream_leaves({&q1, &k1, &q2, &k2});
+  static Tensor forward(AutogradContext* ctx, const Tensor& q1, const Tensor& k1, const Tensor& q2, const Tensor& k2, double init, bool held) {
+    ctx->saved_data["leaves"] = held || default_stream_leaves({&q1, &k1, &q2, &k2});
     ctx->save_for_backward({q1, k1, q2, k2});
     return lambda_call(q1, k1, q2, k2, init);
   }
@@ -267,7 +267,7 @@ struct LambdaNode : torch::autograd::Function<LambdaNode> {
     capturable(ctx, "diff_lambda");
     const auto s = ctx->get_saved_variables();
     c10::DeviceGuard guard(s[0].device());
-    variable_list out{like(s[0]), like(s[0]), like(s[0]), like(s[0]), Tensor()};
+    variable_list out{like(s[0]), like(s[0]), like(s[0]), like(s[0]), Tensor(), Tensor()};
     const Tensor up = g[0].contiguous();
     status(L.lambda_bwd(f(up), f(s[0]), f(s[1]), f(s[2]), f(s[3]), s[0].size(0), s[0].size(1), f(out[0]), f(out[1]), f(out[2]), f(out[3]), stream_of(s[0])),
            "rt_diff_lambda_bwd", false);
@@ -281,7 +281,8 @@ Tensor diff_lambda(const Tensor& q1_in, const Tensor& k1_in, const Tensor& q2_in
   if (q1_in.size(0) > MOST || q1_in.size(1) > MOST) raise(PyExc_NotImplementedError, "diff_lambda: at most 2^31 - 1 heads and columns, got " + shape(q1_in));
   const Tensor q1 = q1_in.contiguous(), k1 = vec(k1_in, q1_in.sizes(), q1_in, "diff_lambda"), q2 = vec(q2_in, q1_in.sizes(), q1_in, "diff_lambda"),
                k2 = vec(k2_in, q1_in.sizes(), q1_in, "diff_lambda");
-  return on_tape({&q1, &k1, &q2, &k2}) ? LambdaNode::apply(q1, k1, q2, k2, init) : lambda_call(q1, k1, q2, k2, init);
+  if (on_tape({&q1, &k1, &q2, &k2})) return LambdaNode::apply(q1, k1, q2, k2, init, default_stream_leaves({&q1_in, &k1_in, &q2_in, &k2_in}));
+  return lambda_call(q1, k1, q2, k2, init);
 }
 
 // ---- differential attention -----------------------------------------------------------------------------------------------------------------
@@ -306,12 +307,12 @@ Tensor attention_call(const Tensor& q, const Tensor& k, const Tensor& v, const T
 }
 struct AttentionNode : torch::autograd::Function<AttentionNode> {
   static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& lam, const OptTensor& w_opt, const OptTensor& cu_q_opt,
-                        const OptTensor& cu_k_opt, const OptTensor& ids_opt, std::vector<int64_t> sizes, double scale, double out_scale, double eps) {
+                        const OptTensor& cu_k_opt, const OptTensor& ids_opt, std::vector<int64_t> sizes, double scale, double out_scale, double eps, bool held) {
     const AttnMeta m{sizes[0], sizes[1], sizes[2], sizes[3], sizes[4], sizes[5], sizes[6], scale, out_scale, eps};
     const Tensor w = got(w_opt), cu_q = got(cu_q_opt), cu_k = got(cu_k_opt), ids = got(ids_opt);
     Tensor saved;
     const Tensor y = attention_call(q, k, v, lam, cu_q, cu_k, ids, w, m, &saved);
-    ctx->saved_data["leaves"] = default_stream_leaves({&q, &k, &v, &lam, &w});
+    ctx->saved_data["leaves"] = held || default_stream_leaves({&q, &k, &v, &lam, &w});
     ctx->save_for_backward({lam, w, cu_q, cu_k, ids, saved});      // (not q, k, v: their planes are in `saved`)
     sizes.push_back(q.size(0));
     sizes.push_back(k.size(0));
@@ -329,7 +330,7 @@ struct AttentionNode : torch::autograd::Function<AttentionNode> {
     c10::DeviceGuard guard(lam.device());
     const Tensor dy = dense_rows(g[0]);
     const int64_t H = z[1], Hkv = z[2], hd = z[3], Nq = z[7], Nk = z[8];
-    variable_list out(12);
+    variable_list out(13);
     out[0] = at::empty({Nq, 2 * H * hd}, lam.options());
     out[1] = at::empty({Nk, 2 * Hkv * hd}, lam.options());
     out[2] = at::empty({Nk, 2 * Hkv * hd}, lam.options());
@@ -368,7 +369,8 @@ Tensor diff_attention(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in
   if (w.defined()) check_eps(eps, what);
   const AttnMeta m{B, H, Hkv, hd, Lq, Lk, causal, scale.value_or(0.0), out_scale, eps};
   if (on_tape({&q, &k, &v, &lam, &w}))
-    return AttentionNode::apply(q, k, v, lam, opt(w), opt(cu_q), opt(cu_k), opt(ids), std::vector<int64_t>{B, H, Hkv, hd, Lq, Lk, causal}, m.scale, out_scale, eps);
+    return AttentionNode::apply(q, k, v, lam, opt(w), opt(cu_q), opt(cu_k), opt(ids), std::vector<int64_t>{B, H, Hkv, hd, Lq, Lk, causal}, m.scale, out_scale, eps,
+                                default_stream_leaves({&q_in, &k_in, &v_in, &lam_in, &w_any}));
   return attention_call(q, k, v, lam, cu_q, cu_k, ids, w, m, nullptr);
 }
 
@@ -387,11 +389,12 @@ variable_list norm_call(const Tensor& x, const Tensor& b, const Tensor& z, const
 }
 struct NormNode : torch::autograd::Function<NormNode> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& b, const OptTensor& z_opt, const OptTensor& sc_opt, const OptTensor& pw_opt,
-                               const OptTensor& pb_opt, const OptTensor& nw_opt, const OptTensor& nb_opt, bool layer, double alpha, double eps, double p, int64_t seed, int64_t sid) {
+                               const OptTensor& pb_opt, const OptTensor& nw_opt, const OptTensor& nb_opt, bool layer, double alpha, double eps, double p, int64_t seed, int64_t sid,
+                               bool held) {
     const Tensor z = got(z_opt), sc = got(sc_opt), pw = got(pw_opt), pb = got(pb_opt), nw = got(nw_opt), nb = got(nb_opt);
     Tensor stat;
     variable_list out = norm_call(x, b, z, sc, pw, pb, nw, nb, {layer, alpha, eps, p, (uint64_t)seed, (uint64_t)sid}, &stat);
-    ctx->saved_data["leaves"] = default_stream_leaves({&x, &b, &z, &sc, &pw, &pb, &nw, &nb});
+    ctx->saved_data["leaves"] = held || default_stream_leaves({&x, &b, &z, &sc, &pw, &pb, &nw, &nb});
     ctx->save_for_backward({nw.defined() ? out[0] : Tensor(), b, z, sc, pw, pb, nw, stat});
     ctx->saved_data["i"] = std::vector<int64_t>{layer, seed, sid, nb.defined()};
     ctx->saved_data["f"] = std::vector<double>{alpha, p};
@@ -401,7 +404,7 @@ struct NormNode : torch::autograd::Function<NormNode> {
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     once("norm_gate_residual");
     capturable(ctx, "norm_gate_residual");
-    variable_list out(14);
+    variable_list out(15);
     Tensor gy = g[0].defined() ? g[0].contiguous() : Tensor(), gh = g.size() > 1 && g[1].defined() ? g[1].contiguous() : Tensor();
     if (!gy.defined() && !gh.defined()) return out;
     const auto s = ctx->get_saved_variables();
@@ -429,11 +432,9 @@ struct NormNode : torch::autograd::Function<NormNode> {
 std::vector<Tensor> norm_gate(const Tensor& x_in, const Tensor& f_in, const OptTensor& z_in, const OptTensor& sc_in, const OptTensor& pw_in, const OptTensor& pb_in,
                               const OptTensor& nw_in, const OptTensor& nb_in, bool layer, double alpha, double eps, double p, uint64_t seed, uint64_t sid) {
   const char* what = "norm_gate_residual";
-  for (const OptTensor* t : {&z_in, &sc_in, &pw_in, &pb_in, &nw_in, &nb_in}) {
-    const Tensor any = got(*t);
-    no_tangent(what, {&any});
-  }
-  no_tangent(what, {&x_in, &f_in});
+  const Tensor z_any = got(z_in), sc_any = got(sc_in), pw_any = got(pw_in), pb_any = got(pb_in), nw_any = got(nw_in), nb_any = got(nb_in);
+  const std::initializer_list<const Tensor*> given{&x_in, &f_in, &z_any, &sc_any, &pw_any, &pb_any, &nw_any, &nb_any};
+  no_tangent(what, given);
   check_f32(x_in, what);
   if (x_in.dim() != 2 || x_in.size(1) == 0) bad(what, "expected [rows, columns], got " + shape(x_in));
   const int64_t d = x_in.size(1);
@@ -441,7 +442,8 @@ std::vector<Tensor> norm_gate(const Tensor& x_in, const Tensor& f_in, const OptT
   const Tensor x = x_in.contiguous(), b = vec(f_in, x_in.sizes(), x_in, what), z = vec(z_in, x_in.sizes(), x_in, what), sc = vec(sc_in, {d}, x_in, what),
                pw = vec(pw_in, {d}, x_in, what), pb = vec(pb_in, {d}, x_in, what), nw = vec(nw_in, {d}, x_in, what), nb = vec(nb_in, {d}, x_in, what);
   check_eps(eps, what);
-  if (on_tape({&x, &b, &z, &sc, &pw, &pb, &nw, &nb})) return NormNode::apply(x, b, opt(z), opt(sc), opt(pw), opt(pb), opt(nw), opt(nb), layer, alpha, eps, p, (int64_t)seed, (int64_t)sid);
+  if (on_tape({&x, &b, &z, &sc, &pw, &pb, &nw, &nb})) return NormNode::apply(x, b, opt(z), opt(sc), opt(pw), opt(pb), opt(nw), opt(nb), layer, alpha, eps, p, (int64_t)seed, (int64_t)sid,
+                                                                            default_stream_leaves(given));
   return norm_call(x, b, z, sc, pw, pb, nw, nb, {layer, alpha, eps, p, seed, sid}, nullptr);
 }
 
