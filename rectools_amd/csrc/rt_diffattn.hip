@@ -9,9 +9,12 @@
 //
 // Arithmetic: fp32 in, fp32 out.  A product runs on the fp16 matrix instruction as three terms of a two-way split: x = 2^e (h + l), e from the
 // largest magnitude of the row, h = fp16(x 2^-e), l = fp16 of the rest; x y ~ h h' + h l' + l h'.  h and l hold 11 bits each and a sign, so x
-// is held to 2^-23 of itself (values below 2^-17 of their row's largest: to 2^-38 of that) and the dropped l l' is below 2^-22 of the product: roundings
-// of the size that fp32 sums of this length carry themselves — over 150 drawn training calls the error against 64 bits is 0.9 x that of the same
-// formulas in fp32 tensors (median; outputs, dq, dk, dv).  Three bf16 planes, the exact split, take six terms: two sessions of 4,096 rows, 4 heads of hd 64,
+// is held to 2^-23 of itself (values below 2^-17 of their row's largest: to 2^-38 of that) and the dropped l l' is below 2^-22 of the product: 8 u of a
+// product (u = 2^-24) where fp32 takes u, and sums over many of them come out as near as those of fp32 tensors: over 150 drawn training calls the error
+// against 64 bits is 0.85 x theirs (median; outputs, dq, dk, dv; 90 % below 1.25), with 85 % of the queries without a gradient, the others' at 1e-6, and half of
+// the value rows zero 0.9 - 1.15 x (90 % below 1.55).  Where a result is what is left of a few products that cancel (a row whose maps nearly cancel; dlam of
+// one head, p90 2.4 x) the 8 u show.  Weights are split with one unit per lane, not per row: their bits last because every row's planes have one
+// size and rows of zeros the least exponent (row_exp).  Three bf16 planes, the exact split, take six terms: two sessions of 4,096 rows, 4 heads of hd 64,
 // forward and backward 1,840 us with them, 1,100 with these.
 // The split is made ONCE per call by diff_planes_kernel (one pass over q, k, v: memory bound), not at every staging: a 4,096-row session
 // stages each of its rows 64 times.  Softmax statistics, sums and accumulators are fp32; scores live in the base-2 domain.
@@ -24,8 +27,8 @@
 // rows lie 3 sixteen-byte units apart modulo the 256 bytes of the banks: 32 rows of 16 bytes without a conflict, 4-row transpose blocks two-way (with 16
 // bytes behind them: four-way, 192 conflict cycles per wave and chunk of the forward pass).
 //
-// What bounds it (two sessions of 4,096, 4 heads of hd 64, causal): forward 215 us, backward 510 us.  Least matrix work, three terms each, at the rate a large
-// 16-bit matrix product reaches on this card (1,385 TFLOP/s): 112 and 260 us.  Counters: the matrix pipe is busy 36 - 38 % of the time, the vector
+// What bounds it (two sessions of 4,096, 4 heads of hd 64, causal): forward 193 us, backward 466 us (on a card that has worked for 100 ms; 217 and 518 in
+// the first passes behind a pause).  Least matrix work, three terms each, at the rate a large 16-bit matrix product reaches on this card (1,385 TFLOP/s): 112 and 260 us.  Counters: the matrix pipe is busy 36 - 38 % of the time, the vector
 // pipe 43 % (exponentials, scales, splits), and the two waves of a SIMD overlap them little; two waves are what 256 registers each leave.
 #include "rt_attn_planes.h"
 
@@ -665,7 +668,7 @@ __global__ __launch_bounds__(NT) void diff_combine_kernel(Args a) {
 // HD / 2 lanes per (row, head), four columns each; a lane group keeps its head, so dlam and dw stay in registers over all of its rows.  They
 // are summed in 64 bits, per workgroup, in a fixed order.  do stands at right angles to o (but for eps) and do . o_m is what is left of that: formed in
 // 64 bits, from the outputs as they are (in 32 the gradient of lam was 2 - 5 x further off; 15.5 -> 17 us).  Memory bound: 8,192 rows of 4 heads of hd 64,
-// 70 MB, 18 us = 3.9 TB/s.
+// 70 MB, 17 us = 4.1 TB/s.
 //
 // A row that sees ONE key has that key's values for both maps' outputs, whatever the logits are: dO stands at right angles to them but for eps, and the
 // row's share of dlam, 1e-5 of its terms, would be the two outputs' own roundings (sessions of one row: 0.3 to 3 % off).  o_2 is o_1 there.  Which rows
@@ -1091,8 +1094,8 @@ __device__ __forceinline__ void bwd_dkv(const Args& a, unsigned char* smem, int 
 }
 
 // Both passes in one launch, the dK/dV workgroups (one and a half times the work of the others) first: they share no data, and each alone ends with
-// a few of its longest workgroups on an empty machine.  Two sessions of 4,096, 4 heads of hd 64, causal: 510 us = 3.6e11 flops (three terms a product) at
-// 710 TFLOP/s; one launch after the other 309 + 445 us before the later steps, together 562.  The column sums of dlam and dw ride along between the two.
+// a few of its longest workgroups on an empty machine.  Two sessions of 4,096, 4 heads of hd 64, causal: 466 us = 3.6e11 flops (three terms a product) at
+// 775 TFLOP/s; one launch after the other 309 + 445 us before the later steps, together 562.  The column sums of dlam and dw ride along between the two.
 template <int HD>
 __global__ __launch_bounds__(NT, 2) void diff_bwd_kernel(Args a, Sums m) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];

@@ -9,8 +9,10 @@
 // row stays in the registers of its threads (16 to 1,024 of them, at most 8 columns each), statistics are two-pass over those
 // registers.  The column sums behind the parameters' gradients stay in registers over all rows of a workgroup, are written once per
 // workgroup and joined by a second launch in a fixed order: no atomics, the same bits every run.  16,384 rows of 2,048, every part: forward
-// 136 us = 4.9 TB/s, backward 197 us = 5.4 TB/s, joining 11 us; 25,600 rows of 256: 26 us = 5.0 TB/s, 40 us, 5 us; 40,001 rows of 50 (pairs of
-// columns: no wider load divides the row): 12.4, 22.6 and 4.6 us (3.2 and 2.8 TB/s).
+// 136 us = 4.9 TB/s, backward 197 us = 5.4 TB/s, joining 11 us; 25,600 rows of 256: 25 us = 5.2 TB/s, 38 us, 5 us; 40,001 rows of 50: 12.2, 22.1 and 4.5 us (3.3
+// and 2.9 TB/s): accesses of 8 bytes, a pair of columns each, and 14 of a row's 64 column slots idle.  Two such rows are 400 bytes, 25 loads of 16; a flat stream of a
+// workgroup's rows through LDS has not been tried.  Dropout hashes once per element, where one hash holds the bits of four: p = 0.2 against 0, 25,600 rows of 256
+// 28.6 | 25.8 us forward, 37.1 | 34.4 backward; 16,384 of 2,048 150 | 143 and 185 | 172.
 #include "rt_common.h"
 
 namespace {
