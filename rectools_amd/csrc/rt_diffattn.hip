@@ -794,8 +794,9 @@ __device__ __forceinline__ void bwd_sums(const Args& a, const Sums& m, int blk) 
 }
 
 // dS = p (G - delta), delta the row's mean of G under p.  delta comes from the outputs (do . o: rows as long as one likes, one number), which is off by
-// the rounding of o; where one key holds nearly all of the weight G - delta cancels down to that.  Rows that see 32 keys at most — a session's
-// first rows, short sessions — take the mean of the very G - delta in a second step: a row with one key has a gradient of exactly zero.
+// the rounding of o; where one key holds nearly all of the weight G - delta cancels down to that.  Rows with 32 keys at most up to their last
+// visible one — a session's first rows, short sessions — take the mean of the very G - delta in a second step: a row with one key has a gradient of exactly zero.
+// (A mask that leaves one key of a longer session does not: dS is rounding there, 1e-7 of |do| |v|.)
 // ---- backward, dQ: the owner is a query; both maps need G^T = V dO^T, each wave makes it over half of V's columns and they swap halves ------
 // STAGES: two where two workgroups with two chunk buffers fit a CU's LDS (HD 32; training passes with two | with one: 128 sessions of 200 285 | 290 us,
 // 16 of 2,048 1,021 | 1,028), else one: the other workgroup's products run under the copy.
